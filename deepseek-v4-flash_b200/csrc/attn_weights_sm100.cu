@@ -1,0 +1,428 @@
+// attn_weights_sm100.cu -- the attention weight every cached token received,
+// summed over the query tokens and heads of a step (what decides which tokens a
+// bounded cache keeps).  No counterpart in the reference.
+//
+//   w[p] = sum over the rows r = (token t, head) that see p of
+//          e^(scale * q[r] . k[p] - lse[r])
+// with the log-sum-exps of the attention that ran before: the scores are made
+// again (2 d FLOP per row and token) rather than kept by the attention, whose
+// running maximum is not final while it has them, and whose fp32 scores would
+// be 512 bytes a token and 128 rows against the 1152 bytes of reading K again.
+//
+// The tokens are the MMAs' M (128 per CTA pair, a 64-token block per CTA) and
+// up to 256 query rows the N, resident in shared memory while K streams past
+// in 24 KB boxes: a token is one TMEM lane (its rows along the columns, half of
+// them in lane + 64), so its sum needs no shuffles, one thread adds it up in
+// registers and one thread owns the result: no atomics, the same bits each
+// time.  A sequence with more rows than a group leaves one partial sum per
+// group and token (4 bytes against the 2 d bytes of its K row), added in group
+// order by weights_combine.  At 128 rows or fewer a token costs 1152 bytes of
+// HBM and less of everything else; with more, the MMAs (2304 cycles for 64
+// tokens x 256 rows a CTA at full rate) and the exponentials (1024 cycles of
+// the MUFU) bound it.
+//
+// Schedule: tree_plan.cuh.  256 threads at most: warp 0 TMA producer, warp 1
+// TMEM allocator and MMA issuer (pair leader), warps 2-5 the epilogue.
+// Every wait is bounded; a timeout raises QCAU_DEVERR_TIMEOUT, drains the
+// copies in flight, frees TMEM and returns.
+#include "common.cuh"
+#include "kernels.h"
+#include "tree_plan.cuh"
+
+namespace qcau {
+namespace {
+
+constexpr int kThreads = 192;
+constexpr int kKSlot = 24576;  // 64 tokens x 3 chunks of 64 dims
+constexpr int kBoxes = 3;      // boxes of a tile: 9 chunks (8: the last box ends in zeros)
+constexpr float kLog2e = 1.4426950408889634f;
+
+// N rows of a group (64, 128 or 256): half of them in each CTA's shared memory.
+template <int N>
+struct WeightsCfg {
+  static constexpr int kQChunk = N / 2 * 128;  // N/2 rows x 64 dims bf16
+  static constexpr int kSlots = N == 256 ? 3 : N == 128 ? 6 : 7;
+  static constexpr uint32_t kTmemCols = N;  // 2 buffers x N/2 columns
+};
+
+template <int N>
+struct WeightsShared {
+  uint64_t kfull[WeightsCfg<N>::kSlots], kempty[WeightsCfg<N>::kSlots];
+  uint64_t q_full, q_empty;
+  uint64_t s_full[2], s_free[2];
+  uint64_t xbar[2][4];  // halves of a token's sum handed over: 2 warp pairs x 4 buffers
+  float xsum[4][64];
+  float neg[4][N / 2];  // per epilogue warp: -lse * log2e of its columns
+  uint32_t tmem_base;
+  int abort;
+  TreePlanShared plan;
+};
+
+template <int N>
+constexpr size_t weights_smem() {
+  using C = WeightsCfg<N>;
+  return 1024 + 9 * (size_t)C::kQChunk + (size_t)C::kSlots * kKSlot + sizeof(WeightsShared<N>);
+}
+static_assert(weights_smem<256>() <= 232448 && weights_smem<128>() <= 232448 &&
+                  weights_smem<64>() <= 232448,
+              "shared memory budget");
+
+struct WeightsParams {
+  TreeShape sh;      // groups of N rows
+  const float* lse;  // [b, s, h]
+  float* sums;       // [b, sums_stride]
+  float* part;       // [groups][b][part_stride] when groups > 1
+  int64_t sums_stride, part_stride;
+  int accumulate, chunks;
+  float scale;
+};
+
+template <int N>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
+    attn_weights_sm100_kernel(const __grid_constant__ CUtensorMap tm_q,
+                              const __grid_constant__ CUtensorMap tm_k, WeightsParams p) {
+  using C = WeightsCfg<N>;
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t pad = (1024u - (smem_u32(smem_raw) & 1023u)) & 1023u;
+  uint8_t* sQ = smem_raw + pad;
+  uint8_t* sK = sQ + 9 * C::kQChunk;
+  WeightsShared<N>* sh = reinterpret_cast<WeightsShared<N>*>(sK + (size_t)C::kSlots * kKSlot);
+  volatile int* abort = &sh->abort;
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = cluster_ctarank();
+  const bool leader = rank == 0;
+  const int pair = blockIdx.x >> 1, npairs = gridDim.x >> 1;
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < C::kSlots; i++) {
+      mbar_init(&sh->kfull[i], 1);
+      mbar_init(&sh->kempty[i], 1);
+    }
+    mbar_init(&sh->q_full, 1);
+    mbar_init(&sh->q_empty, 1);
+    for (int i = 0; i < 2; i++) {
+      mbar_init(&sh->s_full[i], 1);
+      mbar_init(&sh->s_free[i], 8);
+      for (int k = 0; k < 4; k++) mbar_init(&sh->xbar[i][k], 1);
+    }
+    sh->abort = 0;
+    fence_barrier_init();
+  }
+  tree_plan_sums(p.sh, &sh->plan);
+  if (warp == 1) tmem_alloc<2>(&sh->tmem_base, C::kTmemCols);
+  tc_fence_before();
+  cluster_sync();
+  tc_fence_after();
+  const uint32_t tmem = sh->tmem_base;
+  const TreeRange range = tree_plan_range(p.sh, &sh->plan, pair, npairs);
+  cudaTriggerProgrammaticLaunchCompletion();
+
+  if (warp == 0) {
+    // ------------------------------------------------ producer (both CTAs)
+    if (lane == 0) {
+      int last_use[C::kSlots];
+      for (int i = 0; i < C::kSlots; i++) last_use[i] = -1;
+      const uint32_t q_full_l = mapa_shared(smem_u32(&sh->q_full), 0);
+      int n = 0, nq = 0;  // boxes issued; pieces whose Q was issued
+      bool ok = true;
+      TreeCursor c = range.start;
+      TreePiece u;
+      while (ok && tree_piece(p.sh, c, u)) {
+        if (nq > 0 && !(ok = mbar_wait(&sh->q_empty, (nq - 1) & 1, abort))) break;
+        if (leader) mbar_arrive_expect_tx(&sh->q_full, 2 * p.chunks * C::kQChunk);
+        for (int k = 0; k < p.chunks; k++)  // rows past the sequence's are zero-filled
+          tma_load_3d_pair(sQ + k * C::kQChunk, &tm_q, q_full_l, 64 * k,
+                           u.g * N + N / 2 * (int)rank, u.b);
+        nq++;
+        for (int t = u.t_begin; t < u.t_end && ok; t++) {
+          const int blk = tree_block(p.sh, u, 2 * t + (int)rank);
+          for (int i = 0; i < kBoxes; i++, n++) {
+            const int slot = n % C::kSlots, use = n / C::kSlots;
+            if (!(ok = mbar_wait(&sh->kempty[slot], (use & 1) ^ 1, abort))) break;
+            if (leader) mbar_arrive_expect_tx(&sh->kfull[slot], 2 * kKSlot);
+            last_use[slot] = use;
+            tma_load_4d_pair(sK + (size_t)slot * kKSlot, &tm_k,
+                             mapa_shared(smem_u32(&sh->kfull[slot]), 0), 0, 0, 3 * i, blk);
+          }
+        }
+      }
+      if (*abort && leader) {
+        // the leader's full barriers count both CTAs' copies: drain them all
+        volatile int never = 0;
+        if (nq > 0) mbar_wait<true>(&sh->q_full, (nq - 1) & 1, &never);
+        for (int i = 0; i < C::kSlots; i++)
+          if (last_use[i] >= 0) mbar_wait<true>(&sh->kfull[i], last_use[i] & 1, &never);
+      }
+    }
+  } else if (warp == 1) {
+    // ------------------------------------------------ MMA issuer (pair leader)
+    if (leader && lane == 0) {
+      const uint32_t idesc = make_idesc(128, N, kFmtBF16, kFmtBF16, false, false);
+      const uint64_t k_desc = make_sdesc(smem_u32(sK), 16, 1024);
+      const uint64_t q_desc = make_sdesc(smem_u32(sQ), 16, 1024);
+      int n = 0, gt = 0, nu = 0;  // boxes, tiles, pieces
+      uint64_t* last_bar = nullptr;
+      int last_phase = 0;
+      bool ok = true;
+      TreeCursor c = range.start;
+      TreePiece u;
+      while (ok && tree_piece(p.sh, c, u)) {
+        if (!(ok = mbar_wait(&sh->q_full, nu & 1, abort))) break;
+        for (int t = u.t_begin; t < u.t_end && ok; t++, gt++) {
+          const int sb = gt & 1;
+          if (gt >= 2 && !(ok = mbar_wait<true>(&sh->s_free[sb], ((gt >> 1) - 1) & 1, abort)))
+            break;
+          tc_fence_after();
+          for (int g = 0; g < kBoxes; g++, n++) {
+            const int slot = n % C::kSlots, use = n / C::kSlots;
+            if (!(ok = mbar_wait(&sh->kfull[slot], use & 1, abort))) break;
+            // chunk 3g + i: A = this CTA's 64 tokens, B = its N/2 query rows
+            const uint64_t kg = k_desc + (uint64_t)((slot * kKSlot) >> 4);
+            const uint64_t qg = q_desc + (uint64_t)((3 * g * C::kQChunk) >> 4);
+#pragma unroll
+            for (int i = 0; i < 3; i++) {
+              if (3 * g + i >= p.chunks) break;
+#pragma unroll
+              for (int kk = 0; kk < 4; kk++)
+                mma_bf16_pair(tmem + sb * (N / 2), kg + (uint64_t)((i * 8192 + kk * 32) >> 4),
+                              qg + (uint64_t)((i * C::kQChunk + kk * 32) >> 4), idesc,
+                              (g | i | kk) != 0 ? 1u : 0u);
+            }
+            tc_commit_pair(&sh->kempty[slot], 3);
+            last_bar = &sh->kempty[slot];
+            last_phase = use & 1;
+          }
+          if (ok) {
+            tc_commit_pair(&sh->s_full[sb], 3);
+            last_bar = &sh->s_full[sb];
+            last_phase = (gt >> 1) & 1;
+          }
+        }
+        if (ok) tc_commit_pair(&sh->q_empty, 3);
+        nu++;
+      }
+      if (*abort && last_bar != nullptr) {
+        // the MMAs issued so far finish before TMEM and the slots go away
+        volatile int never = 0;
+        mbar_wait<true>(last_bar, last_phase, &never);
+      }
+    }
+  } else {
+    // ------------------------------------------------ epilogue (warps 2-5)
+    const int quarter = warp & 3;
+    const int row = quarter * 32 + lane;  // TMEM lane
+    const int hl = row & 63, half = row >> 6;
+    const int et = threadIdx.x - 64;
+    const uint32_t lane_base = (uint32_t)(quarter * 32) << 16;
+    const float sl2 = p.scale * kLog2e;
+    const uint32_t s_free_l[2] = {mapa_shared(smem_u32(&sh->s_free[0]), 0),
+                                  mapa_shared(smem_u32(&sh->s_free[1]), 0)};
+    const int64_t seq_rows = (int64_t)p.sh.s * p.sh.h;
+    float* neg = sh->neg[warp - 2];
+
+    // positions that no token of the step can see: zero, unless sums are added to
+    if (!p.accumulate)
+      for (int b = blockIdx.x; b < p.sh.b; b += gridDim.x) {
+        const TreeSeq q = tree_seq(p.sh, b);
+        for (int i = (q.n > 0 ? q.len : 0) + et; i < p.sh.max_len; i += 128)
+          p.sums[b * p.sums_stride + i] = 0.f;
+      }
+
+    int gt = 0;
+    bool ok = true;
+    TreeCursor c = range.start;
+    TreePiece u;
+    while (ok && tree_piece(p.sh, c, u)) {
+      const int base = u.q.len - u.q.n;
+      const int col0 = u.g * N + half * (N / 2);  // first row of this thread's columns
+      const int ncol = min(max(u.q.n * p.sh.h - col0, 0), N / 2);
+      __syncwarp();
+      for (int i = lane; i < N / 2; i += 32)
+        neg[i] = i < ncol ? -kLog2e * p.lse[u.b * seq_rows + col0 + i] : 0.f;
+      __syncwarp();
+      const uint8_t* mask = p.sh.mask ? p.sh.mask + u.b * p.sh.mask_stride : nullptr;
+      const bool direct = u.q.groups == 1;
+      float* out = direct ? p.sums + u.b * p.sums_stride
+                          : p.part + ((int64_t)u.g * p.sh.b + u.b) * p.part_stride;
+      for (int t = u.t_begin; t < u.t_end && ok; t++, gt++) {
+        const int sb = gt & 1, xb = gt & 3;
+        const int tok = t * kTreeTile + (int)rank * 64 + hl;
+        // columns (rows of the sequence) that see this token
+        const bool full = t * kTreeTile + (int)rank * 64 + 64 <= base && ncol == N / 2;
+        uint32_t bits[N / 64];
+        if (!full) {
+#pragma unroll
+          for (int k = 0; k < N / 64; k++) bits[k] = 0;
+          auto set = [&](int c0, int c1) {  // columns [c0, c1)
+#pragma unroll
+            for (int k = 0; k < N / 64; k++) {
+              const int lo = max(c0 - 32 * k, 0), hi = min(c1 - 32 * k, 32);
+              if (lo < hi) bits[k] |= (hi - lo == 32 ? 0xffffffffu : ((1u << (hi - lo)) - 1u) << lo);
+            }
+          };
+          if (tok < base) {
+            set(0, ncol);
+          } else if (tok < u.q.len && ncol > 0) {
+            const int j = tok - base, t_end = (col0 + ncol - 1) / p.sh.h;
+#pragma unroll 8
+            for (int node = col0 / p.sh.h; node <= t_end; node++) {
+              const bool sees = mask ? mask[(int64_t)node * p.sh.s + j] != 0 : j <= node;
+              if (sees) set(max(node * p.sh.h - col0, 0), min((node + 1) * p.sh.h - col0, ncol));
+            }
+          }
+        }
+        if (!(ok = tree_warp_wait(&sh->s_full[sb], (gt >> 1) & 1, abort))) break;
+        tc_fence_after();
+        const uint32_t s_addr = tmem + lane_base + sb * (N / 2);
+        const uint64_t sc2 = f2_pack(sl2, sl2);
+        uint64_t acc[4];
+#pragma unroll
+        for (int k = 0; k < 4; k++) acc[k] = f2_pack(0.f, 0.f);
+#pragma unroll
+        for (int k = 0; k < N / 64; k++) {
+          float v[32];
+          tmem_ld32(s_addr + 32 * k, v);
+          tmem_ld_wait_regs(v);
+          if (k == N / 64 - 1) {  // all scores are read: the S buffer is free
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive_remote(s_free_l[sb]);
+          }
+          const ulonglong2* n2 = reinterpret_cast<const ulonglong2*>(neg + 32 * k);
+#pragma unroll
+          for (int i = 0; i < 8; i++) {
+            const ulonglong2 ng = n2[i];
+            float x0, x1, x2, x3;
+            f2_unpack(f2_fma(f2_pack(v[4 * i], v[4 * i + 1]), sc2, ng.x), x0, x1);
+            f2_unpack(f2_fma(f2_pack(v[4 * i + 2], v[4 * i + 3]), sc2, ng.y), x2, x3);
+            float p0 = ex2_approx(x0), p1 = ex2_approx(x1);
+            float p2 = ex2_approx(x2), p3 = ex2_approx(x3);
+            if (!full) {  // a selection, not a product: unseen scores may be NaN
+              const uint32_t m = bits[k] >> (4 * i);
+              p0 = m & 1u ? p0 : 0.f;
+              p1 = m & 2u ? p1 : 0.f;
+              p2 = m & 4u ? p2 : 0.f;
+              p3 = m & 8u ? p3 : 0.f;
+            }
+            acc[(2 * i) & 3] = f2_add(acc[(2 * i) & 3], f2_pack(p0, p1));
+            acc[(2 * i + 1) & 3] = f2_add(acc[(2 * i + 1) & 3], f2_pack(p2, p3));
+          }
+        }
+        float a0, a1;
+        f2_unpack(f2_add(f2_add(acc[0], acc[1]), f2_add(acc[2], acc[3])), a0, a1);
+        float w = a0 + a1;
+        // the token's other half of the columns.  Buffer xb is written again
+        // four tiles on, after an s_full that needs this warp pair's reader to
+        // have released S two tiles later than this one
+        if (half == 1) {
+          sh->xsum[xb][hl] = w;
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&sh->xbar[quarter & 1][xb]);
+        } else {
+          if (!(ok = tree_warp_wait(&sh->xbar[quarter & 1][xb], (gt >> 2) & 1, abort))) break;
+          w += sh->xsum[xb][hl];
+          if (tok < u.q.len) out[tok] = direct && p.accumulate ? out[tok] + w : w;
+        }
+      }
+    }
+  }
+
+  __syncwarp();
+  tc_fence_before();
+  cluster_sync();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc<2>(tmem, C::kTmemCols);
+  }
+  if (threadIdx.x == 0 && *abort) raise_dev_error(p.sh.err, QCAU_DEVERR_TIMEOUT);
+}
+
+// The groups' partial sums of a token, in group order.
+__global__ void __launch_bounds__(256) weights_combine_kernel(WeightsParams p) {
+  cudaGridDependencySynchronize();
+  const int b = blockIdx.y, tok = blockIdx.x * 256 + threadIdx.x;
+  const TreeSeq q = tree_seq(p.sh, b);
+  if (q.groups < 2 || tok >= q.len) return;
+  float w = 0.f;
+#pragma unroll 8
+  for (int g = 0; g < q.groups; g++) w += p.part[((int64_t)g * p.sh.b + b) * p.part_stride + tok];
+  float* out = p.sums + b * p.sums_stride + tok;
+  *out = p.accumulate ? *out + w : w;
+}
+
+// Rows of a group: all the rows in one group up to 256, so that K is read once.
+int weights_group(const TreeArgs& a) {
+  const int64_t rows = a.s * a.h;
+  return rows <= 64 ? 64 : rows <= 128 ? 128 : 256;
+}
+
+template <int N>
+cudaError_t run_weights(const TreeArgs& a, const WeightsParams& p, const CUtensorMap& tq,
+                        const CUtensorMap& tk, int64_t pairs, cudaStream_t st) {
+  cudaError_t e = cudaFuncSetAttribute(attn_weights_sm100_kernel<N>,
+                                       cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                       (int)weights_smem<N>());
+  if (e != cudaSuccess) return e;
+  attn_weights_sm100_kernel<N><<<(unsigned)(2 * pairs), kThreads, weights_smem<N>(), st>>>(tq, tk, p);
+  return cudaGetLastError();
+}
+
+}  // namespace
+
+size_t attn_weights_workspace(const TreeArgs& a) {
+  const int n = weights_group(a);
+  const int64_t groups = (a.s * a.h + n - 1) / n;
+  return groups > 1 ? (size_t)groups * a.b * ((a.max_len + 3) / 4 * 4) * 4 : 0;
+}
+
+cudaError_t launch_attn_weights_sm100(const TreeArgs& a, void* ws, cudaStream_t st) {
+  const int n = weights_group(a);
+  const int64_t rows = a.s * a.h, pairs = tree_pairs(a, n);
+  CUtensorMap tq, tk;
+  {
+    const uint64_t dims[3] = {(uint64_t)a.d_qk, (uint64_t)rows, (uint64_t)a.b};
+    const uint64_t strides[2] = {(uint64_t)a.d_qk * 2, (uint64_t)(rows * a.d_qk) * 2};
+    const uint32_t box[3] = {64, (uint32_t)n / 2, 1};
+    if (!make_tmap(&tq, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, a.q, dims, strides, box,
+                   CU_TENSOR_MAP_SWIZZLE_128B))
+      return cudaErrorInvalidValue;
+  }
+  {
+    // the cache as [64-token blocks][64 tokens][chunks][64 values]
+    const uint64_t dims[4] = {64, 64, (uint64_t)(a.d_qk / 64),
+                              (uint64_t)(a.num_pages * (a.page_size / 64))};
+    const uint64_t strides[3] = {(uint64_t)a.d_qk * 2, 128, (uint64_t)a.d_qk * 128};
+    const uint32_t box[4] = {64, 64, 3, 1};
+    if (!make_tmap(&tk, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, a.cache, dims, strides, box,
+                   CU_TENSOR_MAP_SWIZZLE_128B))
+      return cudaErrorInvalidValue;
+  }
+  WeightsParams p{};
+  p.sh = tree_shape(a, n, pairs);
+  p.lse = a.lse;
+  p.sums = a.sums;
+  p.sums_stride = a.sums_stride;
+  p.part = reinterpret_cast<float*>(ws);
+  p.part_stride = (a.max_len + 3) / 4 * 4;
+  p.accumulate = a.accumulate;
+  p.chunks = (int)(a.d_qk / 64);
+  p.scale = a.scale;
+  cudaError_t e = n == 256   ? run_weights<256>(a, p, tq, tk, pairs, st)
+                  : n == 128 ? run_weights<128>(a, p, tq, tk, pairs, st)
+                             : run_weights<64>(a, p, tq, tk, pairs, st);
+  if (e != cudaSuccess || p.sh.groups == 1) return e;
+  // launched while the sums still run; its blocks wait for their end
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)((a.max_len + 255) / 256), (unsigned)a.b, 1);
+  cfg.blockDim = dim3(256, 1, 1);
+  cfg.stream = st;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, weights_combine_kernel, p);
+}
+
+}  // namespace qcau

@@ -220,4 +220,58 @@ cudaError_t launch_attn_combine(const AttnArgs& args, cudaStream_t st);
 cudaError_t launch_decode_attn_sm100(const AttnArgs& args, cudaStream_t st);
 bool decode_attn_sm100_supported(const AttnArgs& args);
 
+// Attention of drafted tokens over a paged cache that holds their rows, and
+// the sums of its weights (attn_tree_sm100.cu, attn_weights_sm100.cu).
+struct TreeArgs {
+  const void* q;               // [b, s, h, d_qk] bf16
+  const void* cache;           // [num_pages, page_size, d_qk] bf16, V = the first 512 values
+  const int32_t* block_table;  // [b, max_pages]
+  const int32_t* seqlens;      // [b] cached tokens, the drafted ones included
+  const int32_t* tree_lens;    // [b] nodes, or nullptr: s
+  const uint8_t* mask;         // [b, s, s] (mask_stride s * s) or [s, s] (0) or nullptr
+  int64_t mask_stride;
+  int64_t b, s, h, d_qk, page_size, max_pages, num_pages, max_len;
+  float scale;
+  // attention
+  const float* sink;  // [h] or nullptr
+  void* o;            // [b, s, h, 512] bf16
+  float* lse;         // [b, s, h] or nullptr (the weights' input)
+  // weight sums
+  float* sums;        // [b, sums_stride]
+  int64_t sums_stride;
+  int accumulate;
+};
+size_t attn_tree_workspace(const TreeArgs& a);
+cudaError_t launch_attn_tree_sm100(const TreeArgs& a, void* ws, cudaStream_t st);
+size_t attn_weights_workspace(const TreeArgs& a);
+cudaError_t launch_attn_weights_sm100(const TreeArgs& a, void* ws, cudaStream_t st);
+
+// mask[b][t][j] = 1 for node t's ancestors j and itself (evict.cu).
+cudaError_t launch_tree_mask(const int32_t* parents, uint8_t* mask, int64_t b, int64_t s,
+                             cudaStream_t st);
+
+// The tokens to keep by their weight sums (evict.cu).
+cudaError_t launch_evict_select(const float* sums, int64_t sums_stride, const int32_t* seqlens,
+                                int32_t* keep, int32_t* counts, float* sums_out,
+                                int64_t out_stride, int64_t b, int64_t max_len, int64_t budget,
+                                int64_t n_first, int64_t n_recent, cudaStream_t st);
+
+// Rows start + keep[i] of a paged cache to rows start + i of the same or
+// another one (evict.cu).
+struct KeepArgs {
+  const void* cache;
+  const int32_t* table;
+  int64_t max_pages, num_pages;
+  void* dst;
+  const int32_t* dst_table;
+  int64_t dst_max_pages, dst_num_pages;
+  const int32_t* keep;    // [b, keep_stride]
+  int64_t keep_stride;
+  const int32_t* counts;  // [b]
+  const int32_t* start;   // [b] or nullptr: 0
+  int32_t* lens_out;      // [b] or nullptr: start + count
+  int64_t b, k, d, page_size;
+};
+cudaError_t launch_keep_rows(const KeepArgs& a, cudaStream_t st);
+
 }  // namespace qcau

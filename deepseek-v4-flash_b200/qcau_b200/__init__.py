@@ -8,12 +8,16 @@ Host-side mirror of the reference's interfaces over libqcau_b200.so:
 * ``qcau_b200.QCAU``    -- the QCAU(...) block of
   QCAU/QCAU_inference/inference/QCAU.py;
 * ``qcau_b200.mla``     -- the absorbed-MLA decode layer (paged latent cache,
-  head sharding with an NCCL all-reduce).
+  head sharding with an NCCL all-reduce);
+* ``qcau_b200.tree``    -- speculative decoding with draft trees on the paged
+  cache (tree_attn, commit);
+* ``qcau_b200.evict``   -- bounding the paged cache by accumulated attention
+  weight (attn_weight_sums, evict).
 
 Every call runs the CUDA kernels of the library; there is no CPU path.
 """
-from . import _lib, kernel, mla
+from . import _lib, evict, kernel, mla, tree
 from .QCAU import QCAU
 from ._lib import QcauError, device_error
 
-__all__ = ["QCAU", "kernel", "mla", "device_error", "QcauError"]
+__all__ = ["QCAU", "evict", "kernel", "mla", "tree", "device_error", "QcauError"]

@@ -119,6 +119,17 @@ SIGNATURES = {
     "qcau_topk": ([_P, _P, _I64, _I64, _I64, _I64, _I64, _I64, _P], ctypes.c_int),
     "qcau_index_lists_width": ([_I64, _I64, _I64, _I64, _I64], _I64),
     "qcau_index_lists": ([_P, _I64, _I64, _I64, _I64, _I64, _I64, _P, _I64, _P], ctypes.c_int),
+    "qcau_tree_mask": ([_P, _P, _I64, _I64, _P], ctypes.c_int),
+    "qcau_tree_attn_workspace_size": ([_I64, _I64, _I64, _I64], _SZ),
+    "qcau_tree_attn": ([_P, _P, _P, _P, _P, _P, _I64, _P, _P, _P, _I64, _I64, _I64, _I64, _I64,
+                        _I64, _I64, _I64, _I64, _F, _P, _SZ, _P], ctypes.c_int),
+    "qcau_attn_weight_sums_workspace_size": ([_I64, _I64, _I64, _I64], _SZ),
+    "qcau_attn_weight_sums": ([_P, _P, _P, _P, _P, _P, _P, _I64, _P, _I64, _I32, _I64, _I64, _I64,
+                               _I64, _I64, _I64, _I64, _I64, _F, _P, _SZ, _P], ctypes.c_int),
+    "qcau_evict_select": ([_P, _I64, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _I64, _I64, _P],
+                          ctypes.c_int),
+    "qcau_keep_rows": ([_P, _P, _I64, _I64, _P, _P, _I64, _I64, _P, _I64, _P, _P, _P, _I64, _I64,
+                        _I64, _I64, _P], ctypes.c_int),
 }
 
 _lib = None

@@ -113,6 +113,72 @@ def window_slots(bsz: int, seqlen: int, start_pos: int, window: int, ring_rows: 
     return out.to(torch.int32).reshape(-1)
 
 
+def _check_paged(cache: torch.Tensor, block_table: torch.Tensor, what: str) -> None:
+    if cache.dim() != 3 or cache.dtype != torch.bfloat16 or not cache.is_contiguous():
+        raise ValueError(f"{what}: the cache must be a contiguous bf16 [pages, page, width] tensor")
+    if block_table.dim() != 2 or block_table.dtype != torch.int32 or not block_table.is_contiguous():
+        raise ValueError(f"{what}: the block table must be a contiguous int32 [batch, pages] tensor")
+
+
+def _check_ints(t: torch.Tensor, shape: tuple, device, what: str) -> None:
+    if t.dtype != torch.int32 or tuple(t.shape) != shape or not t.is_contiguous() or t.device != device:
+        raise ValueError(f"{what} must be a contiguous int32 {list(shape)} tensor on {device}")
+
+
+def _check_move(what: str, cache, block_table, dst_cache, dst_table):
+    """The cache and block table that rows go to, checked with those they come from."""
+    dc = cache if dst_cache is None else dst_cache
+    dt = block_table if dst_table is None else dst_table
+    require_cuda(cache, block_table, dc, dt)
+    _check_paged(cache, block_table, what)
+    _check_paged(dc, dt, what)
+    if dt.size(0) != block_table.size(0) or dc.shape[1:] != cache.shape[1:]:
+        raise ValueError(f"{what}: one row per sequence in both block tables, and caches of one page "
+                         "size and width are needed")
+    if not cache.device == block_table.device == dc.device == dt.device:
+        raise ValueError(f"{what}: all tensors must be on one device")
+    if cache.size(2) % 16:
+        raise ValueError(f"{what}: the row width must be a multiple of 16")
+    return dc, dt
+
+
+def keep_rows(cache: torch.Tensor, block_table: torch.Tensor, keep: torch.Tensor,
+              counts: torch.Tensor, *, start: Optional[torch.Tensor] = None,
+              dst_cache: Optional[torch.Tensor] = None, dst_table: Optional[torch.Tensor] = None,
+              seqlens: Optional[torch.Tensor] = None) -> None:
+    """Bring each sequence of a paged cache down to a choice of its rows.
+
+    Row start[i] + j of sequence i becomes its row start[i] + keep[i, j], for
+    j < counts[i].  keep [b, k] int32 holds strictly ascending offsets (values
+    past counts[i] are ignored), counts and start [b] int32 (start None: 0),
+    cache [pages, page, width] bf16 and block_table [b, max_pages] int32.
+
+    In place unless another cache or block table is given: dst_cache /
+    dst_table name where the rows go (None: cache / block_table).  Pages that
+    are written must belong to one sequence only.  seqlens [b] int32, when
+    given, becomes start + counts.  An offset out of range or out of order is
+    not copied and raises the device error bit DEVERR_INDEX.
+    """
+    require_cuda(keep, counts, start, seqlens)
+    dc, dt = _check_move("keep_rows", cache, block_table, dst_cache, dst_table)
+    dev, (num_pages, page, d) = cache.device, cache.shape
+    b, k = block_table.size(0), keep.size(-1)
+    _check_ints(keep, (b, k), dev, "keep_rows: keep")
+    _check_ints(counts, (b,), dev, "keep_rows: counts")
+    if start is not None:
+        _check_ints(start, (b,), dev, "keep_rows: start")
+    if seqlens is not None:
+        _check_ints(seqlens, (b,), dev, "keep_rows: seqlens")
+    if k == 0:
+        raise ValueError("keep_rows: keep has no columns")
+    with torch.cuda.device(dev):
+        check(lib().qcau_keep_rows(
+            cache.data_ptr(), block_table.data_ptr(), block_table.size(1), num_pages,
+            dc.data_ptr(), dt.data_ptr(), dt.size(1), dc.size(0), keep.data_ptr(), k,
+            counts.data_ptr(), _lib.ptr(start), _lib.ptr(seqlens), b, k, d, page,
+            stream_ptr(dev)), "keep_rows")
+
+
 class PagedKVCache:
     """A paged latent cache [num_pages, page_size, width] bf16 shared by up to
     max_seqs sequences, with their block tables [max_seqs, max_pages] and
@@ -171,6 +237,20 @@ class PagedKVCache:
         for s, n in zip(seqs, counts):
             pos.extend(range(self._len[s] - n, self._len[s]))
         return torch.tensor(pos, dtype=torch.int32, device=self.device)
+
+    def truncate(self, seqs: Sequence[int], lengths: Sequence[int]) -> None:
+        """Shorten sequences to their first lengths[i] tokens (the rows that
+        keep_rows left after an eviction, or the tokens accepted at a drafting
+        step's end) and return the pages they no longer need."""
+        for s, n in zip(seqs, lengths):
+            if not 0 <= n <= self._len[s]:
+                raise ValueError(f"sequence {s} has {self._len[s]} tokens, cannot keep {n}")
+        for s, n in zip(seqs, lengths):
+            need = (n + self.page_size - 1) // self.page_size
+            self._free.extend(reversed(self._pages[s][need:]))
+            del self._pages[s][need:]
+            self._len[s] = n
+        self._sync(seqs)
 
     def release(self, seq: int) -> None:
         """Return the sequence's pages to the free list."""

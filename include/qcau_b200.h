@@ -587,6 +587,84 @@ int qcau_decode_attn_paged_cp_p2p(const void* q_all, const void* cache,
                                   void* stream);
 int qcau_wait_flags(const uint32_t* flags, int64_t n, uint32_t epoch, void* stream);
 
+/* ------------------------------------------------------------------------
+ * Speculative decoding with draft trees, and cache eviction (no reference
+ * counterpart): operators on the paged latent cache [num_pages, page_size,
+ * d_qk] bf16 (page_size a multiple of 64; d_qk 576 or 512, V = the first
+ * 512 values of a row), block_table [b, max_pages] int32.
+ *
+ * The drafted tokens' rows are in the cache: sequence i has seqlens[i] <=
+ * max_seqlen cached tokens of which the last n = tree_lens[i] (NULL: s, and
+ * n <= s, n <= seqlens[i]) are the nodes of its tree; node t is token
+ * base + t, base = seqlens[i] - n.  Node t attends to all tokens before
+ * base, and to token base + j when tree_mask[i][t][j] != 0 (bytes [b, s, s]
+ * with mask_seq_stride s * s, or one mask [s, s] for all with stride 0;
+ * NULL: j <= t, a chain).  Rows of nodes t >= n are not computed.  What lies
+ * in the cache behind a sequence's end is never used, and a drafted row that
+ * is not finite reaches only the nodes that attend to it.  Lengths outside
+ * these ranges are cut to them and raise QCAU_DEVERR_INDEX.
+ *
+ * tree_mask: parents [b, s] int32 (-1: a child of the last token before the
+ *   tree; else the index of an earlier node) -> mask [b, s, s] bytes, 1 at
+ *   each node's ancestors and itself.  A parent that is not an earlier node
+ *   raises QCAU_DEVERR_INDEX and ends the chain.
+ * tree_attn: q [b, s, h, d_qk], o [b, s, h, 512] bf16, lse [b, s, h] fp32 or
+ *   NULL: the natural logarithm of the softmax denominator, the sink's term
+ *   (attn_sink [h] fp32 or NULL) included.  Any h and s.  Rows that see
+ *   nothing get o = 0 and lse = the sink's value (-inf without one); rows of
+ *   nodes t >= n get o = 0 and lse = -inf.  P is rounded to bf16 before P.V
+ *   as in sparse_attn.
+ * attn_weight_sums: sums[i][p] (+)= sum over the query rows of sequence i
+ *   that see token p of exp(softmax_scale * q . k[p] - lse), with the lse of
+ *   tree_attn (s = 1 and no mask: a decode step).  sums [b, sums_stride]
+ *   fp32; accumulate = 0 writes every position of [0, max_seqlen) (0 where no
+ *   query sees), accumulate = 1 adds at the positions below seqlens[i].  The
+ *   same inputs give the same bits (no atomics).
+ * evict_select: of the seqlens[i] tokens the first n_first, the last n_recent
+ *   and those of the largest sums, count = min(seqlens[i], budget) in all, as
+ *   ascending positions keep [b, budget] int32 (-1 past the count) and counts
+ *   [b]; among equal sums the lower position is kept; NaN ranks above every
+ *   number.  sums_out (or NULL; may be sums, with the same stride) gets the
+ *   kept sums in that order and 0 in the rest of [0, max_seqlen).
+ * keep_rows: row start[i] + j of sequence i in dst_cache := its row start[i] +
+ *   keep[i][j] in cache, j < counts[i] <= k (start NULL: 0).  keep is strictly
+ *   ascending; keep [b, keep_stride].  dst_cache / dst_table may be cache /
+ *   block_table (in place, with no other buffer); pages that are written must
+ *   belong to one sequence.  lens_out [b] int32 (or NULL) := start[i] +
+ *   counts[i].  Entries out of range or out of order are skipped and raise
+ *   QCAU_DEVERR_INDEX.  page_size any, d a multiple of 16.  Evicting: keep
+ *   from evict_select.  Ending a drafting step: start = base, keep = the
+ *   accepted path's nodes.
+ * ---------------------------------------------------------------------- */
+int qcau_tree_mask(const int32_t* parents, void* mask, int64_t b, int64_t s, void* stream);
+size_t qcau_tree_attn_workspace_size(int64_t b, int64_t s, int64_t h, int64_t max_seqlen);
+int qcau_tree_attn(const void* q, const void* cache, const int32_t* block_table,
+                   const int32_t* seqlens, const int32_t* tree_lens, const void* tree_mask,
+                   int64_t mask_seq_stride, const float* attn_sink, void* o, float* lse,
+                   int64_t b, int64_t s, int64_t h, int64_t d_qk, int64_t d_v,
+                   int64_t page_size, int64_t max_pages, int64_t num_pages,
+                   int64_t max_seqlen, float softmax_scale, void* workspace,
+                   size_t workspace_bytes, void* stream);
+size_t qcau_attn_weight_sums_workspace_size(int64_t b, int64_t s, int64_t h,
+                                            int64_t max_seqlen);
+int qcau_attn_weight_sums(const void* q, const void* cache, const int32_t* block_table,
+                          const int32_t* seqlens, const float* lse, const int32_t* tree_lens,
+                          const void* tree_mask, int64_t mask_seq_stride, float* sums,
+                          int64_t sums_stride, int32_t accumulate, int64_t b, int64_t s,
+                          int64_t h, int64_t d_qk, int64_t page_size, int64_t max_pages,
+                          int64_t num_pages, int64_t max_seqlen, float softmax_scale,
+                          void* workspace, size_t workspace_bytes, void* stream);
+int qcau_evict_select(const float* sums, int64_t sums_stride, const int32_t* seqlens,
+                      int32_t* keep, int32_t* counts, float* sums_out, int64_t out_stride,
+                      int64_t b, int64_t max_seqlen, int64_t budget, int64_t n_first,
+                      int64_t n_recent, void* stream);
+int qcau_keep_rows(const void* cache, const int32_t* block_table, int64_t max_pages,
+                   int64_t num_pages, void* dst_cache, const int32_t* dst_table,
+                   int64_t dst_max_pages, int64_t dst_num_pages, const int32_t* keep,
+                   int64_t keep_stride, const int32_t* counts, const int32_t* start,
+                   int32_t* lens_out, int64_t b, int64_t k, int64_t d, int64_t page_size,
+                   void* stream);
+
 #ifdef __cplusplus
 }
 #endif

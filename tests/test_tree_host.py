@@ -1,0 +1,125 @@
+"""Draft-tree and eviction entry points without a GPU: workspace sizes, the C
+ABI's refusals before any device work, and the page bookkeeping."""
+import numpy as np
+import pytest
+import torch
+
+from qcau_b200 import _lib
+from qcau_b200.cache import PagedKVCache
+
+_HOST = [np.zeros(1 << 16, dtype=np.uint8) for _ in range(8)]
+P = [int((a.ctypes.data + 15) // 16 * 16) for a in _HOST]
+
+no_device = pytest.mark.skipif(torch.cuda.is_available(),
+                               reason="argument checks with host buffers run without a device")
+
+
+def _expect(rc, exc, text):
+    with pytest.raises(exc) as e:
+        _lib.check(rc, "call")
+    assert text in str(e.value), str(e.value)
+
+
+def test_workspaces_do_not_grow_with_the_batch():
+    """Two slots of 128 rows per CTA pair whatever the batch; none of the partial
+    sums while a sequence's rows are one group."""
+    L = _lib.lib()
+    pair = 2 * 128 * (512 + 2) * 4 + 16
+    assert L.qcau_tree_attn_workspace_size(1, 1, 16, 1) == pair
+    assert L.qcau_tree_attn_workspace_size(64, 64, 128, 32768) == 74 * pair
+    assert L.qcau_attn_weight_sums_workspace_size(32, 1, 128, 16384) == 0
+    assert L.qcau_attn_weight_sums_workspace_size(7, 24, 32, 6001) == 3 * 7 * 6004 * 4
+
+
+@no_device
+def test_tree_attn_refusals():
+    L = _lib.lib()
+    good = dict(q=P[0], cache=P[1], table=P[2], seqlens=P[3], nodes=None, mask=None, stride=0, sink=None, o=P[4],
+                lse=None, b=1, s=4, h=16, d=576, dv=512, page=64, max_pages=4, num_pages=8, most=200, scale=0.07,
+                ws=P[5], ws_bytes=1 << 30)
+
+    def call(**change):
+        a = {**good, **change}
+        return L.qcau_tree_attn(*a.values(), None)
+
+    for change, exc, text in (
+            (dict(q=None), ValueError, "NULL"), (dict(o=None), ValueError, "NULL"), (dict(s=0), ValueError, "bad shape"),
+            (dict(h=0), ValueError, "bad shape"), (dict(b=-1), ValueError, "bad shape"), (dict(most=0), ValueError, "max_seqlen"),
+            (dict(most=257), ValueError, "max_seqlen"), (dict(d=128), NotImplementedError, "d_qk"),
+            (dict(page=16), ValueError, "max_seqlen"), (dict(page=96), NotImplementedError, "page_size"),
+            (dict(mask=P[6], stride=15), ValueError, "stride"), (dict(scale=0.0), ValueError, "softmax_scale"),
+            (dict(scale=float("nan")), ValueError, "softmax_scale"), (dict(q=P[0] + 2), ValueError, "aligned"),
+            (dict(cache=P[1] + 8), ValueError, "aligned"), (dict(o=P[4] + 4), ValueError, "aligned"),
+            (dict(ws_bytes=100), ValueError, "workspace"), (dict(ws=None), ValueError, "workspace"),
+            (dict(b=1 << 17), NotImplementedError, "too large"), (dict(s=1 << 22), NotImplementedError, "too large"),
+            (dict(num_pages=1 << 31), NotImplementedError, "too large")):
+        _expect(call(**change), exc, text)
+    assert call(b=0) == 0
+
+
+@no_device
+def test_weight_sums_refusals():
+    L = _lib.lib()
+    good = dict(q=P[0], cache=P[1], table=P[2], seqlens=P[3], lse=P[4], nodes=None, mask=None, stride=0, sums=P[5],
+                sums_stride=200, accumulate=0, b=1, s=4, h=16, d=576, page=64, max_pages=4, num_pages=8, most=200,
+                scale=0.07, ws=None, ws_bytes=0)
+
+    def call(**change):
+        return L.qcau_attn_weight_sums(*{**good, **change}.values(), None)
+
+    for change, exc, text in (
+            (dict(lse=None), ValueError, "NULL"), (dict(sums=None), ValueError, "NULL"), (dict(sums_stride=199), ValueError, "row of sums"),
+            (dict(page=32), ValueError, "max_seqlen"), (dict(page=100), NotImplementedError, "page_size"),
+            (dict(d=64), NotImplementedError, "d_qk"), (dict(scale=-1.0), ValueError, "softmax_scale"),
+            (dict(s=40), ValueError, "workspace")):
+        _expect(call(**change), exc, text)
+    assert call(b=0) == 0
+
+
+@no_device
+def test_select_and_keep_refusals():
+    L = _lib.lib()
+    good = dict(sums=P[0], stride=100, seqlens=P[1], keep=P[2], counts=P[3], out=None, out_stride=0, b=1, n=100, budget=10,
+                first=2, recent=3)
+
+    def select(**change):
+        return L.qcau_evict_select(*{**good, **change}.values(), None)
+
+    for change, text in ((dict(keep=None), "NULL"), (dict(budget=0), "bad shape"), (dict(n=0), "bad shape"),
+                         (dict(first=8), "budget"), (dict(first=-1), "budget"), (dict(recent=-1), "budget"),
+                         (dict(stride=99), "row of sums"), (dict(out=P[4], out_stride=99), "row of sums")):
+        _expect(select(**change), ValueError, text)
+    assert select(b=0) == 0
+    good_rows = dict(cache=P[0], table=P[1], max_pages=4, num_pages=8, dst=P[0], dst_table=P[1], dst_max_pages=4,
+                     dst_num_pages=8, keep=P[2], keep_stride=5, counts=P[3], start=None, lens=None, b=1, k=5, d=576, page=64)
+
+    def rows(**change):
+        return L.qcau_keep_rows(*{**good_rows, **change}.values(), None)
+
+    for change, exc, text in ((dict(dst=None), ValueError, "NULL"), (dict(k=0), ValueError, "bad shape"),
+                              (dict(keep_stride=4), ValueError, "bad shape"), (dict(page=0), ValueError, "bad shape"),
+                              (dict(d=24), ValueError, "multiple of 16"), (dict(cache=P[0] + 2), ValueError, "aligned"),
+                              (dict(b=70000), NotImplementedError, "too large"),
+                              (dict(max_pages=1 << 26), NotImplementedError, "too large")):
+        _expect(rows(**change), exc, text)
+    assert rows(b=0) == 0
+    _expect(L.qcau_tree_mask(None, P[0], 1, 4, None), ValueError, "NULL")
+    _expect(L.qcau_tree_mask(P[0], P[1], 1, 0, None), ValueError, "bad shape")
+
+
+def test_truncate_returns_pages():
+    pc = PagedKVCache(num_pages=12, max_seqs=2, max_pages=8, width=16, device="cpu")
+    pc.append([0, 1], [300, 100])
+    assert pc.free_pages == 12 - 5 - 2
+    table = pc.block_table.clone()
+    pc.truncate([0, 1], [129, 100])
+    assert pc.free_pages == 12 - 3 - 2 and pc.length(0) == 129 and pc.seqlens.tolist() == [129, 100]
+    assert torch.equal(pc.block_table[0, :3], table[0, :3]) and pc.block_table[0, 3:].eq(0).all()
+    rows = pc.append([0], [63])  # fills the last page
+    assert rows[0] == int(table[0, 2]) * 64 + 1 and pc.free_pages == 7
+    pc.truncate([0], [0])
+    assert pc.free_pages == 10 and pc.length(0) == 0
+    for bad in (-1, 101):
+        with pytest.raises(ValueError):
+            pc.truncate([0, 1], [0, bad])
+    assert pc.length(1) == 100
