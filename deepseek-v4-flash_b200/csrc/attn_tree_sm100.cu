@@ -92,7 +92,8 @@ struct TreeParams {
   float scale;
   float* part_o;   // [pairs][2][128][512]
   float* part_ml;  // [pairs][2][128][2]: max (log2 units), sum
-  int4* desc;      // [pairs]: the row whose pieces start at this pair {b, group, pieces, pairs between pieces}
+  int4* desc;      // [pairs]: the row whose pieces start at this pair {b or -1, group, rows of
+                   // the sequence, pieces | pairs between pieces << 16}
 };
 
 __device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
@@ -160,6 +161,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     sh->abort = 0;
     fence_barrier_init();
   }
+  if (threadIdx.x == 32) {
+    tma_prefetch_desc(&tm_q);
+    tma_prefetch_desc(&tm_k);
+    tma_prefetch_desc(&tm_v);
+  }
+  cudaGridDependencySynchronize();
   tree_plan_sums(p.sh, &sh->plan);
   if (warp == 1) tmem_alloc<2>(&sh->tmem_base, kTmemCols);
   tc_fence_before();
@@ -588,7 +595,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           if (first) {
             const int64_t end = u.row0 + u.q.tiles;  // the range of the row's last tile
             const int last_range = (int)((end * range.nranges - 1) / range.total);
-            owner = make_int4(u.b, u.g, last_range - range.range + 1, range.tsize);
+            owner = make_int4(u.b, u.g, u.q.n * p.sh.h,
+                              (last_range - range.range + 1) | range.tsize << 16);
           }
         }
       }
@@ -614,38 +622,67 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 // Merge of the rows that several ranges share: block (pair, j) takes rows
 // [8 j, 8 j + 8) of the group whose pieces start at that pair, one warp a row:
 // M = max m_i, L = sum l_i 2^(m_i - M), O = sum O_i 2^(m_i - M), then the sink
-// and the normalisation.  Bound by reading the pieces (2 KB a row and piece).
+// and the normalisation.  Latency-bound (2 KB a row and piece): the descriptor
+// holds all that the loads need, and the states and the first four pieces' O are
+// read together.
+constexpr int kMaxPieces = 96;  // at least kTreePairs
+static_assert(kMaxPieces >= kTreePairs, "a row's pieces fit the merge");
+
 __global__ void __launch_bounds__(256) tree_combine_kernel(TreeParams p) {
   cudaGridDependencySynchronize();
   const int pair = blockIdx.x, lane = threadIdx.x & 31;
   const int4 own = p.desc[pair];
-  if (own.x < 0) return;
   const int local = blockIdx.y * 8 + (threadIdx.x >> 5);
-  const int row = own.y * 128 + local;
-  if (row >= tree_seq(p.sh, own.x).n * p.sh.h) return;
+  const int row = own.y * 128 + local, pieces = own.w & 0xffff, step = own.w >> 16;
+  if (own.x < 0 || row >= own.z) return;
   auto slot = [&](int i) -> int64_t {
-    return ((int64_t)(pair + i * own.w) * 2 + (i == 0 ? 1 : 0)) * 128 + local;
+    return ((int64_t)(pair + i * step) * 2 + (i == 0 ? 1 : 0)) * 128 + local;
   };
+  float4 f[4][4];
+  auto load = [&](int i0) {
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+      const float4* src = reinterpret_cast<const float4*>(p.part_o + slot(i0 + j) * 512) + lane;
+#pragma unroll
+      for (int k = 0; k < 4; k++)
+        f[j][k] = i0 + j < pieces ? src[32 * k] : make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+  };
+  float2 ml[kMaxPieces / 32];
+#pragma unroll
+  for (int r = 0; r < kMaxPieces / 32; r++)
+    ml[r] = 32 * r + lane < pieces
+                ? *reinterpret_cast<const float2*>(p.part_ml + slot(32 * r + lane) * 2)
+                : make_float2(-INFINITY, 0.f);
+  load(0);
   float M = -INFINITY;
-  for (int i = lane; i < own.z; i += 32) M = fmaxf(M, p.part_ml[slot(i) * 2]);
+#pragma unroll
+  for (int r = 0; r < kMaxPieces / 32; r++) M = fmaxf(M, ml[r].x);
   M = warp_max(M);
+  float w[kMaxPieces / 32], L = 0.f;
+#pragma unroll
+  for (int r = 0; r < kMaxPieces / 32; r++) {
+    w[r] = ml[r].x == -INFINITY ? 0.f : exp2f(ml[r].x - M);
+    L = fmaf(ml[r].y, w[r], L);
+  }
+  L = warp_sum(L);
   float a[16];
 #pragma unroll
   for (int j = 0; j < 16; j++) a[j] = 0.f;
-  float L = 0.f;
-#pragma unroll 4
-  for (int i = 0; i < own.z; i++) {
-    const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + slot(i) * 2);
-    const float w = ml.x == -INFINITY ? 0.f : exp2f(ml.x - M);
-    const float4* src = reinterpret_cast<const float4*>(p.part_o + slot(i) * 512) + lane;
-    L = fmaf(ml.y, w, L);
+  for (int i0 = 0; i0 < pieces; i0 += 4) {
+    if (i0 > 0) load(i0);
 #pragma unroll
-    for (int k = 0; k < 4; k++) {
-      const float4 f = src[32 * k];
-      a[4 * k] = fmaf(f.x, w, a[4 * k]);
-      a[4 * k + 1] = fmaf(f.y, w, a[4 * k + 1]);
-      a[4 * k + 2] = fmaf(f.z, w, a[4 * k + 2]);
-      a[4 * k + 3] = fmaf(f.w, w, a[4 * k + 3]);
+    for (int j = 0; j < 4; j++) {
+      const int i = i0 + j;  // past the pieces: weight 0 of zeros
+      const float wr = i < 32 ? w[0] : i < 64 ? w[1] : w[2];
+      const float wi = __shfl_sync(0xffffffffu, wr, i & 31);
+#pragma unroll
+      for (int k = 0; k < 4; k++) {
+        a[4 * k] = fmaf(f[j][k].x, wi, a[4 * k]);
+        a[4 * k + 1] = fmaf(f[j][k].y, wi, a[4 * k + 1]);
+        a[4 * k + 2] = fmaf(f[j][k].z, wi, a[4 * k + 2]);
+        a[4 * k + 3] = fmaf(f[j][k].w, wi, a[4 * k + 3]);
+      }
     }
   }
   float inv, lse;
@@ -731,23 +768,13 @@ cudaError_t launch_attn_tree_sm100(const TreeArgs& a, void* ws, cudaStream_t st)
   p.part_o = reinterpret_cast<float*>(ws);
   p.part_ml = p.part_o + (size_t)pairs * 2 * 128 * 512;
   p.desc = reinterpret_cast<int4*>(p.part_ml + (size_t)pairs * 2 * 128 * 2);
-  cudaError_t e = cudaFuncSetAttribute(attn_tree_sm100_kernel,
-                                       cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmemBytes);
+  static std::atomic<uint64_t> done{0};
+  cudaError_t e = allow_smem((const void*)attn_tree_sm100_kernel, kSmemBytes, done);
   if (e != cudaSuccess) return e;
-  attn_tree_sm100_kernel<<<(unsigned)(2 * pairs), kThreads, kSmemBytes, st>>>(tq, tk, tv, p);
-  e = cudaGetLastError();
-  if (e != cudaSuccess || pairs == 1) return e;
-  // launched while the attention still runs; its blocks wait for its end
-  cudaLaunchAttribute attr;
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr.val.programmaticStreamSerializationAllowed = 1;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)pairs, 16, 1);
-  cfg.blockDim = dim3(256, 1, 1);
-  cfg.stream = st;
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, tree_combine_kernel, p);
+  e = launch_early(attn_tree_sm100_kernel, dim3((unsigned)(2 * pairs)), kThreads, kSmemBytes, st, tq,
+                   tk, tv, p);
+  if (e != cudaSuccess || pairs == 1) return e;  // one pair: no row is shared
+  return launch_early(tree_combine_kernel, dim3((unsigned)pairs, 16), 256, 0, st, p);
 }
 
 }  // namespace qcau

@@ -42,7 +42,11 @@ template <int N>
 struct WeightsCfg {
   static constexpr int kQChunk = N / 2 * 128;  // N/2 rows x 64 dims bf16
   static constexpr int kSlots = N == 256 ? 3 : N == 128 ? 6 : 7;
-  static constexpr uint32_t kTmemCols = N;  // 2 buffers x N/2 columns
+  // accumulation chains of a score (see the issuer): as many as TMEM holds twice
+  static constexpr int kChains = N == 256 ? 2 : 4;
+  static constexpr int kSteps = 36 / kChains;  // MMAs of 16 dims in a chain
+  static constexpr uint32_t kBufCols = kChains * N / 2;
+  static constexpr uint32_t kTmemCols = 2 * kBufCols;
 };
 
 template <int N>
@@ -109,6 +113,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     sh->abort = 0;
     fence_barrier_init();
   }
+  if (threadIdx.x == 32) {
+    tma_prefetch_desc(&tm_q);
+    tma_prefetch_desc(&tm_k);
+  }
+  cudaGridDependencySynchronize();
   tree_plan_sums(p.sh, &sh->plan);
   if (warp == 1) tmem_alloc<2>(&sh->tmem_base, C::kTmemCols);
   tc_fence_before();
@@ -129,12 +138,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       TreeCursor c = range.start;
       TreePiece u;
       while (ok && tree_piece(p.sh, c, u)) {
-        if (nq > 0 && !(ok = mbar_wait(&sh->q_empty, (nq - 1) & 1, abort))) break;
-        if (leader) mbar_arrive_expect_tx(&sh->q_full, 2 * p.chunks * C::kQChunk);
-        for (int k = 0; k < p.chunks; k++)  // rows past the sequence's are zero-filled
-          tma_load_3d_pair(sQ + k * C::kQChunk, &tm_q, q_full_l, 64 * k,
-                           u.g * N + N / 2 * (int)rank, u.b);
-        nq++;
         for (int t = u.t_begin; t < u.t_end && ok; t++) {
           const int blk = tree_block(p.sh, u, 2 * t + (int)rank);
           for (int i = 0; i < kBoxes; i++, n++) {
@@ -144,6 +147,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             last_use[slot] = use;
             tma_load_4d_pair(sK + (size_t)slot * kKSlot, &tm_k,
                              mapa_shared(smem_u32(&sh->kfull[slot]), 0), 0, 0, 3 * i, blk);
+          }
+          if (ok && t == u.t_begin) {
+            // the piece's rows, behind its first tile: K streams on while the last
+            // MMAs of the previous piece, which still read Q, complete
+            if (nq > 0 && !(ok = mbar_wait(&sh->q_empty, (nq - 1) & 1, abort))) break;
+            if (leader) mbar_arrive_expect_tx(&sh->q_full, 2 * p.chunks * C::kQChunk);
+            for (int k = 0; k < p.chunks; k++)  // rows past the sequence's are zero-filled
+              tma_load_3d_pair(sQ + k * C::kQChunk, &tm_q, q_full_l, 64 * k,
+                               u.g * N + N / 2 * (int)rank, u.b);
+            nq++;
           }
         }
       }
@@ -174,20 +187,29 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           if (gt >= 2 && !(ok = mbar_wait<true>(&sh->s_free[sb], ((gt >> 1) - 1) & 1, abort)))
             break;
           tc_fence_after();
+#pragma unroll
           for (int g = 0; g < kBoxes; g++, n++) {
             const int slot = n % C::kSlots, use = n / C::kSlots;
             if (!(ok = mbar_wait(&sh->kfull[slot], use & 1, abort))) break;
-            // chunk 3g + i: A = this CTA's 64 tokens, B = its N/2 query rows
+            // chunk 3g + i: A = this CTA's 64 tokens, B = its N/2 query rows.  The
+            // tensor core truncates a sum to fp32 at every step, so one chain of
+            // 36 steps pulls a score towards zero by up to 7e-7 of it, which the
+            // exponential turns into 1.4e-5 of the weight of a token with x = 18;
+            // kChains accumulators of kSteps steps each, added in registers with
+            // rounding, divide that by kChains
             const uint64_t kg = k_desc + (uint64_t)((slot * kKSlot) >> 4);
             const uint64_t qg = q_desc + (uint64_t)((3 * g * C::kQChunk) >> 4);
 #pragma unroll
             for (int i = 0; i < 3; i++) {
               if (3 * g + i >= p.chunks) break;
 #pragma unroll
-              for (int kk = 0; kk < 4; kk++)
-                mma_bf16_pair(tmem + sb * (N / 2), kg + (uint64_t)((i * 8192 + kk * 32) >> 4),
+              for (int kk = 0; kk < 4; kk++) {
+                const int step = 12 * g + 4 * i + kk;
+                mma_bf16_pair(tmem + sb * C::kBufCols + step / C::kSteps * (N / 2),
+                              kg + (uint64_t)((i * 8192 + kk * 32) >> 4),
                               qg + (uint64_t)((i * C::kQChunk + kk * 32) >> 4), idesc,
-                              (g | i | kk) != 0 ? 1u : 0u);
+                              step % C::kSteps != 0 ? 1u : 0u);
+              }
             }
             tc_commit_pair(&sh->kempty[slot], 3);
             last_bar = &sh->kempty[slot];
@@ -274,32 +296,41 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         }
         if (!(ok = tree_warp_wait(&sh->s_full[sb], (gt >> 1) & 1, abort))) break;
         tc_fence_after();
-        const uint32_t s_addr = tmem + lane_base + sb * (N / 2);
+        const uint32_t s_addr = tmem + lane_base + sb * C::kBufCols;
         const uint64_t sc2 = f2_pack(sl2, sl2);
         uint64_t acc[4];
 #pragma unroll
         for (int k = 0; k < 4; k++) acc[k] = f2_pack(0.f, 0.f);
 #pragma unroll
-        for (int k = 0; k < N / 64; k++) {
-          float v[32];
-          tmem_ld32(s_addr + 32 * k, v);
-          tmem_ld_wait_regs(v);
-          if (k == N / 64 - 1) {  // all scores are read: the S buffer is free
+        for (int k = 0; k < N / 32; k++) {  // 16 columns at a time
+          float v[C::kChains][16];
+#pragma unroll
+          for (int c = 0; c < C::kChains; c++) tmem_ld16(s_addr + c * (N / 2) + 16 * k, v[c]);
+#pragma unroll
+          for (int c = 0; c < C::kChains; c++) tmem_ld_wait_regs16(v[c]);
+          if (k == N / 32 - 1) {  // all scores are read: the S buffer is free
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive_remote(s_free_l[sb]);
           }
-          const ulonglong2* n2 = reinterpret_cast<const ulonglong2*>(neg + 32 * k);
+          const ulonglong2* n2 = reinterpret_cast<const ulonglong2*>(neg + 16 * k);
 #pragma unroll
-          for (int i = 0; i < 8; i++) {
+          for (int i = 0; i < 4; i++) {
             const ulonglong2 ng = n2[i];
+            uint64_t s01 = f2_pack(v[0][4 * i], v[0][4 * i + 1]);
+            uint64_t s23 = f2_pack(v[0][4 * i + 2], v[0][4 * i + 3]);
+#pragma unroll
+            for (int c = 1; c < C::kChains; c++) {
+              s01 = f2_add(s01, f2_pack(v[c][4 * i], v[c][4 * i + 1]));
+              s23 = f2_add(s23, f2_pack(v[c][4 * i + 2], v[c][4 * i + 3]));
+            }
             float x0, x1, x2, x3;
-            f2_unpack(f2_fma(f2_pack(v[4 * i], v[4 * i + 1]), sc2, ng.x), x0, x1);
-            f2_unpack(f2_fma(f2_pack(v[4 * i + 2], v[4 * i + 3]), sc2, ng.y), x2, x3);
+            f2_unpack(f2_fma(s01, sc2, ng.x), x0, x1);
+            f2_unpack(f2_fma(s23, sc2, ng.y), x2, x3);
             float p0 = ex2_approx(x0), p1 = ex2_approx(x1);
             float p2 = ex2_approx(x2), p3 = ex2_approx(x3);
             if (!full) {  // a selection, not a product: unseen scores may be NaN
-              const uint32_t m = bits[k] >> (4 * i);
+              const uint32_t m = bits[k / 2] >> (16 * (k & 1) + 4 * i);
               p0 = m & 1u ? p0 : 0.f;
               p1 = m & 2u ? p1 : 0.f;
               p2 = m & 4u ? p2 : 0.f;
@@ -360,12 +391,11 @@ int weights_group(const TreeArgs& a) {
 template <int N>
 cudaError_t run_weights(const TreeArgs& a, const WeightsParams& p, const CUtensorMap& tq,
                         const CUtensorMap& tk, int64_t pairs, cudaStream_t st) {
-  cudaError_t e = cudaFuncSetAttribute(attn_weights_sm100_kernel<N>,
-                                       cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                       (int)weights_smem<N>());
+  static std::atomic<uint64_t> done{0};
+  cudaError_t e = allow_smem((const void*)attn_weights_sm100_kernel<N>, weights_smem<N>(), done);
   if (e != cudaSuccess) return e;
-  attn_weights_sm100_kernel<N><<<(unsigned)(2 * pairs), kThreads, weights_smem<N>(), st>>>(tq, tk, p);
-  return cudaGetLastError();
+  return launch_early(attn_weights_sm100_kernel<N>, dim3((unsigned)(2 * pairs)), kThreads,
+                      weights_smem<N>(), st, tq, tk, p);
 }
 
 }  // namespace
@@ -412,17 +442,8 @@ cudaError_t launch_attn_weights_sm100(const TreeArgs& a, void* ws, cudaStream_t 
                   : n == 128 ? run_weights<128>(a, p, tq, tk, pairs, st)
                              : run_weights<64>(a, p, tq, tk, pairs, st);
   if (e != cudaSuccess || p.sh.groups == 1) return e;
-  // launched while the sums still run; its blocks wait for their end
-  cudaLaunchAttribute attr;
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr.val.programmaticStreamSerializationAllowed = 1;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)((a.max_len + 255) / 256), (unsigned)a.b, 1);
-  cfg.blockDim = dim3(256, 1, 1);
-  cfg.stream = st;
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, weights_combine_kernel, p);
+  return launch_early(weights_combine_kernel,
+                      dim3((unsigned)((a.max_len + 255) / 256), (unsigned)a.b), 256, 0, st, p);
 }
 
 }  // namespace qcau

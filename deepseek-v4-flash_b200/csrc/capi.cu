@@ -66,6 +66,20 @@ int* device_error_word() {
   return a;
 }
 
+// The attribute outlives the call and is per device and kernel, so setting it
+// twice from two threads is harmless; not setting it each time saves about a
+// microsecond of a short call.
+cudaError_t allow_smem(const void* kernel, size_t bytes, std::atomic<uint64_t>& done) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  const uint64_t bit = dev < 64 ? 1ull << dev : 0;
+  if (done.load(std::memory_order_acquire) & bit) return cudaSuccess;
+  e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+  if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_release);
+  return e;
+}
+
 // ---------------------------------------------------------------- TMA descriptors
 
 typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*,
@@ -1455,13 +1469,14 @@ int qcau_attn_combine_ranks(const void* part_o, const float* part_ml, const floa
 namespace {
 
 // What the tree attention and the weight sums check alike.
-int check_tree(const TreeArgs& a, int64_t d_v, const std::string& who) {
+int check_tree(const TreeArgs& a, int64_t d_v, const char* name) {
+  const std::string who(name);
   QCAU_CHECK_ARG(a.b >= 0 && a.s >= 1 && a.h >= 1 && a.page_size > 0 && a.max_pages > 0 &&
                      a.num_pages > 0,
                  who + ": bad shape");
   QCAU_CHECK_ARG(a.max_len >= 1 && a.max_len <= a.max_pages * a.page_size,
                  who + ": max_seqlen must be at least 1 and within the block table");
-  int rc = check_attn_widths(a.d_qk, d_v, a.d_qk, who.c_str());
+  int rc = check_attn_widths(a.d_qk, d_v, a.d_qk, name);
   if (rc) return rc;
   if (a.page_size % 64)
     return fail(QCAU_ERR_UNSUPPORTED, who + ": page_size must be a multiple of 64");
@@ -1488,11 +1503,28 @@ TreeArgs tree_sizes(int64_t b, int64_t s, int64_t h, int64_t max_seqlen) {
   return a;
 }
 
-int check_tree_ws(size_t need, const void* ws, size_t bytes, const char* who) {
-  if (bytes < need || (need && !ws))
+TreeArgs tree_args(const qcau_tree_args& t) {
+  TreeArgs a = tree_sizes(t.b, t.s, t.h, t.max_seqlen);
+  a.q = t.q;
+  a.cache = t.cache;
+  a.block_table = t.block_table;
+  a.seqlens = t.seqlens;
+  a.tree_lens = t.tree_lens;
+  a.mask = reinterpret_cast<const uint8_t*>(t.tree_mask);
+  a.mask_stride = t.mask_seq_stride;
+  a.d_qk = t.d_qk;
+  a.page_size = t.page_size;
+  a.max_pages = t.max_pages;
+  a.num_pages = t.num_pages;
+  a.scale = t.softmax_scale;
+  return a;
+}
+
+int check_tree_ws(size_t need, const qcau_tree_args& t, const char* who) {
+  if (t.workspace_bytes < need || (need && !t.workspace))
     return fail(QCAU_ERR_WORKSPACE,
                 std::string(who) + ": workspace too small (need " + std::to_string(need) + " bytes)");
-  if (need && (reinterpret_cast<uintptr_t>(ws) & 15))
+  if (need && (reinterpret_cast<uintptr_t>(t.workspace) & 15))
     return fail(QCAU_ERR_INVALID, std::string(who) + ": workspace must be 16-byte aligned");
   return QCAU_OK;
 }
@@ -1515,36 +1547,22 @@ size_t qcau_tree_attn_workspace_size(int64_t b, int64_t s, int64_t h, int64_t ma
   return attn_tree_workspace(tree_sizes(b, s, h, max_seqlen));
 }
 
-int qcau_tree_attn(const void* q, const void* cache, const int32_t* block_table,
-                   const int32_t* seqlens, const int32_t* tree_lens, const void* tree_mask,
-                   int64_t mask_seq_stride, const float* attn_sink, void* o, float* lse, int64_t b,
-                   int64_t s, int64_t h, int64_t d_qk, int64_t d_v, int64_t page_size,
-                   int64_t max_pages, int64_t num_pages, int64_t max_seqlen, float softmax_scale,
-                   void* workspace, size_t workspace_bytes, void* stream) {
-  QCAU_CHECK_ARG(b == 0 || (q && cache && block_table && seqlens && o), "tree_attn: NULL pointer");
-  TreeArgs a = tree_sizes(b, s, h, max_seqlen);
-  a.q = q;
-  a.cache = cache;
-  a.block_table = block_table;
-  a.seqlens = seqlens;
-  a.tree_lens = tree_lens;
-  a.mask = reinterpret_cast<const uint8_t*>(tree_mask);
-  a.mask_stride = mask_seq_stride;
-  a.d_qk = d_qk;
-  a.page_size = page_size;
-  a.max_pages = max_pages;
-  a.num_pages = num_pages;
-  a.scale = softmax_scale;
-  a.sink = attn_sink;
-  a.o = o;
-  a.lse = lse;
-  int rc = check_tree(a, d_v, "tree_attn");
+int qcau_tree_attn(const qcau_tree_args* args, void* stream) {
+  QCAU_CHECK_ARG(args != nullptr, "tree_attn: NULL arguments");
+  const qcau_tree_args& t = *args;
+  QCAU_CHECK_ARG(t.b == 0 || (t.q && t.cache && t.block_table && t.seqlens && t.o),
+                 "tree_attn: NULL pointer");
+  TreeArgs a = tree_args(t);
+  a.sink = t.attn_sink;
+  a.o = t.o;
+  a.lse = t.lse;
+  int rc = check_tree(a, t.d_v, "tree_attn");
   if (rc) return rc;
-  QCAU_CHECK_ARG((reinterpret_cast<uintptr_t>(o) & 15) == 0, "tree_attn: o must be 16-byte aligned");
-  rc = check_tree_ws(attn_tree_workspace(a), workspace, workspace_bytes, "tree_attn");
+  QCAU_CHECK_ARG((reinterpret_cast<uintptr_t>(t.o) & 15) == 0, "tree_attn: o must be 16-byte aligned");
+  rc = check_tree_ws(attn_tree_workspace(a), t, "tree_attn");
   if (rc) return rc;
-  if (b == 0) return QCAU_OK;
-  QCAU_CHECK_CUDA(launch_attn_tree_sm100(a, workspace, to_stream(stream)));
+  if (t.b == 0) return QCAU_OK;
+  QCAU_CHECK_CUDA(launch_attn_tree_sm100(a, t.workspace, to_stream(stream)));
   return QCAU_OK;
 }
 
@@ -1552,95 +1570,62 @@ size_t qcau_attn_weight_sums_workspace_size(int64_t b, int64_t s, int64_t h, int
   return attn_weights_workspace(tree_sizes(b, s, h, max_seqlen));
 }
 
-int qcau_attn_weight_sums(const void* q, const void* cache, const int32_t* block_table,
-                          const int32_t* seqlens, const float* lse, const int32_t* tree_lens,
-                          const void* tree_mask, int64_t mask_seq_stride, float* sums,
-                          int64_t sums_stride, int32_t accumulate, int64_t b, int64_t s, int64_t h,
-                          int64_t d_qk, int64_t page_size, int64_t max_pages, int64_t num_pages,
-                          int64_t max_seqlen, float softmax_scale, void* workspace,
-                          size_t workspace_bytes, void* stream) {
-  QCAU_CHECK_ARG(b == 0 || (q && cache && block_table && seqlens && lse && sums),
+int qcau_attn_weight_sums(const qcau_tree_args* args, void* stream) {
+  QCAU_CHECK_ARG(args != nullptr, "attn_weight_sums: NULL arguments");
+  const qcau_tree_args& t = *args;
+  QCAU_CHECK_ARG(t.b == 0 || (t.q && t.cache && t.block_table && t.seqlens && t.lse && t.sums),
                  "attn_weight_sums: NULL pointer");
-  TreeArgs a = tree_sizes(b, s, h, max_seqlen);
-  a.q = q;
-  a.cache = cache;
-  a.block_table = block_table;
-  a.seqlens = seqlens;
-  a.tree_lens = tree_lens;
-  a.mask = reinterpret_cast<const uint8_t*>(tree_mask);
-  a.mask_stride = mask_seq_stride;
-  a.d_qk = d_qk;
-  a.page_size = page_size;
-  a.max_pages = max_pages;
-  a.num_pages = num_pages;
-  a.scale = softmax_scale;
-  a.lse = const_cast<float*>(lse);
-  a.sums = sums;
-  a.sums_stride = sums_stride;
-  a.accumulate = accumulate;
-  int rc = check_tree(a, 512, "attn_weight_sums");
+  TreeArgs a = tree_args(t);
+  a.lse = t.lse;
+  a.sums = t.sums;
+  a.sums_stride = t.sums_stride;
+  a.accumulate = t.accumulate;
+  int rc = check_tree(a, t.d_v, "attn_weight_sums");
   if (rc) return rc;
-  QCAU_CHECK_ARG(sums_stride >= max_seqlen, "attn_weight_sums: a row of sums must hold max_seqlen values");
-  rc = check_tree_ws(attn_weights_workspace(a), workspace, workspace_bytes, "attn_weight_sums");
+  QCAU_CHECK_ARG(t.sums_stride >= t.max_seqlen,
+                 "attn_weight_sums: a row of sums must hold max_seqlen values");
+  rc = check_tree_ws(attn_weights_workspace(a), t, "attn_weight_sums");
   if (rc) return rc;
-  if (b == 0) return QCAU_OK;
-  QCAU_CHECK_CUDA(launch_attn_weights_sm100(a, workspace, to_stream(stream)));
+  if (t.b == 0) return QCAU_OK;
+  QCAU_CHECK_CUDA(launch_attn_weights_sm100(a, t.workspace, to_stream(stream)));
   return QCAU_OK;
 }
 
-int qcau_evict_select(const float* sums, int64_t sums_stride, const int32_t* seqlens, int32_t* keep,
-                      int32_t* counts, float* sums_out, int64_t out_stride, int64_t b,
-                      int64_t max_seqlen, int64_t budget, int64_t n_first, int64_t n_recent,
-                      void* stream) {
-  QCAU_CHECK_ARG(b == 0 || (sums && seqlens && keep && counts), "evict_select: NULL pointer");
-  QCAU_CHECK_ARG(b >= 0 && max_seqlen >= 1 && budget >= 1, "evict_select: bad shape");
-  QCAU_CHECK_ARG(n_first >= 0 && n_recent >= 0 && n_first <= budget && n_recent <= budget - n_first,
+int qcau_evict_select(const qcau_select_args* args, void* stream) {
+  QCAU_CHECK_ARG(args != nullptr, "evict_select: NULL arguments");
+  const qcau_select_args& t = *args;
+  QCAU_CHECK_ARG(t.b == 0 || (t.sums && t.seqlens && t.keep && t.counts), "evict_select: NULL pointer");
+  QCAU_CHECK_ARG(t.b >= 0 && t.max_seqlen >= 1 && t.budget >= 1, "evict_select: bad shape");
+  QCAU_CHECK_ARG(t.n_first >= 0 && t.n_recent >= 0 && t.n_first <= t.budget &&
+                     t.n_recent <= t.budget - t.n_first,
                  "evict_select: the budget must hold n_first and n_recent tokens");
-  QCAU_CHECK_ARG(sums_stride >= max_seqlen && (sums_out == nullptr || out_stride >= max_seqlen),
+  QCAU_CHECK_ARG(t.sums_stride >= t.max_seqlen && (t.sums_out == nullptr || t.out_stride >= t.max_seqlen),
                  "evict_select: a row of sums must hold max_seqlen values");
-  if (b >= (1LL << 31) || max_seqlen >= (1LL << 31) - 2048 || budget >= (1LL << 31) - 2048)
+  if (t.b >= (1LL << 31) || t.max_seqlen >= (1LL << 31) - 65536 || t.budget >= (1LL << 31) - 65536)
     return fail(QCAU_ERR_UNSUPPORTED, "evict_select: batch too large for one call");
-  if (b == 0) return QCAU_OK;
-  QCAU_CHECK_CUDA(launch_evict_select(sums, sums_stride, seqlens, keep, counts, sums_out, out_stride,
-                                      b, max_seqlen, budget, n_first, n_recent, to_stream(stream)));
+  if (t.b == 0) return QCAU_OK;
+  QCAU_CHECK_CUDA(launch_evict_select(t, to_stream(stream)));
   return QCAU_OK;
 }
 
-int qcau_keep_rows(const void* cache, const int32_t* block_table, int64_t max_pages,
-                   int64_t num_pages, void* dst_cache, const int32_t* dst_table,
-                   int64_t dst_max_pages, int64_t dst_num_pages, const int32_t* keep,
-                   int64_t keep_stride, const int32_t* counts, const int32_t* start,
-                   int32_t* lens_out, int64_t b, int64_t k, int64_t d, int64_t page_size,
-                   void* stream) {
-  QCAU_CHECK_ARG(b == 0 || (cache && block_table && dst_cache && dst_table && keep && counts),
+int qcau_keep_rows(const qcau_keep_args* args, void* stream) {
+  QCAU_CHECK_ARG(args != nullptr, "keep_rows: NULL arguments");
+  const qcau_keep_args& t = *args;
+  QCAU_CHECK_ARG(t.b == 0 || (t.cache && t.block_table && t.dst_cache && t.dst_table && t.keep && t.counts),
                  "keep_rows: NULL pointer");
-  QCAU_CHECK_ARG(b >= 0 && k >= 1 && keep_stride >= k && page_size > 0 && max_pages > 0 &&
-                     num_pages > 0 && dst_max_pages > 0 && dst_num_pages > 0,
+  QCAU_CHECK_ARG(t.b >= 0 && t.k >= 1 && t.keep_stride >= t.k && t.page_size > 0 && t.max_pages > 0 &&
+                     t.num_pages > 0 && t.dst_max_pages > 0 && t.dst_num_pages > 0,
                  "keep_rows: bad shape");
-  QCAU_CHECK_ARG(d > 0 && d % 16 == 0, "keep_rows: the row width must be a multiple of 16");
-  QCAU_CHECK_ARG(((reinterpret_cast<uintptr_t>(cache) | reinterpret_cast<uintptr_t>(dst_cache)) & 15) == 0,
+  QCAU_CHECK_ARG(t.d > 0 && t.d % 16 == 0, "keep_rows: the row width must be a multiple of 16");
+  QCAU_CHECK_ARG(((reinterpret_cast<uintptr_t>(t.cache) | reinterpret_cast<uintptr_t>(t.dst_cache)) & 15) == 0,
                  "keep_rows: the caches must be 16-byte aligned");
-  if (b >= 65536 || k >= (1LL << 31) - 4096 || d >= (1LL << 24) || page_size >= (1LL << 31) ||
-      max_pages >= (1LL << 31) / page_size || dst_max_pages >= (1LL << 31) / page_size)
+  // the kernel counts rows in 32 bits
+  const int64_t most = (1LL << 31) / t.page_size;
+  if (t.b >= 65536 || t.k >= (1LL << 31) - 4096 || t.d >= (1LL << 24) || t.max_pages >= most ||
+      t.dst_max_pages >= most || t.num_pages >= most || t.dst_num_pages >= most)
     return fail(QCAU_ERR_UNSUPPORTED, "keep_rows: batch too large for one call");
-  if (b == 0) return QCAU_OK;
-  KeepArgs a{};
-  a.cache = cache;
-  a.table = block_table;
-  a.max_pages = max_pages;
-  a.num_pages = num_pages;
-  a.dst = dst_cache;
-  a.dst_table = dst_table;
-  a.dst_max_pages = dst_max_pages;
-  a.dst_num_pages = dst_num_pages;
-  a.keep = keep;
-  a.keep_stride = keep_stride;
-  a.counts = counts;
-  a.start = start;
-  a.lens_out = lens_out;
-  a.b = b; a.k = k; a.d = d;
-  a.page_size = page_size;
-  QCAU_CHECK_CUDA(launch_keep_rows(a, to_stream(stream)));
+  if (t.b == 0) return QCAU_OK;
+  QCAU_CHECK_CUDA(launch_keep_rows(t, to_stream(stream)));
   return QCAU_OK;
 }
 

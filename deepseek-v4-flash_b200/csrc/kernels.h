@@ -5,6 +5,10 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
+
+#include "qcau_b200.h"
+
 namespace qcau {
 
 // Host-side TMA descriptor builders (driver entry point resolved once).
@@ -16,6 +20,29 @@ bool make_tmap(CUtensorMap* map, CUtensorMapDataType dtype, int rank, const void
 // Device address of the error word of the current device: a file-scope
 // __device__ int in capi.cu (no allocation), resolved once per device.
 int* device_error_word();
+
+// Raises `kernel`'s dynamic shared memory limit on the current device, once per
+// device (`done` is the caller's static: bit i = device i).
+cudaError_t allow_smem(const void* kernel, size_t bytes, std::atomic<uint64_t>& done);
+
+// Launches a kernel that may be set up while the one before it in the stream
+// still runs: the kernel calls cudaGridDependencySynchronize() in every thread
+// before it touches global memory, and so ends after that one has.
+template <typename... P, typename... A>
+cudaError_t launch_early(void (*kernel)(P...), dim3 grid, unsigned threads, size_t smem,
+                         cudaStream_t st, A... args) {
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads, 1, 1);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, P(args)...);
+}
 
 cudaError_t launch_act_quant(const void* x, void* y, void* s, int64_t m, int64_t n, int block,
                              int round_scale, int scale_e8m0, int inplace, cudaStream_t st);
@@ -250,28 +277,9 @@ cudaError_t launch_attn_weights_sm100(const TreeArgs& a, void* ws, cudaStream_t 
 cudaError_t launch_tree_mask(const int32_t* parents, uint8_t* mask, int64_t b, int64_t s,
                              cudaStream_t st);
 
-// The tokens to keep by their weight sums (evict.cu).
-cudaError_t launch_evict_select(const float* sums, int64_t sums_stride, const int32_t* seqlens,
-                                int32_t* keep, int32_t* counts, float* sums_out,
-                                int64_t out_stride, int64_t b, int64_t max_len, int64_t budget,
-                                int64_t n_first, int64_t n_recent, cudaStream_t st);
-
-// Rows start + keep[i] of a paged cache to rows start + i of the same or
-// another one (evict.cu).
-struct KeepArgs {
-  const void* cache;
-  const int32_t* table;
-  int64_t max_pages, num_pages;
-  void* dst;
-  const int32_t* dst_table;
-  int64_t dst_max_pages, dst_num_pages;
-  const int32_t* keep;    // [b, keep_stride]
-  int64_t keep_stride;
-  const int32_t* counts;  // [b]
-  const int32_t* start;   // [b] or nullptr: 0
-  int32_t* lens_out;      // [b] or nullptr: start + count
-  int64_t b, k, d, page_size;
-};
-cudaError_t launch_keep_rows(const KeepArgs& a, cudaStream_t st);
+// The tokens to keep by their weight sums, and the move of a paged cache's rows
+// (evict.cu).
+cudaError_t launch_evict_select(const qcau_select_args& a, cudaStream_t st);
+cudaError_t launch_keep_rows(const qcau_keep_args& a, cudaStream_t st);
 
 }  // namespace qcau

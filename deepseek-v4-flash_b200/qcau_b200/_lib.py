@@ -7,6 +7,8 @@ present, the call raises.
 from __future__ import annotations
 
 import ctypes
+import functools
+import struct
 from pathlib import Path
 
 import torch
@@ -121,16 +123,19 @@ SIGNATURES = {
     "qcau_index_lists": ([_P, _I64, _I64, _I64, _I64, _I64, _I64, _P, _I64, _P], ctypes.c_int),
     "qcau_tree_mask": ([_P, _P, _I64, _I64, _P], ctypes.c_int),
     "qcau_tree_attn_workspace_size": ([_I64, _I64, _I64, _I64], _SZ),
-    "qcau_tree_attn": ([_P, _P, _P, _P, _P, _P, _I64, _P, _P, _P, _I64, _I64, _I64, _I64, _I64,
-                        _I64, _I64, _I64, _I64, _F, _P, _SZ, _P], ctypes.c_int),
+    "qcau_tree_attn": ([_P, _P], ctypes.c_int),
     "qcau_attn_weight_sums_workspace_size": ([_I64, _I64, _I64, _I64], _SZ),
-    "qcau_attn_weight_sums": ([_P, _P, _P, _P, _P, _P, _P, _I64, _P, _I64, _I32, _I64, _I64, _I64,
-                               _I64, _I64, _I64, _I64, _I64, _F, _P, _SZ, _P], ctypes.c_int),
-    "qcau_evict_select": ([_P, _I64, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _I64, _I64, _P],
-                          ctypes.c_int),
-    "qcau_keep_rows": ([_P, _P, _I64, _I64, _P, _P, _I64, _I64, _P, _I64, _P, _P, _P, _I64, _I64,
-                        _I64, _I64, _P], ctypes.c_int),
+    "qcau_attn_weight_sums": ([_P, _P], ctypes.c_int),
+    "qcau_evict_select": ([_P, _P], ctypes.c_int),
+    "qcau_keep_rows": ([_P, _P], ctypes.c_int),
 }
+
+# Argument structs of the header, packed by struct (a twentieth of the time that
+# ctypes takes to convert as many arguments): qcau_tree_args, qcau_select_args
+# and qcau_keep_args; a NULL pointer is 0.
+pack_tree_args = struct.Struct("@11P11qQfi").pack
+pack_select_args = struct.Struct("@5P7q").pack
+pack_keep_args = struct.Struct("@8P9q").pack
 
 _lib = None
 
@@ -169,6 +174,32 @@ def check(rc: int, what: str) -> None:
 
 def stream_ptr(device: torch.device | None = None) -> int:
     return torch.cuda.current_stream(device).cuda_stream
+
+
+def call_on(index: int, what: str, fn, args: bytes) -> None:
+    """check(fn(args, stream)) with device `index` current and its current stream.
+
+    For the short calls of a decode step: the device is switched only when
+    another one is current (the context manager alone costs about 2 us), and the
+    stream is read without building a Stream object."""
+    if index == torch.cuda.current_device():
+        rc = fn(args, torch._C._cuda_getCurrentRawStream(index))
+    else:
+        with torch.cuda.device(index):
+            rc = fn(args, torch._C._cuda_getCurrentRawStream(index))
+    if rc != QCAU_OK:
+        check(rc, what)
+
+
+@functools.lru_cache(maxsize=1024)
+def workspace_size(name: str, *sizes: int) -> int:
+    """A *_workspace_size() of the library, which depends on the sizes alone."""
+    return getattr(lib(), name)(*sizes)
+
+
+def data(t: torch.Tensor | None) -> int:
+    """The address of a tensor as a packed argument: 0 for None."""
+    return 0 if t is None else t.data_ptr()
 
 
 def ptr(t: torch.Tensor | None) -> int | None:

@@ -113,32 +113,42 @@ def window_slots(bsz: int, seqlen: int, start_pos: int, window: int, ring_rows: 
     return out.to(torch.int32).reshape(-1)
 
 
-def _check_paged(cache: torch.Tensor, block_table: torch.Tensor, what: str) -> None:
+def _check_paged(what: str, cache: torch.Tensor, block_table: torch.Tensor) -> None:
     if cache.dim() != 3 or cache.dtype != torch.bfloat16 or not cache.is_contiguous():
         raise ValueError(f"{what}: the cache must be a contiguous bf16 [pages, page, width] tensor")
     if block_table.dim() != 2 or block_table.dtype != torch.int32 or not block_table.is_contiguous():
         raise ValueError(f"{what}: the block table must be a contiguous int32 [batch, pages] tensor")
 
 
-def _check_ints(t: torch.Tensor, shape: tuple, device, what: str) -> None:
-    if t.dtype != torch.int32 or tuple(t.shape) != shape or not t.is_contiguous() or t.device != device:
-        raise ValueError(f"{what} must be a contiguous int32 {list(shape)} tensor on {device}")
+def _check_ints(what: str, name: str, t: torch.Tensor, shape: tuple, index: int) -> None:
+    if t.dtype != torch.int32 or t.shape != shape or not t.is_contiguous() or t.get_device() != index:
+        raise ValueError(f"{what}: {name} must be a contiguous int32 {list(shape)} tensor on the "
+                         "cache's device")
+
+
+def _check_device(what: str, index: int, *tensors: Optional[torch.Tensor]) -> None:
+    """All tensors on CUDA device `index` (-1: the first one is not on a GPU)."""
+    for t in tensors:
+        if t is not None and t.get_device() != index or index < 0:
+            require_cuda(*tensors)
+            raise ValueError(f"{what}: all tensors must be on one device")
 
 
 def _check_move(what: str, cache, block_table, dst_cache, dst_table):
     """The cache and block table that rows go to, checked with those they come from."""
+    index = cache.get_device()
+    _check_device(what, index, cache, block_table, dst_cache, dst_table)
+    _check_paged(what, cache, block_table)
+    if cache.size(2) % 16:
+        raise ValueError(f"{what}: the row width must be a multiple of 16")
+    if dst_cache is None and dst_table is None:
+        return cache, block_table
     dc = cache if dst_cache is None else dst_cache
     dt = block_table if dst_table is None else dst_table
-    require_cuda(cache, block_table, dc, dt)
-    _check_paged(cache, block_table, what)
-    _check_paged(dc, dt, what)
+    _check_paged(what, dc, dt)
     if dt.size(0) != block_table.size(0) or dc.shape[1:] != cache.shape[1:]:
         raise ValueError(f"{what}: one row per sequence in both block tables, and caches of one page "
                          "size and width are needed")
-    if not cache.device == block_table.device == dc.device == dt.device:
-        raise ValueError(f"{what}: all tensors must be on one device")
-    if cache.size(2) % 16:
-        raise ValueError(f"{what}: the row width must be a multiple of 16")
     return dc, dt
 
 
@@ -159,24 +169,28 @@ def keep_rows(cache: torch.Tensor, block_table: torch.Tensor, keep: torch.Tensor
     given, becomes start + counts.  An offset out of range or out of order is
     not copied and raises the device error bit DEVERR_INDEX.
     """
-    require_cuda(keep, counts, start, seqlens)
     dc, dt = _check_move("keep_rows", cache, block_table, dst_cache, dst_table)
-    dev, (num_pages, page, d) = cache.device, cache.shape
-    b, k = block_table.size(0), keep.size(-1)
-    _check_ints(keep, (b, k), dev, "keep_rows: keep")
-    _check_ints(counts, (b,), dev, "keep_rows: counts")
+    index, b, k = cache.get_device(), block_table.size(0), keep.size(-1)
+    _check_ints("keep_rows", "keep", keep, (b, k), index)
+    _check_ints("keep_rows", "counts", counts, (b,), index)
     if start is not None:
-        _check_ints(start, (b,), dev, "keep_rows: start")
+        _check_ints("keep_rows", "start", start, (b,), index)
     if seqlens is not None:
-        _check_ints(seqlens, (b,), dev, "keep_rows: seqlens")
+        _check_ints("keep_rows", "seqlens", seqlens, (b,), index)
     if k == 0:
         raise ValueError("keep_rows: keep has no columns")
-    with torch.cuda.device(dev):
-        check(lib().qcau_keep_rows(
-            cache.data_ptr(), block_table.data_ptr(), block_table.size(1), num_pages,
-            dc.data_ptr(), dt.data_ptr(), dt.size(1), dc.size(0), keep.data_ptr(), k,
-            counts.data_ptr(), _lib.ptr(start), _lib.ptr(seqlens), b, k, d, page,
-            stream_ptr(dev)), "keep_rows")
+    _launch_keep(cache, block_table, dc, dt, keep, counts, start, seqlens)
+
+
+def _launch_keep(cache, block_table, dc, dt, keep, counts, start, seqlens) -> None:
+    (num_pages, page, d), (b, k) = cache.shape, keep.shape
+    max_pages = block_table.size(1)
+    args = _lib.pack_keep_args(
+        cache.data_ptr(), block_table.data_ptr(), dc.data_ptr(), dt.data_ptr(), keep.data_ptr(),
+        counts.data_ptr(), _lib.data(start), _lib.data(seqlens), max_pages, num_pages,
+        max_pages if dt is block_table else dt.size(1), num_pages if dc is cache else dc.size(0),
+        k, b, k, d, page)
+    _lib.call_on(cache.get_device(), "keep_rows", lib().qcau_keep_rows, args)
 
 
 class PagedKVCache:

@@ -20,16 +20,20 @@ from typing import Optional
 
 import torch
 
-from ._lib import check, lib, ptr, require_cuda, stream_ptr
-from .cache import _check_ints, _check_move, keep_rows
+from ._lib import (call_on, data, lib, pack_select_args, pack_tree_args, require_cuda,
+                   workspace_size)
+from .cache import _check_ints, _check_move, _launch_keep
 from .tree import _check_step
 
 
-def _check_sums(sums: torch.Tensor, b: int, device, what: str) -> None:
-    if sums.dim() != 2 or sums.dtype != torch.float32 or sums.size(0) != b or sums.device != device \
-            or sums.stride(1) != 1 or (b > 1 and sums.stride(0) < sums.size(1)):
-        raise ValueError(f"{what}: sums must be fp32 [batch, positions] with contiguous rows, on "
-                         f"{device}")
+def _check_sums(what: str, sums: torch.Tensor, b: int, index: int) -> int:
+    """The row stride of sums [b, positions]."""
+    if sums.dim() != 2 or sums.dtype != torch.float32 or sums.get_device() != index:
+        raise ValueError(f"{what}: sums must be fp32 [batch, positions] on the device of the lengths")
+    (rows, n), (step, one) = sums.shape, sums.stride()
+    if rows != b or (n > 1 and one != 1) or (b > 1 and step < n):
+        raise ValueError(f"{what}: sums needs one contiguous row per sequence")
+    return max(step, n)
 
 
 def attn_weight_sums(q: torch.Tensor, cache: torch.Tensor, block_table: torch.Tensor,
@@ -47,31 +51,28 @@ def attn_weight_sums(q: torch.Tensor, cache: torch.Tensor, block_table: torch.Te
     weights are added to it instead, at positions below seqlens, and it is
     returned.  The same inputs give the same bits.
     """
-    q, stride, most = _check_step("attn_weight_sums", q, cache, block_table, seqlens, mask,
-                                  tree_lens, max_seqlen)
-    require_cuda(lse, sums)
+    q, stride, pages, most = _check_step("attn_weight_sums", q, cache, block_table, seqlens, mask,
+                                         tree_lens, max_seqlen)
     b, s, h, d = q.shape
-    dev = q.device
-    if lse.dtype != torch.float32 or tuple(lse.shape) != (b, s, h) or not lse.is_contiguous() \
-            or lse.device != dev:
+    index = q.get_device()
+    if lse.dtype != torch.float32 or lse.shape != (b, s, h) or not lse.is_contiguous() \
+            or lse.get_device() != index:
         raise ValueError("attn_weight_sums: lse must be a contiguous fp32 [batch, nodes, heads] tensor")
     add = sums is not None
     if add:
-        _check_sums(sums, b, dev, "attn_weight_sums")
+        sums_stride = _check_sums("attn_weight_sums", sums, b, index)
+        if sums.size(1) < most:
+            raise ValueError("attn_weight_sums: a row of sums must hold max_seqlen values")
     else:
-        sums = torch.empty(b, most, device=dev, dtype=torch.float32)
-    if sums.size(1) < most:
-        raise ValueError("attn_weight_sums: a row of sums must hold max_seqlen values")
-    L = lib()
-    need = L.qcau_attn_weight_sums_workspace_size(b, s, h, most)
-    with torch.cuda.device(dev):
-        ws = torch.empty(need, device=dev, dtype=torch.uint8) if need else None
-        check(L.qcau_attn_weight_sums(
-            q.data_ptr(), cache.data_ptr(), block_table.data_ptr(), seqlens.data_ptr(),
-            lse.data_ptr(), ptr(tree_lens), ptr(mask), stride, sums.data_ptr(),
-            max(sums.stride(0), sums.size(1)), int(add), b, s, h, d, cache.size(1),
-            block_table.size(1), cache.size(0), most, softmax_scale, ptr(ws), need,
-            stream_ptr(dev)), "attn_weight_sums")
+        sums = torch.empty((b, most), dtype=torch.float32, device=q.device)
+        sums_stride = most
+    need = workspace_size("qcau_attn_weight_sums_workspace_size", b, s, h, most)
+    ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
+    args = pack_tree_args(
+        q.data_ptr(), cache.data_ptr(), block_table.data_ptr(), seqlens.data_ptr(),
+        data(tree_lens), data(mask), 0, 0, lse.data_ptr(), sums.data_ptr(), data(ws), stride, b, s, h,
+        d, 512, *pages, most, sums_stride, need, softmax_scale, add)
+    call_on(index, "attn_weight_sums", lib().qcau_attn_weight_sums, args)
     return sums
 
 
@@ -86,26 +87,25 @@ def select_rows(sums: torch.Tensor, seqlens: torch.Tensor, budget: int, *, n_fir
     position stays; NaN ranks above every number.  sums_out (may be sums itself)
     gets the kept sums in the new order and 0 behind them.
     """
-    require_cuda(sums, seqlens, sums_out)
-    b = seqlens.numel()
-    dev = sums.device
-    _check_ints(seqlens, (b,), dev, "select_rows: seqlens")
-    _check_sums(sums, b, dev, "select_rows")
-    n = sums.size(1)
-    if sums_out is not None:
-        _check_sums(sums_out, b, dev, "select_rows")
+    b, index = seqlens.numel(), seqlens.get_device()
+    if index < 0:
+        require_cuda(seqlens)
+    _check_ints("select_rows", "seqlens", seqlens, (b,), index)
+    stride = _check_sums("select_rows", sums, b, index)
+    n, out_stride = sums.size(1), 0
+    if sums_out is sums:
+        out_stride = stride
+    elif sums_out is not None:
+        out_stride = _check_sums("select_rows", sums_out, b, index)
         if sums_out.size(1) != n:
             raise ValueError("select_rows: sums_out must have the shape of sums")
-        if sums_out.data_ptr() == sums.data_ptr() and sums_out.stride(0) != sums.stride(0):
+        if sums_out.data_ptr() == sums.data_ptr() and out_stride != stride:
             raise ValueError("select_rows: in place, sums_out must be sums")
-    keep = torch.empty(b, max(budget, 0), device=dev, dtype=torch.int32)
-    counts = torch.empty(b, device=dev, dtype=torch.int32)
-    with torch.cuda.device(dev):
-        check(lib().qcau_evict_select(
-            sums.data_ptr(), max(sums.stride(0), n), seqlens.data_ptr(), keep.data_ptr(),
-            counts.data_ptr(), ptr(sums_out),
-            0 if sums_out is None else max(sums_out.stride(0), n), b, n, budget, n_first, n_recent,
-            stream_ptr(dev)), "evict_select")
+    keep = torch.empty((b, max(budget, 0)), dtype=torch.int32, device=seqlens.device)
+    counts = torch.empty_like(seqlens)
+    args = pack_select_args(sums.data_ptr(), seqlens.data_ptr(), keep.data_ptr(), counts.data_ptr(),
+                            data(sums_out), stride, out_stride, b, n, budget, n_first, n_recent)
+    call_on(index, "evict_select", lib().qcau_evict_select, args)
     return keep, counts
 
 
@@ -123,12 +123,12 @@ def evict(cache: torch.Tensor, block_table: torch.Tensor, seqlens: torch.Tensor,
     """
     # every refusal comes before the sums are touched
     dc, dt = _check_move("evict", cache, block_table, dst_cache, dst_table)
-    if seqlens.numel() != dt.size(0) or sums.device != cache.device:
+    if seqlens.numel() != dt.size(0) or sums.get_device() != cache.get_device():
         raise ValueError("evict: one length per block-table row, and all tensors on one device")
     n = sums.size(-1)
     if n > block_table.size(1) * cache.size(1) or min(budget, n) > dt.size(1) * dc.size(1):
         raise ValueError("evict: a block table does not hold the positions of sums, or the budget")
     keep, counts = select_rows(sums, seqlens, budget, n_first=n_first, n_recent=n_recent,
                                sums_out=sums if sums_out is None else sums_out)
-    keep_rows(cache, block_table, keep, counts, dst_cache=dst_cache, dst_table=dst_table)
+    _launch_keep(cache, block_table, dc, dt, keep, counts, None, None)
     return keep, counts

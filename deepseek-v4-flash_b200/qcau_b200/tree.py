@@ -21,9 +21,9 @@ from typing import Optional
 
 import torch
 
-from . import _lib
-from ._lib import check, lib, ptr, require_cuda, stream_ptr
-from .cache import _check_ints, _check_paged, keep_rows
+from ._lib import (call_on, check, data, lib, pack_tree_args, require_cuda, stream_ptr,
+                   workspace_size)
+from .cache import _check_device, _check_ints, _check_paged, keep_rows
 
 
 def tree_mask(parents: torch.Tensor) -> torch.Tensor:
@@ -34,45 +34,49 @@ def tree_mask(parents: torch.Tensor) -> torch.Tensor:
     require_cuda(parents)
     if parents.dim() != 2 or parents.size(1) == 0:
         raise ValueError("tree_mask: parents must be [batch, nodes]")
-    _check_ints(parents, tuple(parents.shape), parents.device, "tree_mask: parents")
+    _check_ints("tree_mask", "parents", parents, parents.shape, parents.get_device())
     b, s = parents.shape
     mask = torch.empty(b, s, s, device=parents.device, dtype=torch.bool)
-    if b:
-        with torch.cuda.device(parents.device):
-            check(lib().qcau_tree_mask(parents.data_ptr(), mask.data_ptr(), b, s,
-                                       stream_ptr(parents.device)), "tree_mask")
+    with torch.cuda.device(parents.device):
+        check(lib().qcau_tree_mask(parents.data_ptr(), mask.data_ptr(), b, s,
+                                   stream_ptr(parents.device)), "tree_mask")
     return mask
 
 
 def _check_step(what: str, q, cache, block_table, seqlens, mask, tree_lens, max_seqlen):
-    """The checks that the attention and the weight sums share: (q contiguous,
-    sequence stride of the mask, max_seqlen)."""
-    require_cuda(q, cache, block_table, seqlens, mask, tree_lens)
+    """The checks that the attention and the weight sums share.  Returns q
+    contiguous, the mask's sequence stride, (pages, page size, pages of a
+    sequence) and the bound of the lengths."""
+    index = q.get_device()
+    _check_device(what, index, q, cache, block_table, mask)
     if q.dim() != 4 or q.dtype != torch.bfloat16:
         raise ValueError(f"{what}: q must be bf16 [batch, nodes, heads, width]")
-    _check_paged(cache, block_table, what)
+    _check_paged(what, cache, block_table)
     b, s, h, d = q.shape
-    dev = q.device
+    num_pages, page, width = cache.shape
+    rows, max_pages = block_table.shape
     if s == 0 or h == 0:
         raise ValueError(f"{what}: q has no rows")
-    if cache.size(2) != d:
+    if width != d:
         raise ValueError(f"{what}: q and the cache must have one width")
-    if block_table.size(0) != b:
+    if rows != b:
         raise ValueError(f"{what}: one block-table row per sequence is needed")
-    if cache.device != dev or block_table.device != dev:
-        raise ValueError(f"{what}: all tensors must be on one device")
-    _check_ints(seqlens, (b,), dev, f"{what}: seqlens")
+    _check_ints(what, "seqlens", seqlens, (b,), index)
     if tree_lens is not None:
-        _check_ints(tree_lens, (b,), dev, f"{what}: tree_lens")
+        _check_ints(what, "tree_lens", tree_lens, (b,), index)
     stride = 0
     if mask is not None:
-        if mask.dtype not in (torch.bool, torch.uint8) or tuple(mask.shape) not in ((b, s, s), (s, s)) \
-                or not mask.is_contiguous() or mask.device != dev:
+        shape = mask.shape
+        if shape == (b, s, s):
+            stride = s * s
+        if shape not in ((b, s, s), (s, s)) or not mask.is_contiguous() \
+                or mask.dtype not in (torch.bool, torch.uint8):
             raise ValueError(f"{what}: the mask must be a contiguous bool [batch, nodes, nodes] or "
-                             f"[nodes, nodes] tensor on {dev}")
-        stride = s * s if mask.dim() == 3 else 0
-    room = block_table.size(1) * cache.size(1)
-    return q.contiguous(), stride, room if max_seqlen is None else max_seqlen
+                             "[nodes, nodes] tensor")
+    if not q.is_contiguous():
+        q = q.contiguous()
+    most = max_pages * page if max_seqlen is None else max_seqlen
+    return q, stride, (page, max_pages, num_pages), most
 
 
 def tree_attn(q: torch.Tensor, cache: torch.Tensor, block_table: torch.Tensor,
@@ -95,30 +99,29 @@ def tree_attn(q: torch.Tensor, cache: torch.Tensor, block_table: torch.Tensor,
     Nodes past tree_lens[i] get zeros and -inf.  max_seqlen bounds seqlens
     (None: what the block table holds) and sizes the launch.
     """
-    q, stride, most = _check_step("tree_attn", q, cache, block_table, seqlens, mask, tree_lens,
-                                  max_seqlen)
+    q, stride, pages, most = _check_step("tree_attn", q, cache, block_table, seqlens, mask,
+                                         tree_lens, max_seqlen)
     b, s, h, d = q.shape
     dev = q.device
-    sink = None
-    if attn_sink is not None:
-        if attn_sink.numel() != h or attn_sink.device != dev:
+    sink = attn_sink
+    if sink is not None:
+        if sink.numel() != h or sink.device != dev:
             raise ValueError("tree_attn: attn_sink needs one value per head, on q's device")
-        sink = attn_sink.to(torch.float32).contiguous()
+        if sink.dtype != torch.float32 or not sink.is_contiguous():
+            sink = sink.to(torch.float32).contiguous()
     if out is None:
-        out = torch.empty(b, s, h, 512, device=dev, dtype=torch.bfloat16)
-    elif tuple(out.shape) != (b, s, h, 512) or out.dtype != torch.bfloat16 \
+        out = torch.empty((b, s, h, 512), dtype=torch.bfloat16, device=dev)
+    elif out.shape != (b, s, h, 512) or out.dtype != torch.bfloat16 \
             or not out.is_contiguous() or out.device != dev:
         raise ValueError("tree_attn: out must be a contiguous bf16 [batch, nodes, heads, 512] tensor")
-    lse = torch.empty(b, s, h, device=dev, dtype=torch.float32) if return_lse else None
-    L = lib()
-    need = L.qcau_tree_attn_workspace_size(b, s, h, most)
-    with torch.cuda.device(dev):
-        ws = torch.empty(need, device=dev, dtype=torch.uint8)
-        check(L.qcau_tree_attn(
-            q.data_ptr(), cache.data_ptr(), block_table.data_ptr(), seqlens.data_ptr(),
-            ptr(tree_lens), ptr(mask), stride, ptr(sink), out.data_ptr(), ptr(lse), b, s, h, d, 512,
-            cache.size(1), block_table.size(1), cache.size(0), most, softmax_scale, ws.data_ptr(),
-            need, stream_ptr(dev)), "tree_attn")
+    lse = torch.empty((b, s, h), dtype=torch.float32, device=dev) if return_lse else None
+    need = workspace_size("qcau_tree_attn_workspace_size", b, s, h, most)
+    ws = torch.empty(need, dtype=torch.uint8, device=dev)
+    args = pack_tree_args(
+        q.data_ptr(), cache.data_ptr(), block_table.data_ptr(), seqlens.data_ptr(),
+        data(tree_lens), data(mask), data(sink), out.data_ptr(), data(lse), 0, ws.data_ptr(), stride,
+        b, s, h, d, 512, *pages, most, 0, need, softmax_scale, 0)
+    call_on(dev.index, "tree_attn", lib().qcau_tree_attn, args)
     return (out, lse) if return_lse else out
 
 

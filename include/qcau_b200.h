@@ -636,34 +636,58 @@ int qcau_wait_flags(const uint32_t* flags, int64_t n, uint32_t epoch, void* stre
  *   from evict_select.  Ending a drafting step: start = base, keep = the
  *   accepted path's nodes.
  * ---------------------------------------------------------------------- */
+typedef struct {
+    const void* q;
+    const void* cache;
+    const int32_t* block_table;
+    const int32_t* seqlens;
+    const int32_t* tree_lens;  /* or NULL */
+    const void* tree_mask;     /* or NULL */
+    const float* attn_sink;    /* tree_attn: or NULL */
+    void* o;                   /* tree_attn */
+    float* lse;                /* tree_attn: written, or NULL; attn_weight_sums: read */
+    float* sums;               /* attn_weight_sums */
+    void* workspace;           /* at least the *_workspace_size() of the call */
+    int64_t mask_seq_stride;
+    int64_t b, s, h, d_qk, d_v;
+    int64_t page_size, max_pages, num_pages, max_seqlen;
+    int64_t sums_stride;       /* attn_weight_sums */
+    uint64_t workspace_bytes;
+    float softmax_scale;
+    int32_t accumulate;        /* attn_weight_sums */
+} qcau_tree_args;
+
+typedef struct {
+    const float* sums;
+    const int32_t* seqlens;
+    int32_t* keep;
+    int32_t* counts;
+    float* sums_out;           /* or NULL */
+    int64_t sums_stride, out_stride;
+    int64_t b, max_seqlen, budget, n_first, n_recent;
+} qcau_select_args;
+
+typedef struct {
+    const void* cache;
+    const int32_t* block_table;
+    void* dst_cache;
+    const int32_t* dst_table;
+    const int32_t* keep;
+    const int32_t* counts;
+    const int32_t* start;      /* or NULL */
+    int32_t* lens_out;         /* or NULL */
+    int64_t max_pages, num_pages, dst_max_pages, dst_num_pages;
+    int64_t keep_stride, b, k, d, page_size;
+} qcau_keep_args;
+
 int qcau_tree_mask(const int32_t* parents, void* mask, int64_t b, int64_t s, void* stream);
 size_t qcau_tree_attn_workspace_size(int64_t b, int64_t s, int64_t h, int64_t max_seqlen);
-int qcau_tree_attn(const void* q, const void* cache, const int32_t* block_table,
-                   const int32_t* seqlens, const int32_t* tree_lens, const void* tree_mask,
-                   int64_t mask_seq_stride, const float* attn_sink, void* o, float* lse,
-                   int64_t b, int64_t s, int64_t h, int64_t d_qk, int64_t d_v,
-                   int64_t page_size, int64_t max_pages, int64_t num_pages,
-                   int64_t max_seqlen, float softmax_scale, void* workspace,
-                   size_t workspace_bytes, void* stream);
+int qcau_tree_attn(const qcau_tree_args* args, void* stream);
 size_t qcau_attn_weight_sums_workspace_size(int64_t b, int64_t s, int64_t h,
                                             int64_t max_seqlen);
-int qcau_attn_weight_sums(const void* q, const void* cache, const int32_t* block_table,
-                          const int32_t* seqlens, const float* lse, const int32_t* tree_lens,
-                          const void* tree_mask, int64_t mask_seq_stride, float* sums,
-                          int64_t sums_stride, int32_t accumulate, int64_t b, int64_t s,
-                          int64_t h, int64_t d_qk, int64_t page_size, int64_t max_pages,
-                          int64_t num_pages, int64_t max_seqlen, float softmax_scale,
-                          void* workspace, size_t workspace_bytes, void* stream);
-int qcau_evict_select(const float* sums, int64_t sums_stride, const int32_t* seqlens,
-                      int32_t* keep, int32_t* counts, float* sums_out, int64_t out_stride,
-                      int64_t b, int64_t max_seqlen, int64_t budget, int64_t n_first,
-                      int64_t n_recent, void* stream);
-int qcau_keep_rows(const void* cache, const int32_t* block_table, int64_t max_pages,
-                   int64_t num_pages, void* dst_cache, const int32_t* dst_table,
-                   int64_t dst_max_pages, int64_t dst_num_pages, const int32_t* keep,
-                   int64_t keep_stride, const int32_t* counts, const int32_t* start,
-                   int32_t* lens_out, int64_t b, int64_t k, int64_t d, int64_t page_size,
-                   void* stream);
+int qcau_attn_weight_sums(const qcau_tree_args* args, void* stream);
+int qcau_evict_select(const qcau_select_args* args, void* stream);
+int qcau_keep_rows(const qcau_keep_args* args, void* stream);
 
 #ifdef __cplusplus
 }

@@ -34,23 +34,24 @@ def test_workspaces_do_not_grow_with_the_batch():
 @no_device
 def test_tree_attn_refusals():
     L = _lib.lib()
-    good = dict(q=P[0], cache=P[1], table=P[2], seqlens=P[3], nodes=None, mask=None, stride=0, sink=None, o=P[4],
-                lse=None, b=1, s=4, h=16, d=576, dv=512, page=64, max_pages=4, num_pages=8, most=200, scale=0.07,
-                ws=P[5], ws_bytes=1 << 30)
+    good = dict(q=P[0], cache=P[1], table=P[2], seqlens=P[3], nodes=0, mask=0, sink=0, o=P[4], lse=0, sums=0, ws=P[5],
+                stride=0, b=1, s=4, h=16, d=576, dv=512, page=64, max_pages=4, num_pages=8, most=200, sums_stride=0,
+                ws_bytes=1 << 30, scale=0.07, accumulate=0)
 
     def call(**change):
-        a = {**good, **change}
-        return L.qcau_tree_attn(*a.values(), None)
+        return L.qcau_tree_attn(_lib.pack_tree_args(*{**good, **change}.values()), None)
+
+    _expect(L.qcau_tree_attn(None, None), ValueError, "NULL")
 
     for change, exc, text in (
-            (dict(q=None), ValueError, "NULL"), (dict(o=None), ValueError, "NULL"), (dict(s=0), ValueError, "bad shape"),
+            (dict(q=0), ValueError, "NULL"), (dict(o=0), ValueError, "NULL"), (dict(s=0), ValueError, "bad shape"),
             (dict(h=0), ValueError, "bad shape"), (dict(b=-1), ValueError, "bad shape"), (dict(most=0), ValueError, "max_seqlen"),
             (dict(most=257), ValueError, "max_seqlen"), (dict(d=128), NotImplementedError, "d_qk"),
             (dict(page=16), ValueError, "max_seqlen"), (dict(page=96), NotImplementedError, "page_size"),
             (dict(mask=P[6], stride=15), ValueError, "stride"), (dict(scale=0.0), ValueError, "softmax_scale"),
             (dict(scale=float("nan")), ValueError, "softmax_scale"), (dict(q=P[0] + 2), ValueError, "aligned"),
             (dict(cache=P[1] + 8), ValueError, "aligned"), (dict(o=P[4] + 4), ValueError, "aligned"),
-            (dict(ws_bytes=100), ValueError, "workspace"), (dict(ws=None), ValueError, "workspace"),
+            (dict(ws_bytes=100), ValueError, "workspace"), (dict(ws=0), ValueError, "workspace"),
             (dict(b=1 << 17), NotImplementedError, "too large"), (dict(s=1 << 22), NotImplementedError, "too large"),
             (dict(num_pages=1 << 31), NotImplementedError, "too large")):
         _expect(call(**change), exc, text)
@@ -60,15 +61,17 @@ def test_tree_attn_refusals():
 @no_device
 def test_weight_sums_refusals():
     L = _lib.lib()
-    good = dict(q=P[0], cache=P[1], table=P[2], seqlens=P[3], lse=P[4], nodes=None, mask=None, stride=0, sums=P[5],
-                sums_stride=200, accumulate=0, b=1, s=4, h=16, d=576, page=64, max_pages=4, num_pages=8, most=200,
-                scale=0.07, ws=None, ws_bytes=0)
+    good = dict(q=P[0], cache=P[1], table=P[2], seqlens=P[3], nodes=0, mask=0, sink=0, o=0, lse=P[4], sums=P[5], ws=0,
+                stride=0, b=1, s=4, h=16, d=576, dv=512, page=64, max_pages=4, num_pages=8, most=200, sums_stride=200,
+                ws_bytes=0, scale=0.07, accumulate=0)
 
     def call(**change):
-        return L.qcau_attn_weight_sums(*{**good, **change}.values(), None)
+        return L.qcau_attn_weight_sums(_lib.pack_tree_args(*{**good, **change}.values()), None)
+
+    _expect(L.qcau_attn_weight_sums(None, None), ValueError, "NULL")
 
     for change, exc, text in (
-            (dict(lse=None), ValueError, "NULL"), (dict(sums=None), ValueError, "NULL"), (dict(sums_stride=199), ValueError, "row of sums"),
+            (dict(lse=0), ValueError, "NULL"), (dict(sums=0), ValueError, "NULL"), (dict(sums_stride=199), ValueError, "row of sums"),
             (dict(page=32), ValueError, "max_seqlen"), (dict(page=100), NotImplementedError, "page_size"),
             (dict(d=64), NotImplementedError, "d_qk"), (dict(scale=-1.0), ValueError, "softmax_scale"),
             (dict(s=40), ValueError, "workspace")):
@@ -79,24 +82,28 @@ def test_weight_sums_refusals():
 @no_device
 def test_select_and_keep_refusals():
     L = _lib.lib()
-    good = dict(sums=P[0], stride=100, seqlens=P[1], keep=P[2], counts=P[3], out=None, out_stride=0, b=1, n=100, budget=10,
+    good = dict(sums=P[0], seqlens=P[1], keep=P[2], counts=P[3], out=0, stride=100, out_stride=0, b=1, n=100, budget=10,
                 first=2, recent=3)
 
     def select(**change):
-        return L.qcau_evict_select(*{**good, **change}.values(), None)
+        return L.qcau_evict_select(_lib.pack_select_args(*{**good, **change}.values()), None)
 
-    for change, text in ((dict(keep=None), "NULL"), (dict(budget=0), "bad shape"), (dict(n=0), "bad shape"),
+    _expect(L.qcau_evict_select(None, None), ValueError, "NULL")
+
+    for change, text in ((dict(keep=0), "NULL"), (dict(budget=0), "bad shape"), (dict(n=0), "bad shape"),
                          (dict(first=8), "budget"), (dict(first=-1), "budget"), (dict(recent=-1), "budget"),
                          (dict(stride=99), "row of sums"), (dict(out=P[4], out_stride=99), "row of sums")):
         _expect(select(**change), ValueError, text)
     assert select(b=0) == 0
-    good_rows = dict(cache=P[0], table=P[1], max_pages=4, num_pages=8, dst=P[0], dst_table=P[1], dst_max_pages=4,
-                     dst_num_pages=8, keep=P[2], keep_stride=5, counts=P[3], start=None, lens=None, b=1, k=5, d=576, page=64)
+    good_rows = dict(cache=P[0], table=P[1], dst=P[0], dst_table=P[1], keep=P[2], counts=P[3], start=0, lens=0, max_pages=4,
+                     num_pages=8, dst_max_pages=4, dst_num_pages=8, keep_stride=5, b=1, k=5, d=576, page=64)
 
     def rows(**change):
-        return L.qcau_keep_rows(*{**good_rows, **change}.values(), None)
+        return L.qcau_keep_rows(_lib.pack_keep_args(*{**good_rows, **change}.values()), None)
 
-    for change, exc, text in ((dict(dst=None), ValueError, "NULL"), (dict(k=0), ValueError, "bad shape"),
+    _expect(L.qcau_keep_rows(None, None), ValueError, "NULL")
+
+    for change, exc, text in ((dict(dst=0), ValueError, "NULL"), (dict(k=0), ValueError, "bad shape"),
                               (dict(keep_stride=4), ValueError, "bad shape"), (dict(page=0), ValueError, "bad shape"),
                               (dict(d=24), ValueError, "multiple of 16"), (dict(cache=P[0] + 2), ValueError, "aligned"),
                               (dict(b=70000), NotImplementedError, "too large"),
