@@ -43,6 +43,7 @@ namespace qcau {
 namespace {
 
 constexpr int kThreads = 256;
+constexpr int kTile = 128;            // tokens per tile (two blocks of 64, one per CTA for K)
 constexpr int kKSlot = 24576;         // this CTA's 64 tokens x 3 chunks of 64 dims (one box)
 constexpr int kKSlots = 3;            // 9 chunks = 576 dims (8 = 512: the last box ends in zeros)
 constexpr int kVSlot = 32768;         // 64 tokens x this CTA's 256 dims (4 chunks, one box)
@@ -237,7 +238,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           } else if (!(ok = tree_warp_wait(&sh->vempty[i], (gt & 1) ^ 1, abort))) {
             break;
           }
-          const int tok0 = t * kTreeTile + 64 * i;
+          const int tok0 = t * kTile + 64 * i;
           uint8_t* slot = sV + i * kVSlot;
           const uint32_t full_l = mapa_shared(smem_u32(&sh->vfull[i]), 0);
           const bool tail = tok0 + 64 > base;
@@ -431,7 +432,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       for (int t = u.t_begin; t < u.t_end && ok; t++, gt++) {
         const int sb = gt & 1;
         const uint32_t s_addr = tmem + lane_base + kTmemS + sb * 64;
-        const int tok0 = t * kTreeTile + half * 64;
+        const int tok0 = t * kTile + half * 64;
         // which of the half tile's 64 tokens this thread's row sees
         const bool full = tok0 + 64 <= base;
         uint32_t bits[2] = {0xffffffffu, 0xffffffffu};
@@ -700,14 +701,14 @@ __global__ void __launch_bounds__(256) tree_combine_kernel(TreeParams p) {
 
 // As many pairs as there can be ranges of kTreeMinTiles tiles, up to one per
 // two SMs.
-int64_t tree_pairs(const TreeArgs& a, int group_rows) {
+int64_t tree_pairs(const TreeArgs& a, int group_rows, int tile) {
   const int64_t groups = (a.s * a.h + group_rows - 1) / group_rows;
-  const int64_t tiles = a.b * groups * ((a.max_len + kTreeTile - 1) / kTreeTile);
+  const int64_t tiles = a.b * groups * ((a.max_len + tile - 1) / tile);
   const int64_t n = tiles / kTreeMinTiles;
   return n < 1 ? 1 : (n < kTreePairs ? n : kTreePairs);
 }
 
-TreeShape tree_shape(const TreeArgs& a, int group_rows, int64_t pairs) {
+TreeShape tree_shape(const TreeArgs& a, int group_rows, int tile, int64_t pairs) {
   TreeShape p{};
   p.table = a.block_table;
   p.seqlens = a.seqlens;
@@ -722,6 +723,7 @@ TreeShape tree_shape(const TreeArgs& a, int group_rows, int64_t pairs) {
   p.h = (int)a.h;
   p.max_len = (int)a.max_len;
   p.page_blocks = (int)(a.page_size / 64);
+  p.tile = tile;
   p.group_rows = group_rows;
   p.groups = (int)((a.s * a.h + group_rows - 1) / group_rows);
   // teams of `groups` pairs when they leave at most 4 of the 74 pairs idle
@@ -732,12 +734,12 @@ TreeShape tree_shape(const TreeArgs& a, int group_rows, int64_t pairs) {
 }
 
 size_t attn_tree_workspace(const TreeArgs& a) {
-  return (size_t)tree_pairs(a, 128) * (2 * 128 * (512 + 2) * 4 + 16);
+  return (size_t)tree_pairs(a, 128, kTile) * (2 * 128 * (512 + 2) * 4 + 16);
 }
 
 cudaError_t launch_attn_tree_sm100(const TreeArgs& a, void* ws, cudaStream_t st) {
   const int64_t rows = a.s * a.h;
-  const int64_t pairs = tree_pairs(a, 128);
+  const int64_t pairs = tree_pairs(a, 128, kTile);
   CUtensorMap tq, tk, tv;
   {
     const uint64_t dims[3] = {(uint64_t)a.d_qk, (uint64_t)rows, (uint64_t)a.b};
@@ -759,7 +761,7 @@ cudaError_t launch_attn_tree_sm100(const TreeArgs& a, void* ws, cudaStream_t st)
                  CU_TENSOR_MAP_SWIZZLE_128B))
     return cudaErrorInvalidValue;
   TreeParams p{};
-  p.sh = tree_shape(a, 128, pairs);
+  p.sh = tree_shape(a, 128, kTile, pairs);
   p.out = reinterpret_cast<__nv_bfloat16*>(a.o);
   p.lse = a.lse;
   p.sink = a.sink;

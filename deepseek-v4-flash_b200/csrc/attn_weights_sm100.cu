@@ -9,20 +9,26 @@
 // running maximum is not final while it has them, and whose fp32 scores would
 // be 512 bytes a token and 128 rows against the 1152 bytes of reading K again.
 //
-// The tokens are the MMAs' M (128 per CTA pair, a 64-token block per CTA) and
-// up to 256 query rows the N, resident in shared memory while K streams past
-// in 24 KB boxes: a token is one TMEM lane (its rows along the columns, half of
-// them in lane + 64), so its sum needs no shuffles, one thread adds it up in
-// registers and one thread owns the result: no atomics, the same bits each
-// time.  A sequence with more rows than a group leaves one partial sum per
-// group and token (4 bytes against the 2 d bytes of its K row), added in group
-// order by weights_combine.  At 128 rows or fewer a token costs 1152 bytes of
-// HBM and less of everything else; with more, the MMAs (2304 cycles for 64
-// tokens x 256 rows a CTA at full rate) and the exponentials (1024 cycles of
-// the MUFU) bound it.
+// The tokens are the MMAs' M and the query rows the N, resident in shared
+// memory while K streams past: a token is one TMEM lane and its rows lie along
+// the columns, so its sum needs no shuffles, one thread adds it up in registers
+// and one thread owns the result: no atomics, the same bits each time.  A
+// sequence with more rows than a group leaves one partial sum per group and
+// token (4 bytes against the 2 d bytes of its K row), added in group order by
+// weights_combine.
 //
-// Schedule: tree_plan.cuh.  256 threads at most: warp 0 TMA producer, warp 1
-// TMEM allocator and MMA issuer (pair leader), warps 2-5 the epilogue.
+// Up to 128 rows (a decode step) HBM bounds it: 1152 bytes a token.  There M is
+// 256 (128 tokens per CTA: two 64-token blocks) and N 64 or 128: at M = 128 and
+// N = 128 a CTA reads as many operand bytes per MMA as shared memory delivers in
+// its time, and the MMAs took longer than the loads (B200, 32 x 16384 tokens x
+// 128 heads: 117 us, 98.6 us with a third of them).  The M operand of 128 tokens
+// is two boxes of 64 tokens x 3 chunks laid out [8 rows][chunk][8 groups], which
+// makes its 8-row groups 3072 bytes apart across both.  With more rows, N is 256
+// (K is read half as often, from L2, and N = 256 needs fewer operand bytes) and
+// M 128: Q takes 147 KB, and 72 KB of ring hold one 128-token tile.
+//
+// Schedule: tree_plan.cuh.  Warp 0 TMA producer, warp 1 TMEM allocator and MMA
+// issuer (pair leader), warps 2-5 the epilogue.
 // Every wait is bounded; a timeout raises QCAU_DEVERR_TIMEOUT, drains the
 // copies in flight, frees TMEM and returns.
 #include "common.cuh"
@@ -33,30 +39,36 @@ namespace qcau {
 namespace {
 
 constexpr int kThreads = 192;
-constexpr int kKSlot = 24576;  // 64 tokens x 3 chunks of 64 dims
-constexpr int kBoxes = 3;      // boxes of a tile: 9 chunks (8: the last box ends in zeros)
+constexpr int kBlockBox = 24576;  // 64 tokens x 3 chunks of 64 dims
+constexpr int kBoxes = 3;         // stages of a tile: 9 chunks (8: the last stage ends in zeros)
 constexpr float kLog2e = 1.4426950408889634f;
 
 // N rows of a group (64, 128 or 256): half of them in each CTA's shared memory.
 template <int N>
 struct WeightsCfg {
+  static constexpr int kBlocks = N == 256 ? 1 : 2;  // 64-token blocks per CTA and tile
+  static constexpr int kTile = 128 * kBlocks;       // tokens of a pair's tile (MMA M)
+  static constexpr int kStage = kBlocks * kBlockBox;
+  static constexpr int kStages = 3;
   static constexpr int kQChunk = N / 2 * 128;  // N/2 rows x 64 dims bf16
-  static constexpr int kSlots = N == 256 ? 3 : N == 128 ? 6 : 7;
+  // TMEM: M = 128 puts a token's first N/2 columns in lanes 0-63 and the rest in
+  // lanes 64-127; M = 256 all N in its one lane
+  static constexpr int kCols = N == 256 ? 128 : N;
   // accumulation chains of a score (see the issuer): as many as TMEM holds twice
-  static constexpr int kChains = N == 256 ? 2 : 4;
+  static constexpr int kChains = N == 64 ? 4 : 2;
   static constexpr int kSteps = 36 / kChains;  // MMAs of 16 dims in a chain
-  static constexpr uint32_t kBufCols = kChains * N / 2;
+  static constexpr uint32_t kBufCols = kChains * kCols;
   static constexpr uint32_t kTmemCols = 2 * kBufCols;
 };
 
 template <int N>
 struct WeightsShared {
-  uint64_t kfull[WeightsCfg<N>::kSlots], kempty[WeightsCfg<N>::kSlots];
+  uint64_t kfull[WeightsCfg<N>::kStages], kempty[WeightsCfg<N>::kStages];
   uint64_t q_full, q_empty;
   uint64_t s_full[2], s_free[2];
-  uint64_t xbar[2][4];  // halves of a token's sum handed over: 2 warp pairs x 4 buffers
+  uint64_t xbar[2][4];  // M = 128: halves of a token's sum handed over: 2 warp pairs x 4 buffers
   float xsum[4][64];
-  float neg[4][N / 2];  // per epilogue warp: -lse * log2e of its columns
+  float neg[4][WeightsCfg<N>::kCols];  // per epilogue warp: -lse * log2e of its columns
   uint32_t tmem_base;
   int abort;
   TreePlanShared plan;
@@ -65,7 +77,7 @@ struct WeightsShared {
 template <int N>
 constexpr size_t weights_smem() {
   using C = WeightsCfg<N>;
-  return 1024 + 9 * (size_t)C::kQChunk + (size_t)C::kSlots * kKSlot + sizeof(WeightsShared<N>);
+  return 1024 + 9 * (size_t)C::kQChunk + (size_t)C::kStages * C::kStage + sizeof(WeightsShared<N>);
 }
 static_assert(weights_smem<256>() <= 232448 && weights_smem<128>() <= 232448 &&
                   weights_smem<64>() <= 232448,
@@ -90,7 +102,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   const uint32_t pad = (1024u - (smem_u32(smem_raw) & 1023u)) & 1023u;
   uint8_t* sQ = smem_raw + pad;
   uint8_t* sK = sQ + 9 * C::kQChunk;
-  WeightsShared<N>* sh = reinterpret_cast<WeightsShared<N>*>(sK + (size_t)C::kSlots * kKSlot);
+  WeightsShared<N>* sh = reinterpret_cast<WeightsShared<N>*>(sK + (size_t)C::kStages * C::kStage);
   volatile int* abort = &sh->abort;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -99,7 +111,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   const int pair = blockIdx.x >> 1, npairs = gridDim.x >> 1;
 
   if (threadIdx.x == 0) {
-    for (int i = 0; i < C::kSlots; i++) {
+    for (int i = 0; i < C::kStages; i++) {
       mbar_init(&sh->kfull[i], 1);
       mbar_init(&sh->kempty[i], 1);
     }
@@ -130,8 +142,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   if (warp == 0) {
     // ------------------------------------------------ producer (both CTAs)
     if (lane == 0) {
-      int last_use[C::kSlots];
-      for (int i = 0; i < C::kSlots; i++) last_use[i] = -1;
+      int last_use[C::kStages];
+      for (int i = 0; i < C::kStages; i++) last_use[i] = -1;
       const uint32_t q_full_l = mapa_shared(smem_u32(&sh->q_full), 0);
       int n = 0, nq = 0;  // boxes issued; pieces whose Q was issued
       bool ok = true;
@@ -139,14 +151,20 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       TreePiece u;
       while (ok && tree_piece(p.sh, c, u)) {
         for (int t = u.t_begin; t < u.t_end && ok; t++) {
-          const int blk = tree_block(p.sh, u, 2 * t + (int)rank);
+          int blk[C::kBlocks];
+#pragma unroll
+          for (int j = 0; j < C::kBlocks; j++)
+            blk[j] = tree_block(p.sh, u, (2 * t + (int)rank) * C::kBlocks + j);
           for (int i = 0; i < kBoxes; i++, n++) {
-            const int slot = n % C::kSlots, use = n / C::kSlots;
+            const int slot = n % C::kStages, use = n / C::kStages;
             if (!(ok = mbar_wait(&sh->kempty[slot], (use & 1) ^ 1, abort))) break;
-            if (leader) mbar_arrive_expect_tx(&sh->kfull[slot], 2 * kKSlot);
+            if (leader) mbar_arrive_expect_tx(&sh->kfull[slot], 2 * C::kStage);
             last_use[slot] = use;
-            tma_load_4d_pair(sK + (size_t)slot * kKSlot, &tm_k,
-                             mapa_shared(smem_u32(&sh->kfull[slot]), 0), 0, 0, 3 * i, blk);
+            const uint32_t bar = mapa_shared(smem_u32(&sh->kfull[slot]), 0);
+#pragma unroll
+            for (int j = 0; j < C::kBlocks; j++)
+              tma_load_5d_pair(sK + (size_t)slot * C::kStage + j * kBlockBox, &tm_k, bar, 0, 0, 3 * i,
+                               0, blk[j]);
           }
           if (ok && t == u.t_begin) {
             // the piece's rows, behind its first tile: K streams on while the last
@@ -164,15 +182,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         // the leader's full barriers count both CTAs' copies: drain them all
         volatile int never = 0;
         if (nq > 0) mbar_wait<true>(&sh->q_full, (nq - 1) & 1, &never);
-        for (int i = 0; i < C::kSlots; i++)
+        for (int i = 0; i < C::kStages; i++)
           if (last_use[i] >= 0) mbar_wait<true>(&sh->kfull[i], last_use[i] & 1, &never);
       }
     }
   } else if (warp == 1) {
     // ------------------------------------------------ MMA issuer (pair leader)
     if (leader && lane == 0) {
-      const uint32_t idesc = make_idesc(128, N, kFmtBF16, kFmtBF16, false, false);
-      const uint64_t k_desc = make_sdesc(smem_u32(sK), 16, 1024);
+      const uint32_t idesc = make_idesc(C::kTile, N, kFmtBF16, kFmtBF16, false, false);
+      const uint64_t k_desc = make_sdesc(smem_u32(sK), 16, 3072);
       const uint64_t q_desc = make_sdesc(smem_u32(sQ), 16, 1024);
       int n = 0, gt = 0, nu = 0;  // boxes, tiles, pieces
       uint64_t* last_bar = nullptr;
@@ -189,15 +207,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           tc_fence_after();
 #pragma unroll
           for (int g = 0; g < kBoxes; g++, n++) {
-            const int slot = n % C::kSlots, use = n / C::kSlots;
+            const int slot = n % C::kStages, use = n / C::kStages;
             if (!(ok = mbar_wait(&sh->kfull[slot], use & 1, abort))) break;
-            // chunk 3g + i: A = this CTA's 64 tokens, B = its N/2 query rows.  The
-            // tensor core truncates a sum to fp32 at every step, so one chain of
-            // 36 steps pulls a score towards zero by up to 7e-7 of it, which the
+            // chunk 3g + i: A = this CTA's tokens, B = its N/2 query rows.  The
+            // tensor core truncates a sum to fp32 at every step, so a chain of 36
+            // steps pulls a score towards zero by about 8e-7 of it, which the
             // exponential turns into 1.4e-5 of the weight of a token with x = 18;
             // kChains accumulators of kSteps steps each, added in registers with
             // rounding, divide that by kChains
-            const uint64_t kg = k_desc + (uint64_t)((slot * kKSlot) >> 4);
+            const uint64_t kg = k_desc + (uint64_t)((slot * C::kStage) >> 4);
             const uint64_t qg = q_desc + (uint64_t)((3 * g * C::kQChunk) >> 4);
 #pragma unroll
             for (int i = 0; i < 3; i++) {
@@ -205,8 +223,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 #pragma unroll
               for (int kk = 0; kk < 4; kk++) {
                 const int step = 12 * g + 4 * i + kk;
-                mma_bf16_pair(tmem + sb * C::kBufCols + step / C::kSteps * (N / 2),
-                              kg + (uint64_t)((i * 8192 + kk * 32) >> 4),
+                mma_bf16_pair(tmem + sb * C::kBufCols + step / C::kSteps * C::kCols,
+                              kg + (uint64_t)((i * 1024 + kk * 32) >> 4),
                               qg + (uint64_t)((i * C::kQChunk + kk * 32) >> 4), idesc,
                               step % C::kSteps != 0 ? 1u : 0u);
               }
@@ -234,7 +252,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     // ------------------------------------------------ epilogue (warps 2-5)
     const int quarter = warp & 3;
     const int row = quarter * 32 + lane;  // TMEM lane
-    const int hl = row & 63, half = row >> 6;
+    constexpr bool kSplit = C::kCols < N;  // a token's columns in two lanes
+    const int hl = kSplit ? row & 63 : row, half = kSplit ? row >> 6 : 0;
     const int et = threadIdx.x - 64;
     const uint32_t lane_base = (uint32_t)(quarter * 32) << 16;
     const float sl2 = p.scale * kLog2e;
@@ -257,10 +276,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     TreePiece u;
     while (ok && tree_piece(p.sh, c, u)) {
       const int base = u.q.len - u.q.n;
-      const int col0 = u.g * N + half * (N / 2);  // first row of this thread's columns
-      const int ncol = min(max(u.q.n * p.sh.h - col0, 0), N / 2);
+      const int col0 = u.g * N + half * C::kCols;  // first row of this thread's columns
+      const int ncol = min(max(u.q.n * p.sh.h - col0, 0), C::kCols);
       __syncwarp();
-      for (int i = lane; i < N / 2; i += 32)
+      for (int i = lane; i < C::kCols; i += 32)
         neg[i] = i < ncol ? -kLog2e * p.lse[u.b * seq_rows + col0 + i] : 0.f;
       __syncwarp();
       const uint8_t* mask = p.sh.mask ? p.sh.mask + u.b * p.sh.mask_stride : nullptr;
@@ -269,16 +288,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                           : p.part + ((int64_t)u.g * p.sh.b + u.b) * p.part_stride;
       for (int t = u.t_begin; t < u.t_end && ok; t++, gt++) {
         const int sb = gt & 1, xb = gt & 3;
-        const int tok = t * kTreeTile + (int)rank * 64 + hl;
+        const int tok0 = t * C::kTile + (int)rank * (C::kTile / 2), tok = tok0 + hl;
         // columns (rows of the sequence) that see this token
-        const bool full = t * kTreeTile + (int)rank * 64 + 64 <= base && ncol == N / 2;
-        uint32_t bits[N / 64];
+        const bool full = tok0 + C::kTile / 2 <= base && ncol == C::kCols;
+        uint32_t bits[C::kCols / 32];
         if (!full) {
 #pragma unroll
-          for (int k = 0; k < N / 64; k++) bits[k] = 0;
+          for (int k = 0; k < C::kCols / 32; k++) bits[k] = 0;
           auto set = [&](int c0, int c1) {  // columns [c0, c1)
 #pragma unroll
-            for (int k = 0; k < N / 64; k++) {
+            for (int k = 0; k < C::kCols / 32; k++) {
               const int lo = max(c0 - 32 * k, 0), hi = min(c1 - 32 * k, 32);
               if (lo < hi) bits[k] |= (hi - lo == 32 ? 0xffffffffu : ((1u << (hi - lo)) - 1u) << lo);
             }
@@ -302,13 +321,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 #pragma unroll
         for (int k = 0; k < 4; k++) acc[k] = f2_pack(0.f, 0.f);
 #pragma unroll
-        for (int k = 0; k < N / 32; k++) {  // 16 columns at a time
+        for (int k = 0; k < C::kCols / 16; k++) {  // 16 columns at a time
           float v[C::kChains][16];
 #pragma unroll
-          for (int c = 0; c < C::kChains; c++) tmem_ld16(s_addr + c * (N / 2) + 16 * k, v[c]);
+          for (int c = 0; c < C::kChains; c++) tmem_ld16(s_addr + c * C::kCols + 16 * k, v[c]);
 #pragma unroll
           for (int c = 0; c < C::kChains; c++) tmem_ld_wait_regs16(v[c]);
-          if (k == N / 32 - 1) {  // all scores are read: the S buffer is free
+          if (k == C::kCols / 16 - 1) {  // all scores are read: the S buffer is free
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive_remote(s_free_l[sb]);
@@ -343,18 +362,22 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         float a0, a1;
         f2_unpack(f2_add(f2_add(acc[0], acc[1]), f2_add(acc[2], acc[3])), a0, a1);
         float w = a0 + a1;
-        // the token's other half of the columns.  Buffer xb is written again
-        // four tiles on, after an s_full that needs this warp pair's reader to
-        // have released S two tiles later than this one
-        if (half == 1) {
-          sh->xsum[xb][hl] = w;
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&sh->xbar[quarter & 1][xb]);
-        } else {
-          if (!(ok = tree_warp_wait(&sh->xbar[quarter & 1][xb], (gt >> 2) & 1, abort))) break;
-          w += sh->xsum[xb][hl];
-          if (tok < u.q.len) out[tok] = direct && p.accumulate ? out[tok] + w : w;
+        bool owner = true;
+        if constexpr (kSplit) {
+          // the token's other half of the columns.  Buffer xb is written again
+          // four tiles on, after an s_full that needs this warp pair's reader to
+          // have released S two tiles later than this one
+          owner = half == 0;
+          if (!owner) {
+            sh->xsum[xb][hl] = w;
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sh->xbar[quarter & 1][xb]);
+          } else {
+            if (!(ok = tree_warp_wait(&sh->xbar[quarter & 1][xb], (gt >> 2) & 1, abort))) break;
+            w += sh->xsum[xb][hl];
+          }
         }
+        if (owner && tok < u.q.len) out[tok] = direct && p.accumulate ? out[tok] + w : w;
       }
     }
   }
@@ -408,7 +431,8 @@ size_t attn_weights_workspace(const TreeArgs& a) {
 
 cudaError_t launch_attn_weights_sm100(const TreeArgs& a, void* ws, cudaStream_t st) {
   const int n = weights_group(a);
-  const int64_t rows = a.s * a.h, pairs = tree_pairs(a, n);
+  const int tile = n == 256 ? WeightsCfg<256>::kTile : WeightsCfg<128>::kTile;
+  const int64_t rows = a.s * a.h, pairs = tree_pairs(a, n, tile);
   CUtensorMap tq, tk;
   {
     const uint64_t dims[3] = {(uint64_t)a.d_qk, (uint64_t)rows, (uint64_t)a.b};
@@ -419,17 +443,18 @@ cudaError_t launch_attn_weights_sm100(const TreeArgs& a, void* ws, cudaStream_t 
       return cudaErrorInvalidValue;
   }
   {
-    // the cache as [64-token blocks][64 tokens][chunks][64 values]
-    const uint64_t dims[4] = {64, 64, (uint64_t)(a.d_qk / 64),
+    // the cache as [64-token blocks][groups of 8 tokens][chunks][8 tokens][64 values]
+    const uint64_t row = (uint64_t)a.d_qk * 2;
+    const uint64_t dims[5] = {64, 8, (uint64_t)(a.d_qk / 64), 8,
                               (uint64_t)(a.num_pages * (a.page_size / 64))};
-    const uint64_t strides[3] = {(uint64_t)a.d_qk * 2, 128, (uint64_t)a.d_qk * 128};
-    const uint32_t box[4] = {64, 64, 3, 1};
-    if (!make_tmap(&tk, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, a.cache, dims, strides, box,
+    const uint64_t strides[4] = {row, 128, 8 * row, 64 * row};
+    const uint32_t box[5] = {64, 8, 3, 8, 1};
+    if (!make_tmap(&tk, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 5, a.cache, dims, strides, box,
                    CU_TENSOR_MAP_SWIZZLE_128B))
       return cudaErrorInvalidValue;
   }
   WeightsParams p{};
-  p.sh = tree_shape(a, n, pairs);
+  p.sh = tree_shape(a, n, tile, pairs);
   p.lse = a.lse;
   p.sums = a.sums;
   p.sums_stride = a.sums_stride;

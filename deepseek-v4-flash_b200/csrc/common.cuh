@@ -254,6 +254,17 @@ __device__ __forceinline__ void tma_load_4d_pair(void* dst, const void* map,
       : "memory");
 }
 
+// 5-D two-CTA form.  No multicast.
+__device__ __forceinline__ void tma_load_5d_pair(void* dst, const void* map,
+                                                 uint32_t bar_cluster_addr, int x, int y, int z,
+                                                 int w, int v) {
+  asm volatile(
+      "cp.async.bulk.tensor.5d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%3, %4, %5, %6, %7}], [%2];" ::"r"(smem_u32(dst)),
+      "l"(map), "r"(bar_cluster_addr), "r"(x), "r"(y), "r"(z), "r"(w), "r"(v)
+      : "memory");
+}
+
 // ------------------------------------------------------------ tcgen05
 
 template <int kCtaGroup>

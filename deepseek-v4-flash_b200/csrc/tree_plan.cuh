@@ -3,7 +3,7 @@
 // attention and the attention weight sums.
 //
 // The query rows of a sequence (its n nodes x h heads) form groups of
-// `group_rows`; a (sequence, group) row has one tile per 128 cached tokens.
+// `group_rows`; a (sequence, group) row has one tile per `tile` cached tokens.
 // The tiles of all rows, laid end to end at the batch's own lengths (read on
 // the device, so a ragged batch is balanced too), are cut into equal ranges.
 // In the team schedule the tiles of the sequences are cut instead, and each of
@@ -15,7 +15,6 @@
 
 namespace qcau {
 
-constexpr int kTreeTile = 128;  // tokens per tile (two blocks of 64, one per CTA of the pair)
 constexpr int kTreePairs = 74;  // CTA pairs of a B200 (148 SMs)
 constexpr int kTreeMinTiles = 1;
 
@@ -28,6 +27,7 @@ struct TreeShape {
   int64_t max_pages, num_pages, mask_stride;
   int b, s, h, max_len;
   int page_blocks;  // 64-token blocks of a page
+  int tile;         // tokens of a tile (a multiple of 64)
   int group_rows;
   int groups;       // groups of a sequence at s nodes
   int team;         // 1: the team schedule may be used
@@ -35,8 +35,8 @@ struct TreeShape {
 };
 
 // Host side (attn_tree_sm100.cu): CTA pairs of a launch, and its shape.
-int64_t tree_pairs(const TreeArgs& a, int group_rows);
-TreeShape tree_shape(const TreeArgs& a, int group_rows, int64_t pairs);
+int64_t tree_pairs(const TreeArgs& a, int group_rows, int tile);
+TreeShape tree_shape(const TreeArgs& a, int group_rows, int tile, int64_t pairs);
 
 struct TreeSeq {
   int len, n, tiles, groups;
@@ -51,7 +51,7 @@ __device__ __forceinline__ TreeSeq tree_seq(const TreeShape& p, int b) {
   q.n = min(min(max(n, 0), p.s), q.len);
   if (q.len != len || q.n != n) raise_dev_error(p.err, QCAU_DEVERR_INDEX);
   q.groups = (q.n * p.h + p.group_rows - 1) / p.group_rows;
-  q.tiles = q.n > 0 ? (q.len + kTreeTile - 1) / kTreeTile : 0;
+  q.tiles = q.n > 0 ? (q.len + p.tile - 1) / p.tile : 0;
   return q;
 }
 
