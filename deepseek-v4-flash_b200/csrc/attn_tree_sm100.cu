@@ -189,12 +189,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       TreeCursor c = range.start;
       TreePiece u;
       while (ok && tree_piece(p.sh, c, u)) {
-        // Q of the previous piece is free once its last QK has completed
-        if (nq > 0 && !(ok = mbar_wait(&sh->q_empty, (nq - 1) & 1, abort))) break;
-        if (leader) mbar_arrive_expect_tx(&sh->q_full, 2 * p.chunks * 8192);
-        for (int k = 0; k < p.chunks; k++)  // rows past the sequence's are zero-filled
-          tma_load_3d_pair(sQ + k * 8192, &tm_q, q_full_l, 64 * k, u.g * 128 + 64 * (int)rank, u.b);
-        nq++;
         for (int t = u.t_begin; t < u.t_end && ok; t++, gt++) {
           const int blk = tree_block(p.sh, u, 2 * t + (int)rank);
           for (int i = 0; i < kKSlots; i++) {
@@ -209,6 +203,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             last_use[i] = gt;
             tma_load_4d_pair(sK + i * kKSlot, &tm_k, mapa_shared(smem_u32(&sh->kfull[i]), 0), 0, 0,
                              3 * i, blk);
+            if (i == 0 && t == u.t_begin) {
+              // the piece's rows (past the sequence's: zeros), behind its first K
+              // box: free once the previous piece's last QK has completed
+              if (nq > 0 && !(ok = mbar_wait(&sh->q_empty, (nq - 1) & 1, abort))) break;
+              if (leader) mbar_arrive_expect_tx(&sh->q_full, 2 * p.chunks * 8192);
+              tma_load_4d_pair(sQ, &tm_q, q_full_l, 0, u.g * 128 + 64 * (int)rank, 0, u.b);
+              nq++;
+            }
           }
         }
       }
@@ -409,12 +411,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 
     // the rows of nodes that a sequence does not have: zero, log-sum-exp -inf
     const int64_t seq_rows = (int64_t)p.sh.s * p.sh.h;
-    for (int b = blockIdx.x; b < p.sh.b; b += gridDim.x) {
+    // (CTA c: sequence c mod b, together with the other CTAs of that sequence)
+    const int parts = max((int)gridDim.x / p.sh.b, 1), part = blockIdx.x / p.sh.b;
+    for (int b = blockIdx.x % p.sh.b; b < p.sh.b && part < parts; b += gridDim.x) {
       const int64_t r0 = (int64_t)tree_seq(p.sh, b).n * p.sh.h;
       uint4* o = reinterpret_cast<uint4*>(p.out + ((int64_t)b * seq_rows + r0) * 512);
-      for (int64_t i = et; i < (seq_rows - r0) * 64; i += 128) o[i] = make_uint4(0u, 0u, 0u, 0u);
+      for (int64_t i = part * 128 + et; i < (seq_rows - r0) * 64; i += parts * 128)
+        o[i] = make_uint4(0u, 0u, 0u, 0u);
       if (p.lse)
-        for (int64_t i = r0 + et; i < seq_rows; i += 128) p.lse[b * seq_rows + i] = -INFINITY;
+        for (int64_t i = r0 + part * 128 + et; i < seq_rows; i += parts * 128)
+          p.lse[b * seq_rows + i] = -INFINITY;
     }
 
     int4 owner = make_int4(-1, 0, 0, 0);
@@ -550,52 +556,71 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         tc_fence_after();
         const float l_tot = l_run + sh->xsum[row ^ 64];
         const bool first = u.t_begin == 0, last = u.t_end == u.q.tiles;
+        // A thread holds 256 dims of one row; stored as they are, every store of a
+        // warp would touch 32 lines (5300 cycles for bf16, 10200 for fp32).  So
+        // each warp turns 32 rows x 128 bytes at a time in its own 4 KB of the P
+        // buffer, which its last PV has left: 16-byte units swizzled within rows
+        uint8_t* stage = sP + quarter * 4096;
+        const int warp_row = u.g * 128 + (int)rank * 64 + (quarter & 1) * 32;
+        const int live = u.q.n * p.sh.h - warp_row;  // rows of this warp that exist
+        auto put = [&](int k, uint4 v) {
+          *reinterpret_cast<uint4*>(stage + lane * 128 + ((k ^ (lane & 7)) << 4)) = v;
+        };
+        // 128 bytes of each row, from the stage to dst + row * stride
+        auto turn = [&](uint8_t* dst, int stride) {
+          __syncwarp();
+#pragma unroll
+          for (int i = 0; i < 8; i++) {
+            const int r = 4 * i + (lane >> 3), k = lane & 7;
+            const uint4 v = *reinterpret_cast<const uint4*>(stage + r * 128 + ((k ^ (r & 7)) << 4));
+            if (r < live) *reinterpret_cast<uint4*>(dst + (int64_t)r * stride + k * 16) = v;
+          }
+          __syncwarp();
+        };
         if (first && last) {
           // the whole row: normalise and write it
           float inv, lse;
           tree_norm(m_run, l_tot, mine && p.sink ? p.sink[my_row % p.sh.h] : -INFINITY, inv, lse);
           const int64_t orow = u.b * seq_rows + my_row;
-          __nv_bfloat16* po = p.out + orow * 512 + 256 * half;
+          uint8_t* po = reinterpret_cast<uint8_t*>(p.out + (u.b * seq_rows + warp_row) * 512 + 256 * half);
 #pragma unroll 1
-          for (int k = 0; k < 8; k++) {
-            float v[32];
-            tmem_ld32(tmem + lane_base + kTmemO + k * 32, v);
-            tmem_ld_wait_regs(v);
-            uint4* dst = reinterpret_cast<uint4*>(po + k * 32);
-            if (mine) {
+          for (int c = 0; c < 4; c++) {  // 64 dims
+            float v[64];
 #pragma unroll
-              for (int i = 0; i < 4; i++)
-                dst[i] = make_uint4(pack_bf16(v[8 * i] * inv, v[8 * i + 1] * inv),
-                                    pack_bf16(v[8 * i + 2] * inv, v[8 * i + 3] * inv),
-                                    pack_bf16(v[8 * i + 4] * inv, v[8 * i + 5] * inv),
-                                    pack_bf16(v[8 * i + 6] * inv, v[8 * i + 7] * inv));
-            }
+            for (int k = 0; k < 2; k++)
+              tmem_ld32(tmem + lane_base + kTmemO + 64 * c + 32 * k,
+                        *reinterpret_cast<float(*)[32]>(v + 32 * k));
+#pragma unroll
+            for (int k = 0; k < 2; k++) tmem_ld_wait_regs(v + 32 * k);
+#pragma unroll
+            for (int k = 0; k < 8; k++)
+              put(k, make_uint4(pack_bf16(v[8 * k] * inv, v[8 * k + 1] * inv),
+                                pack_bf16(v[8 * k + 2] * inv, v[8 * k + 3] * inv),
+                                pack_bf16(v[8 * k + 4] * inv, v[8 * k + 5] * inv),
+                                pack_bf16(v[8 * k + 6] * inv, v[8 * k + 7] * inv)));
+            turn(po + 128 * c, 1024);
           }
           if (p.lse && half == 0 && mine) p.lse[orow] = lse;
         } else {
           // a piece: its state and unnormalised O (fp32) to slot 1 when the row
           // starts here, else to slot 0
-          const int64_t prow = ((int64_t)pair * 2 + (first ? 1 : 0)) * 128 + rank * 64 + hl;
-          float* po = p.part_o + prow * 512 + 256 * half;
+          const int64_t prow0 = ((int64_t)pair * 2 + (first ? 1 : 0)) * 128 + rank * 64;
+          uint8_t* po = reinterpret_cast<uint8_t*>(p.part_o + (prow0 + (quarter & 1) * 32) * 512 + 256 * half);
 #pragma unroll 1
-          for (int k = 0; k < 8; k++) {
+          for (int c = 0; c < 8; c++) {  // 32 dims
             float v[32];
-            tmem_ld32(tmem + lane_base + kTmemO + k * 32, v);
+            tmem_ld32(tmem + lane_base + kTmemO + c * 32, v);
             tmem_ld_wait_regs(v);
-            float4* dst = reinterpret_cast<float4*>(po + k * 32);
-            if (mine) {
 #pragma unroll
-              for (int i = 0; i < 8; i++)
-                dst[i] = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
-            }
+            for (int k = 0; k < 8; k++)
+              put(k, make_uint4(__float_as_uint(v[4 * k]), __float_as_uint(v[4 * k + 1]),
+                                __float_as_uint(v[4 * k + 2]), __float_as_uint(v[4 * k + 3])));
+            turn(po + 128 * c, 2048);
           }
-          if (half == 0) {
-            p.part_ml[prow * 2] = m_run;
-            p.part_ml[prow * 2 + 1] = l_tot;
-          }
+          if (half == 0)
+            *reinterpret_cast<float2*>(p.part_ml + (prow0 + hl) * 2) = make_float2(m_run, l_tot);
           if (first) {
-            const int64_t end = u.row0 + u.q.tiles;  // the range of the row's last tile
-            const int last_range = (int)((end * range.nranges - 1) / range.total);
+            const int last_range = tree_range_of(range, u.row0 + u.q.tiles - 1);
             owner = make_int4(u.b, u.g, u.q.n * p.sh.h,
                               (last_range - range.range + 1) | range.tsize << 16);
           }
@@ -742,10 +767,12 @@ cudaError_t launch_attn_tree_sm100(const TreeArgs& a, void* ws, cudaStream_t st)
   const int64_t pairs = tree_pairs(a, 128, kTile);
   CUtensorMap tq, tk, tv;
   {
-    const uint64_t dims[3] = {(uint64_t)a.d_qk, (uint64_t)rows, (uint64_t)a.b};
-    const uint64_t strides[2] = {(uint64_t)a.d_qk * 2, (uint64_t)(rows * a.d_qk) * 2};
-    const uint32_t box[3] = {64, 64, 1};
-    if (!make_tmap(&tq, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, a.q, dims, strides, box,
+    // Q as [b][chunks][rows][64 values]: a CTA's 64 rows in one box
+    const uint64_t row = (uint64_t)a.d_qk * 2;
+    const uint64_t dims[4] = {64, (uint64_t)rows, (uint64_t)(a.d_qk / 64), (uint64_t)a.b};
+    const uint64_t strides[3] = {row, 128, (uint64_t)rows * row};
+    const uint32_t box[4] = {64, 64, (uint32_t)(a.d_qk / 64), 1};
+    if (!make_tmap(&tq, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, a.q, dims, strides, box,
                    CU_TENSOR_MAP_SWIZZLE_128B))
       return cudaErrorInvalidValue;
   }

@@ -171,9 +171,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             // MMAs of the previous piece, which still read Q, complete
             if (nq > 0 && !(ok = mbar_wait(&sh->q_empty, (nq - 1) & 1, abort))) break;
             if (leader) mbar_arrive_expect_tx(&sh->q_full, 2 * p.chunks * C::kQChunk);
-            for (int k = 0; k < p.chunks; k++)  // rows past the sequence's are zero-filled
-              tma_load_3d_pair(sQ + k * C::kQChunk, &tm_q, q_full_l, 64 * k,
-                               u.g * N + N / 2 * (int)rank, u.b);
+            // (rows past the sequence's are zero-filled)
+            tma_load_4d_pair(sQ, &tm_q, q_full_l, 0, u.g * N + N / 2 * (int)rank, 0, u.b);
             nq++;
           }
         }
@@ -435,10 +434,12 @@ cudaError_t launch_attn_weights_sm100(const TreeArgs& a, void* ws, cudaStream_t 
   const int64_t rows = a.s * a.h, pairs = tree_pairs(a, n, tile);
   CUtensorMap tq, tk;
   {
-    const uint64_t dims[3] = {(uint64_t)a.d_qk, (uint64_t)rows, (uint64_t)a.b};
-    const uint64_t strides[2] = {(uint64_t)a.d_qk * 2, (uint64_t)(rows * a.d_qk) * 2};
-    const uint32_t box[3] = {64, (uint32_t)n / 2, 1};
-    if (!make_tmap(&tq, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, a.q, dims, strides, box,
+    // Q as [b][chunks][rows][64 values]: a CTA's rows in one box
+    const uint64_t row = (uint64_t)a.d_qk * 2;
+    const uint64_t dims[4] = {64, (uint64_t)rows, (uint64_t)(a.d_qk / 64), (uint64_t)a.b};
+    const uint64_t strides[3] = {row, 128, (uint64_t)rows * row};
+    const uint32_t box[4] = {64, (uint32_t)n / 2, (uint32_t)(a.d_qk / 64), 1};
+    if (!make_tmap(&tq, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, a.q, dims, strides, box,
                    CU_TENSOR_MAP_SWIZZLE_128B))
       return cudaErrorInvalidValue;
   }

@@ -126,6 +126,17 @@ __device__ __forceinline__ void tree_plan_sums(const TreeShape& p, TreePlanShare
   }
 }
 
+// First tile of range i: floor(i total / nranges), in 32 bits (nranges is small).
+__device__ __forceinline__ int tree_cut(const TreeRange& r, int i) {
+  const int q = r.total / r.nranges, rem = r.total - q * r.nranges;
+  return i * q + i * rem / r.nranges;
+}
+
+// The range that tile x belongs to: the largest i with tree_cut(i) <= x.
+__device__ __forceinline__ int tree_range_of(const TreeRange& r, int x) {
+  return (int)(((int64_t)(x + 1) * r.nranges - 1) / r.total);
+}
+
 // Second half, after that barrier (all threads of the CTA): this pair's range.
 // Every CTA sums the same lengths, so all take one plan.
 __device__ __forceinline__ TreeRange tree_plan_range(const TreeShape& p, TreePlanShared* sh,
@@ -145,8 +156,8 @@ __device__ __forceinline__ TreeRange tree_plan_range(const TreeShape& p, TreePla
   r.nranges = max(1, min(npairs / r.tsize, r.total / p.min_tiles));
   r.range = pair / r.tsize;
   const bool busy = r.range < r.nranges;
-  r.start.x = busy ? (int)((int64_t)r.range * r.total / r.nranges) : 0;
-  r.start.x_end = busy ? (int)((int64_t)(r.range + 1) * r.total / r.nranges) : 0;
+  r.start.x = busy ? tree_cut(r, r.range) : 0;
+  r.start.x_end = busy ? tree_cut(r, r.range + 1) : 0;
   r.start.group = team ? pair % r.tsize : -1;
   r.start.b = 0;
   r.start.first = 0;
