@@ -57,49 +57,52 @@ __device__ __forceinline__ uint32_t sum_key(float x) {
   return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
 
-__device__ __forceinline__ float key_sum(uint32_t k) {
-  return __uint_as_float(k == 0xfffffffeu ? 0x7fc00000u : k & 0x80000000u ? k & 0x7fffffffu : ~k);
-}
-
 constexpr int kBins = 2048;
 
 struct SelShared {
-  int hist[kBins];
-  int gt[32 * kSelWarps], eq[32 * kSelWarps];
-  int scan[2][kSelWarps];
+  int hist[3][kBins];            // one per digit, all cleared at the start
+  uint32_t count[32 * kSelWarps];  // kept-token counts per (j, warp): above the bar | at it << 16
+  uint32_t scan[2][kSelWarps];
   int pick[3];
 };
+
+__device__ __forceinline__ void select_clear(SelShared* sh) {
+  for (int i = threadIdx.x; i < 3 * kBins; i += kSelThreads) (&sh->hist[0][0])[i] = 0;
+}
 
 // The budget-th largest key, or a value that exactly `budget` keys reach: three
 // digits of 11, 11 and 10 bits from the top, a histogram of the keys that share
 // the digits so far, and the bin that holds the budget-th key.  A bin that ends
 // exactly there ends the search.  visit(f) calls f(key) for each of the thread's
-// keys (0: none).
+// keys (0: none).  Starts behind select_clear and a barrier; a digit costs three
+// barriers, which is most of its time after the first.
 template <typename Visit>
 __device__ __forceinline__ uint32_t select_bar(SelShared* sh, int budget, Visit visit) {
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   uint32_t prefix = 0, known = 0;
   int want = budget;
+#pragma unroll 1
   for (int digit = 0; digit < 3; digit++) {
     const int width = digit < 2 ? 11 : 10, shift = digit == 0 ? 21 : digit == 1 ? 10 : 0;
-    for (int i = tid; i < kBins; i += kSelThreads) sh->hist[i] = 0;
-    __syncthreads();
+    int* hist = sh->hist[digit];
     visit([&](uint32_t k) {
       if (k != 0 && (k & known) == prefix)
-        atomicAdd(&sh->hist[(k >> shift) & ((1u << width) - 1u)], 1);
+        atomicAdd(&hist[(k >> shift) & ((1u << width) - 1u)], 1);
     });
     __syncthreads();
     // thread i owns bins 2047 - 2i and 2046 - 2i
-    const int h0 = sh->hist[kBins - 1 - 2 * tid], h1 = sh->hist[kBins - 2 - 2 * tid];
+    const int2 h = *reinterpret_cast<const int2*>(&hist[kBins - 2 - 2 * tid]);
+    const int h0 = h.y, h1 = h.x;
     int inc = h0 + h1;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const int x = __shfl_up_sync(0xffffffffu, inc, o);
       if (lane >= o) inc += x;
     }
-    if (lane == 31) sh->scan[0][warp] = inc;
+    if (lane == 31) sh->scan[digit & 1][warp] = inc;
     __syncthreads();
-    const int above = __reduce_add_sync(0xffffffffu, lane < warp ? sh->scan[0][lane] : 0) + inc - h0 - h1;
+    const int above = (int)__reduce_add_sync(0xffffffffu, lane < warp ? sh->scan[digit & 1][lane] : 0u) +
+                      inc - h0 - h1;
     if (above < want && want <= above + h0 + h1) {
       const bool second = want > above + h0;
       sh->pick[0] = kBins - 1 - 2 * tid - (second ? 1 : 0);
@@ -116,110 +119,83 @@ __device__ __forceinline__ uint32_t select_bar(SelShared* sh, int budget, Visit 
 }
 
 // One block per sequence, its keys in registers: value j of thread i is token
-// j * 1024 + i.  One read of the sums; select_bar works on the registers and a
-// shared-memory histogram (16384 random sums: see the table of the design
-// notes); then each kept token's place is the number of kept tokens before it,
-// from ballots and one scan over (j, warp).  Latency-bound: a sequence is one
-// SM's work, 64 KB at 16384 tokens.
+// j * 1024 + i.  One read of the sums (all loads in flight at once, past the
+// length they read the last sum again); select_bar works on the registers and
+// shared-memory histograms; then each kept token's place is the number of kept
+// tokens before it, from ballots and one scan over (j, warp).  Latency-bound: a
+// sequence is one SM's work (64 KB at 16384 tokens).
 template <int V>
 __global__ void __launch_bounds__(kSelThreads)
     evict_select_kernel(qcau_select_args p, int* err) {
-  __shared__ SelShared shared;
+  __shared__ __align__(16) SelShared shared;
   SelShared* sh = &shared;
+  select_clear(sh);
   cudaGridDependencySynchronize();
   cudaTriggerProgrammaticLaunchCompletion();  // the move of the rows may be launched; it waits
   const int b = blockIdx.x, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int max_len = (int)p.max_seqlen, budget = (int)p.budget;
   const int n_first = (int)p.n_first, n_recent = (int)p.n_recent;
   int len = p.seqlens[b];
+  const float* src = p.sums + b * p.sums_stride;
+  float x[V];
+#pragma unroll
+  for (int j = 0; j < V; j++) x[j] = src[min(j * kSelThreads + tid, max_len - 1)];
   if (len < 0 || len > max_len) {
     if (tid == 0) raise_dev_error(err, QCAU_DEVERR_INDEX);
     len = min(max(len, 0), max_len);
   }
-  const float* src = p.sums + b * p.sums_stride;
+  // the always-kept tokens rank above every sum
   uint32_t key[V];
 #pragma unroll
   for (int j = 0; j < V; j++) {
     const int i = j * kSelThreads + tid;
-    key[j] = i < len ? sum_key(src[i]) : 0u;
+    key[j] = i >= len ? 0u : i < n_first || i >= len - n_recent ? 0xffffffffu : sum_key(x[j]);
   }
   const int count = min(len, budget);
-  // the always-kept tokens rank above every sum
-  auto rank_key = [&](int j) {
-    const int i = j * kSelThreads + tid;
-    return i < len && (i < n_first || i >= len - n_recent) ? 0xffffffffu : key[j];
-  };
   uint32_t bar = 1;  // every token's key is above it
+  __syncthreads();
   if (len > budget)
     bar = select_bar(sh, budget, [&](auto f) {
 #pragma unroll
-      for (int j = 0; j < V; j++) f(rank_key(j));
+      for (int j = 0; j < V; j++) f(key[j]);
     });
   // tokens above the bar and at it, per (j, warp)
 #pragma unroll
   for (int j = 0; j < V; j++) {
-    const uint32_t k = rank_key(j);
-    const unsigned g = __ballot_sync(0xffffffffu, k > bar), e = __ballot_sync(0xffffffffu, k == bar);
-    if (lane == 0) {
-      sh->gt[j * kSelWarps + warp] = __popc(g);
-      sh->eq[j * kSelWarps + warp] = __popc(e);
-    }
+    const unsigned g = __ballot_sync(0xffffffffu, key[j] > bar);
+    const unsigned e = __ballot_sync(0xffffffffu, key[j] == bar);
+    if (lane == 0) sh->count[j * kSelWarps + warp] = __popc(g) | __popc(e) << 16;
   }
   __syncthreads();
-  // exclusive prefix sums over the V * 32 entries in token order: thread i owns
-  // V / 32 (at least 1) of them
-  constexpr int kPer = V * kSelWarps > kSelThreads ? V * kSelWarps / kSelThreads : 1;
-  int g[kPer], e[kPer], gs = 0, es = 0;
-#pragma unroll
-  for (int k = 0; k < kPer; k++) {
-    const int i = tid * kPer + k;
-    g[k] = i < V * kSelWarps ? sh->gt[i] : 0;
-    e[k] = i < V * kSelWarps ? sh->eq[i] : 0;
-    gs += g[k];
-    es += e[k];
-  }
-  int gi = gs, ei = es;
+  // exclusive prefix sums over the V * 32 entries in token order, both counts at
+  // once (at most 32768 tokens: no carry between the halves)
+  const uint32_t mine = tid < V * kSelWarps ? sh->count[tid] : 0u;
+  uint32_t inc = mine;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const int x = __shfl_up_sync(0xffffffffu, gi, o), y = __shfl_up_sync(0xffffffffu, ei, o);
-    if (lane >= o) {
-      gi += x;
-      ei += y;
-    }
+    const uint32_t y = __shfl_up_sync(0xffffffffu, inc, o);
+    if (lane >= o) inc += y;
   }
-  if (lane == 31) {
-    sh->scan[0][warp] = gi;
-    sh->scan[1][warp] = ei;
-  }
+  if (lane == 31) sh->scan[0][warp] = inc;
   __syncthreads();
-  const int sg = sh->scan[0][lane], se = sh->scan[1][lane];
-  const int total_gt = __reduce_add_sync(0xffffffffu, sg);
-  int gx = gi - gs + __reduce_add_sync(0xffffffffu, lane < warp ? sg : 0);
-  int ex = ei - es + __reduce_add_sync(0xffffffffu, lane < warp ? se : 0);
-#pragma unroll
-  for (int k = 0; k < kPer; k++) {
-    const int i = tid * kPer + k;
-    if (i < V * kSelWarps) {
-      sh->gt[i] = gx;
-      sh->eq[i] = ex;
-    }
-    gx += g[k];
-    ex += e[k];
-  }
+  const uint32_t sums = sh->scan[0][lane];
+  const int total_gt = (int)(__reduce_add_sync(0xffffffffu, sums) & 0xffffu);
+  if (tid < V * kSelWarps)
+    sh->count[tid] = inc - mine + __reduce_add_sync(0xffffffffu, lane < warp ? sums : 0u);
   const int ties = count - total_gt;  // of the tokens at the bar, the first ones
   __syncthreads();  // the values of this sequence are all read: sums_out may be sums
   int32_t* kp = p.keep + (int64_t)b * budget;
   float* out = p.sums_out ? p.sums_out + b * p.out_stride : nullptr;
 #pragma unroll
   for (int j = 0; j < V; j++) {
-    const uint32_t k = rank_key(j);
-    const unsigned bg = __ballot_sync(0xffffffffu, k > bar), be = __ballot_sync(0xffffffffu, k == bar);
+    const uint32_t k = key[j], before = sh->count[j * kSelWarps + warp];
+    const unsigned g = __ballot_sync(0xffffffffu, k > bar), e = __ballot_sync(0xffffffffu, k == bar);
     const unsigned lt = (1u << lane) - 1u;
-    const int before_eq = sh->eq[j * kSelWarps + warp] + __popc(be & lt);
-    const int pos = sh->gt[j * kSelWarps + warp] + __popc(bg & lt) + min(before_eq, ties);
+    const int before_eq = (int)(before >> 16) + __popc(e & lt);
+    const int pos = (int)(before & 0xffffu) + __popc(g & lt) + min(before_eq, ties);
     if (k > bar || (k == bar && before_eq < ties)) {
       kp[pos] = j * kSelThreads + tid;
-      if (out) out[pos] = key_sum(key[j]);
+      if (out) out[pos] = x[j];
     }
   }
   for (int i = count + tid; i < budget; i += kSelThreads) kp[i] = -1;
@@ -234,8 +210,10 @@ __global__ void __launch_bounds__(kSelThreads)
 // earlier one).
 __global__ void __launch_bounds__(kSelThreads)
     evict_select_long_kernel(qcau_select_args p, int* err) {
-  __shared__ SelShared shared;
+  __shared__ __align__(16) SelShared shared;
   SelShared* sh = &shared;
+  select_clear(sh);
+  __syncthreads();
   cudaGridDependencySynchronize();
   cudaTriggerProgrammaticLaunchCompletion();
   const int b = blockIdx.x, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -264,7 +242,7 @@ __global__ void __launch_bounds__(kSelThreads)
     n = __reduce_add_sync(0xffffffffu, n);
     if (lane == 0) sh->scan[1][warp] = n;
     __syncthreads();
-    total_gt = __reduce_add_sync(0xffffffffu, sh->scan[1][lane]);
+    total_gt = (int)__reduce_add_sync(0xffffffffu, sh->scan[1][lane]);
     __syncthreads();
   }
   const int ties = count - total_gt;

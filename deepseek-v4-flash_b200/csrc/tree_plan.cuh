@@ -77,9 +77,9 @@ struct TreeRange {
 };
 
 struct TreePlanShared {
-  long long sum_rows[8], sum_seqs[8];  // per warp (up to 8): tiles of all rows, of all sequences
-  int scan[8];                         // per warp: tiles of a run of sequences
-  int start_b, start_tile;             // first sequence of the range, and its first tile
+  long long sum_rows[12], sum_seqs[12];  // per warp (up to 12): tiles of all rows, of all sequences
+  int scan[12];                          // per warp: tiles of a run of sequences
+  int start_b, start_tile;               // first sequence of the range, and its first tile
 };
 
 __device__ __forceinline__ bool tree_piece(const TreeShape& p, TreeCursor& c, TreePiece& u) {
