@@ -182,7 +182,7 @@ def call_on(index: int, what: str, fn, args: bytes) -> None:
     For the short calls of a decode step: the device is switched only when
     another one is current (the context manager alone costs about 2 us), and the
     stream is read without building a Stream object."""
-    if index == torch.cuda.current_device():
+    if index == torch._C._cuda_getDevice():
         rc = fn(args, torch._C._cuda_getCurrentRawStream(index))
     else:
         with torch.cuda.device(index):

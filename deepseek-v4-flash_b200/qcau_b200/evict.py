@@ -26,14 +26,15 @@ from .cache import _check_ints, _check_move, _launch_keep
 from .tree import _check_step
 
 
-def _check_sums(what: str, sums: torch.Tensor, b: int, index: int) -> int:
-    """The row stride of sums [b, positions]."""
-    if sums.dim() != 2 or sums.dtype != torch.float32 or sums.get_device() != index:
-        raise ValueError(f"{what}: sums must be fp32 [batch, positions] on the device of the lengths")
-    (rows, n), (step, one) = sums.shape, sums.stride()
+def _check_sums(what: str, sums: torch.Tensor, b: int, index: int):
+    """(positions, row stride) of sums [b, positions]."""
+    shape = sums.shape
+    if len(shape) != 2 or sums.dtype != torch.float32 or sums.get_device() != index:
+        raise ValueError(f"{what}: sums must be fp32 [batch, positions] on the device of the others")
+    (rows, n), (step, one) = shape, sums.stride()
     if rows != b or (n > 1 and one != 1) or (b > 1 and step < n):
         raise ValueError(f"{what}: sums needs one contiguous row per sequence")
-    return max(step, n)
+    return n, max(step, n)
 
 
 def attn_weight_sums(q: torch.Tensor, cache: torch.Tensor, block_table: torch.Tensor,
@@ -51,17 +52,15 @@ def attn_weight_sums(q: torch.Tensor, cache: torch.Tensor, block_table: torch.Te
     weights are added to it instead, at positions below seqlens, and it is
     returned.  The same inputs give the same bits.
     """
-    q, stride, pages, most = _check_step("attn_weight_sums", q, cache, block_table, seqlens, mask,
-                                         tree_lens, max_seqlen)
-    b, s, h, d = q.shape
-    index = q.get_device()
+    index, q, (b, s, h, d), stride, pages, most = _check_step(
+        "attn_weight_sums", q, cache, block_table, seqlens, mask, tree_lens, max_seqlen)
     if lse.dtype != torch.float32 or lse.shape != (b, s, h) or not lse.is_contiguous() \
             or lse.get_device() != index:
         raise ValueError("attn_weight_sums: lse must be a contiguous fp32 [batch, nodes, heads] tensor")
     add = sums is not None
     if add:
-        sums_stride = _check_sums("attn_weight_sums", sums, b, index)
-        if sums.size(1) < most:
+        n, sums_stride = _check_sums("attn_weight_sums", sums, b, index)
+        if n < most:
             raise ValueError("attn_weight_sums: a row of sums must hold max_seqlen values")
     else:
         sums = torch.empty((b, most), dtype=torch.float32, device=q.device)
@@ -87,20 +86,29 @@ def select_rows(sums: torch.Tensor, seqlens: torch.Tensor, budget: int, *, n_fir
     position stays; NaN ranks above every number.  sums_out (may be sums itself)
     gets the kept sums in the new order and 0 behind them.
     """
-    b, index = seqlens.numel(), seqlens.get_device()
+    index = seqlens.get_device()
     if index < 0:
         require_cuda(seqlens)
-    _check_ints("select_rows", "seqlens", seqlens, (b,), index)
-    stride = _check_sums("select_rows", sums, b, index)
-    n, out_stride = sums.size(1), 0
+    out = _check_select("select_rows", index, sums, seqlens, seqlens.numel(), sums_out)
+    return _launch_select(index, sums, seqlens, budget, n_first, n_recent, sums_out, out)
+
+
+def _check_select(what: str, index: int, sums, seqlens, b: int, sums_out):
+    """(sequences, positions, row strides of sums and sums_out)."""
+    _check_ints(what, "seqlens", seqlens, (b,), index)
+    n, stride = _check_sums(what, sums, b, index)
+    if sums_out is None:
+        return b, n, stride, 0
     if sums_out is sums:
-        out_stride = stride
-    elif sums_out is not None:
-        out_stride = _check_sums("select_rows", sums_out, b, index)
-        if sums_out.size(1) != n:
-            raise ValueError("select_rows: sums_out must have the shape of sums")
-        if sums_out.data_ptr() == sums.data_ptr() and out_stride != stride:
-            raise ValueError("select_rows: in place, sums_out must be sums")
+        return b, n, stride, stride
+    out_n, out_stride = _check_sums(what, sums_out, b, index)
+    if out_n != n or (sums_out.data_ptr() == sums.data_ptr() and out_stride != stride):
+        raise ValueError(f"{what}: sums_out must have the shape of sums, and be sums or other memory")
+    return b, n, stride, out_stride
+
+
+def _launch_select(index, sums, seqlens, budget, n_first, n_recent, sums_out, sizes):
+    b, n, stride, out_stride = sizes
     keep = torch.empty((b, max(budget, 0)), dtype=torch.int32, device=seqlens.device)
     counts = torch.empty_like(seqlens)
     args = pack_select_args(sums.data_ptr(), seqlens.data_ptr(), keep.data_ptr(), counts.data_ptr(),
@@ -122,13 +130,15 @@ def evict(cache: torch.Tensor, block_table: torch.Tensor, seqlens: torch.Tensor,
     is left to the caller (seqlens.copy_(lens), PagedKVCache.truncate).
     """
     # every refusal comes before the sums are touched
-    dc, dt = _check_move("evict", cache, block_table, dst_cache, dst_table)
-    if seqlens.numel() != dt.size(0) or sums.get_device() != cache.get_device():
-        raise ValueError("evict: one length per block-table row, and all tensors on one device")
-    n = sums.size(-1)
-    if n > block_table.size(1) * cache.size(1) or min(budget, n) > dt.size(1) * dc.size(1):
+    if sums_out is None:
+        sums_out = sums
+    index = cache.get_device()
+    move = _check_move("evict", cache, block_table, dst_cache, dst_table)
+    _, _, (_, page, _, b, max_pages), _, dst_max = move
+    sizes = _check_select("evict", index, sums, seqlens, b, sums_out)
+    n = sizes[1]
+    if n > max_pages * page or min(budget, n) > dst_max * page:
         raise ValueError("evict: a block table does not hold the positions of sums, or the budget")
-    keep, counts = select_rows(sums, seqlens, budget, n_first=n_first, n_recent=n_recent,
-                               sums_out=sums if sums_out is None else sums_out)
-    _launch_keep(cache, block_table, dc, dt, keep, counts, None, None)
+    keep, counts = _launch_select(index, sums, seqlens, budget, n_first, n_recent, sums_out, sizes)
+    _launch_keep(index, cache, block_table, move, keep, budget, counts, 0, 0)
     return keep, counts

@@ -23,7 +23,7 @@ import torch
 
 from ._lib import (call_on, check, data, lib, pack_tree_args, require_cuda, stream_ptr,
                    workspace_size)
-from .cache import _check_device, _check_ints, _check_paged, keep_rows
+from .cache import _check_ints, _check_paged, keep_rows
 
 
 def tree_mask(parents: torch.Tensor) -> torch.Tensor:
@@ -44,17 +44,17 @@ def tree_mask(parents: torch.Tensor) -> torch.Tensor:
 
 
 def _check_step(what: str, q, cache, block_table, seqlens, mask, tree_lens, max_seqlen):
-    """The checks that the attention and the weight sums share.  Returns q
-    contiguous, the mask's sequence stride, (pages, page size, pages of a
-    sequence) and the bound of the lengths."""
+    """The checks that the attention and the weight sums share.  Returns the device
+    index, q contiguous, its shape, the mask's sequence stride, (page size, pages
+    of a sequence, pages) and the bound of the lengths."""
     index = q.get_device()
-    _check_device(what, index, q, cache, block_table, mask)
-    if q.dim() != 4 or q.dtype != torch.bfloat16:
+    if index < 0:
+        require_cuda(q)
+    num_pages, page, width, rows, max_pages = _check_paged(what, index, cache, block_table)
+    shape = q.shape
+    if len(shape) != 4 or q.dtype != torch.bfloat16:
         raise ValueError(f"{what}: q must be bf16 [batch, nodes, heads, width]")
-    _check_paged(what, cache, block_table)
-    b, s, h, d = q.shape
-    num_pages, page, width = cache.shape
-    rows, max_pages = block_table.shape
+    b, s, h, d = shape
     if s == 0 or h == 0:
         raise ValueError(f"{what}: q has no rows")
     if width != d:
@@ -66,17 +66,17 @@ def _check_step(what: str, q, cache, block_table, seqlens, mask, tree_lens, max_
         _check_ints(what, "tree_lens", tree_lens, (b,), index)
     stride = 0
     if mask is not None:
-        shape = mask.shape
-        if shape == (b, s, s):
+        dims = mask.shape
+        if dims == (b, s, s):
             stride = s * s
-        if shape not in ((b, s, s), (s, s)) or not mask.is_contiguous() \
-                or mask.dtype not in (torch.bool, torch.uint8):
+        if dims not in ((b, s, s), (s, s)) or not mask.is_contiguous() \
+                or mask.dtype not in (torch.bool, torch.uint8) or mask.get_device() != index:
             raise ValueError(f"{what}: the mask must be a contiguous bool [batch, nodes, nodes] or "
-                             "[nodes, nodes] tensor")
+                             "[nodes, nodes] tensor on q's device")
     if not q.is_contiguous():
         q = q.contiguous()
     most = max_pages * page if max_seqlen is None else max_seqlen
-    return q, stride, (page, max_pages, num_pages), most
+    return index, q, shape, stride, (page, max_pages, num_pages), most
 
 
 def tree_attn(q: torch.Tensor, cache: torch.Tensor, block_table: torch.Tensor,
@@ -99,20 +99,19 @@ def tree_attn(q: torch.Tensor, cache: torch.Tensor, block_table: torch.Tensor,
     Nodes past tree_lens[i] get zeros and -inf.  max_seqlen bounds seqlens
     (None: what the block table holds) and sizes the launch.
     """
-    q, stride, pages, most = _check_step("tree_attn", q, cache, block_table, seqlens, mask,
-                                         tree_lens, max_seqlen)
-    b, s, h, d = q.shape
+    index, q, (b, s, h, d), stride, pages, most = _check_step(
+        "tree_attn", q, cache, block_table, seqlens, mask, tree_lens, max_seqlen)
     dev = q.device
     sink = attn_sink
     if sink is not None:
-        if sink.numel() != h or sink.device != dev:
+        if sink.numel() != h or sink.get_device() != index:
             raise ValueError("tree_attn: attn_sink needs one value per head, on q's device")
         if sink.dtype != torch.float32 or not sink.is_contiguous():
             sink = sink.to(torch.float32).contiguous()
     if out is None:
         out = torch.empty((b, s, h, 512), dtype=torch.bfloat16, device=dev)
     elif out.shape != (b, s, h, 512) or out.dtype != torch.bfloat16 \
-            or not out.is_contiguous() or out.device != dev:
+            or not out.is_contiguous() or out.get_device() != index:
         raise ValueError("tree_attn: out must be a contiguous bf16 [batch, nodes, heads, 512] tensor")
     lse = torch.empty((b, s, h), dtype=torch.float32, device=dev) if return_lse else None
     need = workspace_size("qcau_tree_attn_workspace_size", b, s, h, most)
@@ -121,7 +120,7 @@ def tree_attn(q: torch.Tensor, cache: torch.Tensor, block_table: torch.Tensor,
         q.data_ptr(), cache.data_ptr(), block_table.data_ptr(), seqlens.data_ptr(),
         data(tree_lens), data(mask), data(sink), out.data_ptr(), data(lse), 0, ws.data_ptr(), stride,
         b, s, h, d, 512, *pages, most, 0, need, softmax_scale, 0)
-    call_on(dev.index, "tree_attn", lib().qcau_tree_attn, args)
+    call_on(index, "tree_attn", lib().qcau_tree_attn, args)
     return (out, lse) if return_lse else out
 
 
