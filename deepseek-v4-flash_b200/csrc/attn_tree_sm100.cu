@@ -15,8 +15,11 @@
 // (5, 48) costs one partly filled group at the end, not padding per node.
 // The pair's tile pipeline is the decode kernel's (attn_decode_sm100.cu): CTA
 // r of the pair owns rows [64 r, 64 r + 64) of the group, tiles of 128 tokens,
-// QK 128 x 128 x d, P rounded to bf16 (the denominator is summed from the fp32
-// P), PV 128 x 256 x 128 twice.
+// QK 128 x 128 x d, P rounded to bf16 at the exact running max of each tile
+// (the denominator is summed from the fp32 P), PV 128 x 256 x 128 twice.  (A
+// maximum raised only past 2^8 spares most rescales of O, 5 % of the time, but
+// the largest P is then no exact 1: errors of 2.0e-3 against 1.7e-3 of the
+// output's norm at 16 x 64 nodes x 16 heads x 32768 tokens.)
 //
 // Schedule: the tiles of all (sequence, group) rows, laid end to end at the
 // batch's own lengths (read on the device: a ragged batch is balanced too),
@@ -50,12 +53,6 @@ constexpr int kVSlot = 32768;         // 64 tokens x this CTA's 256 dims (4 chun
 constexpr int kVSlots = 2;            // the tile's two blocks
 constexpr int kQBytes = 9 * 8192;     // 64 rows x 576 bf16 (9 chunks of 64 rows)
 constexpr int kPBytes = 2 * 8192;     // 64 rows x 128 tokens bf16 (2 chunks of 64 tokens)
-// P is taken relative to a maximum that is raised (and O rescaled) only where a
-// tile exceeds it by more than 2^kRaise: bf16 rounds P to the same relative half
-// step at any scale, and the fp32 sums have room.  Exact maxima cost a rescale in
-// most tiles of random scores: 5 % (9 sequences x 8 nodes x 128 heads x 4096
-// tokens: 79.2 us against 75.2).
-constexpr float kRaise = 8.f;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 
@@ -409,7 +406,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     const int hl = row & 63, half = row >> 6;
     const int et = threadIdx.x - 64;      // 0..127 over warps 2-5
     const uint32_t lane_base = (uint32_t)(quarter * 32) << 16;
-    const float sl2 = p.scale * kLog2e;
+    const float sl2 = p.scale * kLog2e * (1.f + 36 * kTruncPerStep);
     const uint32_t s_free_l[2] = {mapa_shared(smem_u32(&sh->s_free[0]), 0),
                                   mapa_shared(smem_u32(&sh->s_free[1]), 0)};
     const uint32_t p_full_l = mapa_shared(smem_u32(&sh->p_full), 0);
@@ -498,7 +495,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         bool resc = false;
         if (m_run == -INFINITY) {
           m_run = tmax;  // nothing seen yet: O holds zeros (or PV starts a fresh accumulator)
-        } else if (tmax > m_run + kRaise) {
+        } else if (tmax > m_run) {
           alpha = exp2f(m_run - tmax);
           m_run = tmax;
           resc = true;
@@ -761,6 +758,7 @@ TreeShape tree_shape(const TreeArgs& a, int group_rows, int tile, int64_t pairs)
   p.team = p.groups > 1 && pairs == kTreePairs &&
            kTreePairs / p.groups * p.groups >= kTreePairs - 4;
   p.min_tiles = kTreeMinTiles;
+  p.row_cost = kTreeRowCost;
   return p;
 }
 

@@ -209,11 +209,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             const int slot = n % C::kStages, use = n / C::kStages;
             if (!(ok = mbar_wait(&sh->kfull[slot], use & 1, abort))) break;
             // chunk 3g + i: A = this CTA's tokens, B = its N/2 query rows.  The
-            // tensor core truncates a sum to fp32 at every step, so a chain of 36
-            // steps pulls a score towards zero by about 8e-7 of it, which the
-            // exponential turns into 1.4e-5 of the weight of a token with x = 18;
-            // kChains accumulators of kSteps steps each, added in registers with
-            // rounding, divide that by kChains
+            // exponential turns what a score loses in truncated sums (kTruncPerStep)
+            // into a share of the weight: 18 * 4.9e-7 for a token with x = 18 and one
+            // chain of 36 steps.  kChains accumulators of kSteps steps each, added in
+            // registers with rounding, divide it by kChains; the scale takes the mean
+            // of the rest back
             const uint64_t kg = k_desc + (uint64_t)((slot * C::kStage) >> 4);
             const uint64_t qg = q_desc + (uint64_t)((3 * g * C::kQChunk) >> 4);
 #pragma unroll
@@ -255,7 +255,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     const int hl = kSplit ? row & 63 : row, half = kSplit ? row >> 6 : 0;
     const int et = threadIdx.x - 64;
     const uint32_t lane_base = (uint32_t)(quarter * 32) << 16;
-    const float sl2 = p.scale * kLog2e;
+    const float sl2 = p.scale * kLog2e * (1.f + C::kSteps * kTruncPerStep);
     const uint32_t s_free_l[2] = {mapa_shared(smem_u32(&sh->s_free[0]), 0),
                                   mapa_shared(smem_u32(&sh->s_free[1]), 0)};
     const int64_t seq_rows = (int64_t)p.sh.s * p.sh.h;
@@ -456,6 +456,9 @@ cudaError_t launch_attn_weights_sm100(const TreeArgs& a, void* ws, cudaStream_t 
   }
   WeightsParams p{};
   p.sh = tree_shape(a, n, tile, pairs);
+  // a row's start hides behind the K stream where HBM is the bound (64 x 4000 tokens
+  // x 64 heads: 41.8 us against 43.2 with the cost)
+  if (n < 256) p.sh.row_cost = 0;
   p.lse = a.lse;
   p.sums = a.sums;
   p.sums_stride = a.sums_stride;

@@ -5,7 +5,9 @@
 // The query rows of a sequence (its n nodes x h heads) form groups of
 // `group_rows`; a (sequence, group) row has one tile per `tile` cached tokens.
 // The tiles of all rows, laid end to end at the batch's own lengths (read on
-// the device, so a ragged batch is balanced too), are cut into equal ranges.
+// the device, so a ragged batch is balanced too), are cut into equal ranges.  In
+// long ranges a row takes `row_cost` places in front of its tiles, for its Q
+// load and its epilogue, which its tiles do not hide.
 // In the team schedule the tiles of the sequences are cut instead, and each of
 // a team's `groups` pairs runs one group over the team's range.
 #pragma once
@@ -17,6 +19,17 @@ namespace qcau {
 
 constexpr int kTreePairs = 74;  // CTA pairs of a B200 (148 SMs)
 constexpr int kTreeMinTiles = 1;
+// 32 sequences x up to 8 nodes x 128 heads, ragged: 132.6 us with 0, 126.6 with 1,
+// 124.7 with 2, 124.8 with 3.
+constexpr int kTreeRowCost = 2;
+
+// The tensor core truncates an accumulator to fp32 at every MMA step, towards
+// zero: scores come out short by a share that grows with the steps of their chain,
+// half an ulp of the running sum a step on average.  Measured (16384 tokens, rows
+// of standard deviations 1.7 and 4.3): 1.3e-7 of a score in chains of 9 steps,
+// 2.4e-7 in chains of 18, with about as much scatter.  The softmax scale takes the
+// mean back.
+constexpr float kTruncPerStep = 1.35e-8f;
 
 struct TreeShape {
   const int32_t* table;      // [b, max_pages]
@@ -32,6 +45,7 @@ struct TreeShape {
   int groups;       // groups of a sequence at s nodes
   int team;         // 1: the team schedule may be used
   int min_tiles;    // tiles of a range, at least
+  int row_cost;     // what starting a row costs, in tiles (long ranges only)
 };
 
 // Host side (attn_tree_sm100.cu): CTA pairs of a launch, and its shape.
@@ -58,15 +72,16 @@ __device__ __forceinline__ TreeSeq tree_seq(const TreeShape& p, int b) {
 // One piece of work: tiles [t_begin, t_end) of group g of sequence b.
 struct TreePiece {
   int b, g, t_begin, t_end;
-  int row0;  // the row's first tile in the list of all tiles
+  int row0;  // the place of the row's first tile in the list of all rows
   TreeSeq q;
 };
 
-// A pair's walk over its range of tiles [x, x_end).  Every role of the pair
+// A pair's walk over its range of places [x, x_end).  Every role of the pair
 // takes the same walk.
 struct TreeCursor {
-  int b, first;  // current sequence and its first tile in the list
+  int b, first;  // current sequence and its first place in the list
   int x, x_end;
+  int extra;     // places in front of a row's tiles
   int group;     // team schedule: this pair's group; else -1
 };
 
@@ -77,28 +92,31 @@ struct TreeRange {
 };
 
 struct TreePlanShared {
-  long long sum_rows[12], sum_seqs[12];  // per warp (up to 12): tiles of all rows, of all sequences
-  int scan[12];                          // per warp: tiles of a run of sequences
-  int start_b, start_tile;               // first sequence of the range, and its first tile
+  long long sum_rows[8], sum_seqs[8];  // per warp (up to 8): tiles of all rows, of all sequences
+  int num_rows[8], num_seqs[8];        // per warp: rows, sequences that have tiles
+  int scan[8];                         // per warp: tiles of a run of sequences
+  int start_b, start_tile;             // first sequence of the range, and its first tile
 };
 
 __device__ __forceinline__ bool tree_piece(const TreeShape& p, TreeCursor& c, TreePiece& u) {
   while (c.x < c.x_end && c.b < p.b) {
     u.q = tree_seq(p, c.b);
-    const int rows = c.group >= 0 ? 1 : u.q.groups;
-    if (u.q.tiles == 0 || c.x >= c.first + u.q.tiles * rows) {
-      c.first += u.q.tiles * rows;
+    const int rows = c.group >= 0 ? 1 : u.q.groups, places = u.q.tiles + c.extra;
+    if (u.q.tiles == 0 || c.x >= c.first + places * rows) {
+      c.first += u.q.tiles == 0 ? 0 : places * rows;
       c.b++;
       continue;
     }
-    const int k = (c.x - c.first) / u.q.tiles;
+    const int k = (c.x - c.first) / places;
     u.b = c.b;
     u.g = c.group >= 0 ? c.group : k;
-    u.row0 = c.first + k * u.q.tiles;
-    u.t_begin = c.x - u.row0;
+    u.row0 = c.first + k * places + c.extra;
+    u.t_begin = max(c.x - u.row0, 0);
     u.t_end = min(u.q.tiles, c.x_end - u.row0);
-    c.x = u.row0 + u.t_end;
-    if (u.g < u.q.groups) return true;  // a team's pair past the sequence's groups has nothing to do
+    c.x = min(u.row0 + u.q.tiles, c.x_end);
+    // a range that ends in front of a row's tiles leaves the row to the next one, and
+    // a team's pair past the sequence's groups has nothing to do
+    if (u.t_end > u.t_begin && u.g < u.q.groups) return true;
   }
   return false;
 }
@@ -106,19 +124,26 @@ __device__ __forceinline__ bool tree_piece(const TreeShape& p, TreeCursor& c, Tr
 // First half of the plan, before a barrier of the CTA: the batch's tiles.
 __device__ __forceinline__ void tree_plan_sums(const TreeShape& p, TreePlanShared* sh) {
   long long rows = 0, seqs = 0;
+  int nrows = 0, nseqs = 0;
   for (int i = threadIdx.x; i < p.b; i += blockDim.x) {
     const TreeSeq q = tree_seq(p, i);
     rows += (long long)q.tiles * q.groups;
     seqs += q.tiles;
+    nrows += q.groups;
+    nseqs += q.tiles > 0 ? 1 : 0;
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
     rows += __shfl_xor_sync(0xffffffffu, rows, o);
     seqs += __shfl_xor_sync(0xffffffffu, seqs, o);
   }
+  nrows = __reduce_add_sync(0xffffffffu, nrows);
+  nseqs = __reduce_add_sync(0xffffffffu, nseqs);
   if ((threadIdx.x & 31) == 0) {
     sh->sum_rows[threadIdx.x >> 5] = rows;
     sh->sum_seqs[threadIdx.x >> 5] = seqs;
+    sh->num_rows[threadIdx.x >> 5] = nrows;
+    sh->num_seqs[threadIdx.x >> 5] = nseqs;
   }
   if (threadIdx.x == 0) {
     sh->start_b = p.b;
@@ -126,13 +151,13 @@ __device__ __forceinline__ void tree_plan_sums(const TreeShape& p, TreePlanShare
   }
 }
 
-// First tile of range i: floor(i total / nranges), in 32 bits (nranges is small).
+// First place of range i: floor(i total / nranges), in 32 bits (nranges is small).
 __device__ __forceinline__ int tree_cut(const TreeRange& r, int i) {
   const int q = r.total / r.nranges, rem = r.total - q * r.nranges;
   return i * q + i * rem / r.nranges;
 }
 
-// The range that tile x belongs to: the largest i with tree_cut(i) <= x.
+// The range that place x belongs to: the largest i with tree_cut(i) <= x.
 __device__ __forceinline__ int tree_range_of(const TreeRange& r, int x) {
   return (int)(((int64_t)(x + 1) * r.nranges - 1) / r.total);
 }
@@ -143,9 +168,12 @@ __device__ __forceinline__ TreeRange tree_plan_range(const TreeShape& p, TreePla
                                                      int pair, int npairs) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, nwarps = blockDim.x >> 5;
   long long rows = 0, seqs = 0;
+  int nrows = 0, nseqs = 0;
   for (int w = 0; w < nwarps; w++) {
     rows += sh->sum_rows[w];
     seqs += sh->sum_seqs[w];
+    nrows += sh->num_rows[w];
+    nseqs += sh->num_seqs[w];
   }
   TreeRange r;
   // a team runs every group on every sequence's tiles: not worth it where the
@@ -154,6 +182,10 @@ __device__ __forceinline__ TreeRange tree_plan_range(const TreeShape& p, TreePla
   r.tsize = team ? p.groups : 1;
   r.total = (int)(team ? seqs : rows);
   r.nranges = max(1, min(npairs / r.tsize, r.total / p.min_tiles));
+  // ranges of 8 tiles or more: the rows' starts count too
+  const int extra = r.total >= 8 * r.nranges ? p.row_cost : 0;
+  r.total += extra * (team ? nseqs : nrows);
+  r.start.extra = extra;
   r.range = pair / r.tsize;
   const bool busy = r.range < r.nranges;
   r.start.x = busy ? tree_cut(r, r.range) : 0;
@@ -162,14 +194,14 @@ __device__ __forceinline__ TreeRange tree_plan_range(const TreeShape& p, TreePla
   r.start.b = 0;
   r.start.first = 0;
   if (p.b > 1) {
-    // the sequence that tile start.x belongs to: prefix sums of a block's worth of sequences
+    // the sequence that place start.x belongs to: prefix sums of a block's worth of sequences
     int before = 0;
     for (int b0 = 0; b0 < p.b; b0 += blockDim.x) {
       const int i = b0 + threadIdx.x;
       int w = 0;
       if (i < p.b) {
         const TreeSeq q = tree_seq(p, i);
-        w = q.tiles * (team ? 1 : q.groups);
+        w = q.tiles > 0 ? (q.tiles + extra) * (team ? 1 : q.groups) : 0;
       }
       int inc = w;
 #pragma unroll
