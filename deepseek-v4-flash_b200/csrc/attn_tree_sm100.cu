@@ -804,10 +804,10 @@ cudaError_t launch_attn_tree_sm100(const TreeArgs& a, void* ws, cudaStream_t st)
   static std::atomic<uint64_t> done{0};
   cudaError_t e = allow_smem((const void*)attn_tree_sm100_kernel, kSmemBytes, done);
   if (e != cudaSuccess) return e;
-  e = launch_early(attn_tree_sm100_kernel, dim3((unsigned)(2 * pairs)), kThreads, kSmemBytes, st, tq,
-                   tk, tv, p);
+  e = launch_early(attn_tree_sm100_kernel, dim3((unsigned)(2 * pairs)), 1, kThreads, kSmemBytes, st,
+                   tq, tk, tv, p);
   if (e != cudaSuccess || pairs == 1) return e;  // one pair: no row is shared
-  return launch_early(tree_combine_kernel, dim3((unsigned)pairs, 16), 256, 0, st, p);
+  return launch_early(tree_combine_kernel, dim3((unsigned)pairs, 16), 1, 256, 0, st, p);
 }
 
 }  // namespace qcau

@@ -416,7 +416,7 @@ cudaError_t run_weights(const TreeArgs& a, const WeightsParams& p, const CUtenso
   static std::atomic<uint64_t> done{0};
   cudaError_t e = allow_smem((const void*)attn_weights_sm100_kernel<N>, weights_smem<N>(), done);
   if (e != cudaSuccess) return e;
-  return launch_early(attn_weights_sm100_kernel<N>, dim3((unsigned)(2 * pairs)), kThreads,
+  return launch_early(attn_weights_sm100_kernel<N>, dim3((unsigned)(2 * pairs)), 1, kThreads,
                       weights_smem<N>(), st, tq, tk, p);
 }
 
@@ -472,7 +472,8 @@ cudaError_t launch_attn_weights_sm100(const TreeArgs& a, void* ws, cudaStream_t 
                              : run_weights<64>(a, p, tq, tk, pairs, st);
   if (e != cudaSuccess || p.sh.groups == 1) return e;
   return launch_early(weights_combine_kernel,
-                      dim3((unsigned)((a.max_len + 255) / 256), (unsigned)a.b), 256, 0, st, p);
+                      dim3((unsigned)((a.max_len + 255) / 256), (unsigned)a.b), 1, 256, 0, st,
+                      p);
 }
 
 }  // namespace qcau

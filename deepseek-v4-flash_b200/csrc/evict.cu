@@ -283,17 +283,18 @@ __global__ void __launch_bounds__(kSelThreads)
 constexpr int kKeepThreads = 256;
 constexpr int kKeepLoads = 8;  // 16-byte loads in flight per thread
 
-// Block (slice, b) moves one column slice of UNITS x 16 bytes (0: whole rows) of
-// all kept rows of sequence b, in order, some rows a turn: keep is strictly
-// ascending, so row start + i comes from itself or from a later row, and a turn
-// overwrites only rows that this turn or an earlier one has read.  So the move
-// is in place with one barrier a turn (between a turn's loads and its stores),
-// needs no other buffer, and blocks never wait for one another.  A turn's loads
-// are issued before the stores of the turn before it, whose rows lie in front of
-// all that is still to be read; the addresses (two dependent table lookups) are
-// made a turn ahead.  Bound by HBM: 4 d bytes a row moved.
+// A cluster of `spread` blocks moves one column slice of UNITS x 16 bytes (0:
+// whole rows) of all kept rows of sequence b, in order, spread x some rows a turn:
+// keep is strictly ascending, so row start + i comes from itself or from a later
+// row, and a turn overwrites only rows that this turn or an earlier one has read.
+// So the move is in place with one barrier a turn (between a turn's loads and its
+// stores), needs no other buffer, and clusters never wait for one another.  A
+// turn's loads are issued before the stores of the turn before it, whose rows lie
+// in front of all that is still to be read; the addresses (two dependent table
+// lookups) are made a turn ahead.  Bound by HBM: 4 d bytes a row moved (32 x 4096
+// rows of 576 values: 60 us, 5.0 TB/s, random or consecutive, in place or not).
 template <int UNITS>
-__global__ void __launch_bounds__(kKeepThreads) keep_rows_kernel(qcau_keep_args p, int* err) {
+__global__ void __launch_bounds__(kKeepThreads) keep_rows_kernel(qcau_keep_args p, int spread, int* err) {
   constexpr int U = kKeepLoads;
   constexpr int kMaxRows = UNITS ? kKeepThreads * U / UNITS : 128;
   __shared__ int from[2][kMaxRows], to[2][kMaxRows];  // cache rows, or -1
@@ -302,7 +303,8 @@ __global__ void __launch_bounds__(kKeepThreads) keep_rows_kernel(qcau_keep_args 
   const int row_units = (int)(p.d / 8);
   const int units = UNITS ? UNITS : row_units;             // of this block's slice
   const int rows = UNITS ? kMaxRows : min(kMaxRows, kKeepThreads * U / row_units);  // a turn
-  const int unit0 = UNITS ? blockIdx.x * UNITS : 0;
+  const int unit0 = UNITS ? blockIdx.x / spread * UNITS : 0;
+  const int share = blockIdx.x % spread;  // this block's rows of a turn
   const int start = p.start ? p.start[b] : 0, page = (int)p.page_size;
   const int room = (int)(p.max_pages * p.page_size), dst_room = (int)(p.dst_max_pages * p.page_size);
   int count = p.counts[b];
@@ -315,7 +317,7 @@ __global__ void __launch_bounds__(kKeepThreads) keep_rows_kernel(qcau_keep_args 
   const bool same = p.cache == p.dst_cache && p.block_table == p.dst_table;
   auto place = [&](int turn) {
     for (int r = tid; r < rows; r += kKeepThreads) {
-      const int i = turn * rows + r;
+      const int i = (turn * spread + share) * rows + r;
       int f = -1, t = -1;
       if (i < count) {
         const int k = keep[i], before = i > 0 ? keep[i - 1] : -1, at = start + k, row = start + i;
@@ -366,24 +368,30 @@ __global__ void __launch_bounds__(kKeepThreads) keep_rows_kernel(qcau_keep_args 
     for (int u = 0; u < U; u++)
       if (w.t[u] >= 0) dst[(int64_t)w.t[u] * row_units + unit_of[u]] = w.v[u];
   };
-  const int turns = (count + rows - 1) / rows;
+  const int turns = (count + rows * spread - 1) / (rows * spread);
+  auto barrier = [&]() {
+    if (spread > 1)
+      cluster_sync();
+    else
+      __syncthreads();
+  };
   if (turns > 0) {
     Turn even, odd;
     place(0);
     __syncthreads();
     load(0, even);
     if (turns > 1) place(1);
-    __syncthreads();
+    barrier();
     for (int turn = 0; turn < turns; turn += 2) {
       if (turn + 1 < turns) load(turn + 1, odd);
       store(even);
       if (turn + 2 < turns) place(turn + 2);
-      __syncthreads();
+      barrier();
       if (turn + 1 >= turns) break;
       if (turn + 2 < turns) load(turn + 2, even);
       store(odd);
       if (turn + 3 < turns) place(turn + 3);
-      __syncthreads();
+      barrier();
     }
   }
   if (bad) raise_dev_error(err, QCAU_DEVERR_INDEX);
@@ -401,7 +409,7 @@ cudaError_t launch_tree_mask(const int32_t* parents, uint8_t* mask, int64_t b, i
 
 cudaError_t launch_evict_select(const qcau_select_args& a, cudaStream_t st) {
   auto run = [&](auto kernel) {
-    return launch_early(kernel, dim3((unsigned)a.b), kSelThreads, 0, st, a, device_error_word());
+    return launch_early(kernel, dim3((unsigned)a.b), 1, kSelThreads, 0, st, a, device_error_word());
   };
   if (a.max_seqlen <= 4 * kSelThreads) return run(evict_select_kernel<4>);
   if (a.max_seqlen <= 8 * kSelThreads) return run(evict_select_kernel<8>);
@@ -413,16 +421,25 @@ cudaError_t launch_evict_select(const qcau_select_args& a, cudaStream_t st) {
 cudaError_t launch_keep_rows(const qcau_keep_args& a, cudaStream_t st) {
   int* err = device_error_word();
   const int64_t units = a.d / 8;  // 16-byte units of a row
-  auto run = [&](auto kernel, int64_t slices) {
-    return launch_early(kernel, dim3((unsigned)slices, (unsigned)a.b), kKeepThreads, 0, st, a, err);
+  auto run = [&](auto kernel, int64_t slices, int64_t spread) {
+    return launch_early(kernel, dim3((unsigned)(slices * spread), (unsigned)a.b), (unsigned)spread,
+                        kKeepThreads, 0, st, a, (int)spread, err);
   };
-  // few rows (a commit): a block takes whole rows, up to 28 of 576 values a turn.
-  // Many: 128-byte slices, or narrower ones (down to a 32-byte sector) where
-  // the blocks would leave SMs idle
-  if (a.k <= 64 && units <= kKeepThreads) return run(keep_rows_kernel<0>, 1);
-  if (units % 8 == 0 && a.b * (units / 8) >= 148) return run(keep_rows_kernel<8>, units / 8);
-  if (units % 4 == 0 && a.b * (units / 4) >= 148) return run(keep_rows_kernel<4>, units / 4);
-  return run(keep_rows_kernel<2>, units / 2);
+  // few rows (a commit): a block takes whole rows, up to 28 of 576 values a turn
+  if (a.k <= 64 && units <= kKeepThreads) return run(keep_rows_kernel<0>, 1, 1);
+  // 128-byte slices, narrower ones (down to a 32-byte sector) while the blocks leave
+  // SMs idle; then clusters of up to 8 blocks a slice, while each block has several
+  // turns left (8192 rows kept of 1 sequence: 14 us, 31 unclustered; a cluster costs
+  // some 2 us, more than the one turn of 1024 rows)
+  const int64_t most = 2 * 148;
+  int64_t width = units % 8 == 0 ? 8 : units % 4 == 0 ? 4 : 2;
+  while (width > 2 && a.b * (units / width) * 2 <= most) width /= 2;
+  const int64_t turns = (a.k * width + kKeepThreads * kKeepLoads - 1) / (kKeepThreads * kKeepLoads);
+  int64_t spread = 1;
+  while (spread < 8 && turns >= 4 * spread && a.b * (units / width) * spread * 2 <= most) spread *= 2;
+  if (width == 8) return run(keep_rows_kernel<8>, units / 8, spread);
+  if (width == 4) return run(keep_rows_kernel<4>, units / 4, spread);
+  return run(keep_rows_kernel<2>, units / 2, spread);
 }
 
 }  // namespace qcau

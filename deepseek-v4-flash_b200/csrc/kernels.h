@@ -27,20 +27,23 @@ cudaError_t allow_smem(const void* kernel, size_t bytes, std::atomic<uint64_t>& 
 
 // Launches a kernel that may be set up while the one before it in the stream
 // still runs: the kernel calls cudaGridDependencySynchronize() in every thread
-// before it touches global memory, and so ends after that one has.
+// before it touches global memory, and so ends after that one has.  `cluster`:
+// blocks of a cluster along x (1: none, or what the kernel itself declares).
 template <typename... P, typename... A>
-cudaError_t launch_early(void (*kernel)(P...), dim3 grid, unsigned threads, size_t smem,
-                         cudaStream_t st, A... args) {
-  cudaLaunchAttribute attr;
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr.val.programmaticStreamSerializationAllowed = 1;
+cudaError_t launch_early(void (*kernel)(P...), dim3 grid, unsigned cluster, unsigned threads,
+                         size_t smem, cudaStream_t st, A... args) {
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim = {cluster, 1, 1};
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = grid;
   cfg.blockDim = dim3(threads, 1, 1);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = cluster > 1 ? 2 : 1;
   return cudaLaunchKernelEx(&cfg, kernel, P(args)...);
 }
 

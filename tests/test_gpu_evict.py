@@ -180,7 +180,8 @@ def test_lengths_out_of_range_are_flagged():
 
 
 @pytest.mark.parametrize("lens,budget,d,page", [([700, 64, 1500, 1], 300, 576, 64), ([5000], 2000, 576, 64),
-                                                ([900, 3000], 2999, 512, 128), ([300] * 40, 100, 64, 16)])
+                                                ([900, 3000], 2999, 512, 128), ([300] * 40, 100, 64, 16),
+                                                ([12000], 9001, 576, 64), ([9000, 9500, 20], 8000, 512, 128)])
 @pytest.mark.parametrize("inplace", [True, False])
 def test_evict_moves_rows_and_sums(lens, budget, d, page, inplace):
     cache, table, rows = R.paged(lens, d, page, seed=2, stale=3.0)
