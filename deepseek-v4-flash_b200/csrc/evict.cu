@@ -9,6 +9,7 @@
 //  * keep_rows: row start + keep[i] of a sequence to row start + i, for i in
 //    order, through the block table (in place, or into another cache).
 #include <algorithm>
+#include <cmath>
 
 #include "common.cuh"
 #include "kernels.h"
@@ -282,19 +283,22 @@ __global__ void __launch_bounds__(kSelThreads)
 
 constexpr int kKeepThreads = 256;
 constexpr int kKeepLoads = 8;  // 16-byte loads in flight per thread
+constexpr int64_t kKeepSlots = 4 * 148;  // blocks that run at once
 
 // A cluster of `spread` blocks moves one column slice of UNITS x 16 bytes (0:
 // whole rows) of all kept rows of sequence b, in order, spread x some rows a turn:
 // keep is strictly ascending, so row start + i comes from itself or from a later
 // row, and a turn overwrites only rows that this turn or an earlier one has read.
 // So the move is in place with one barrier a turn (between a turn's loads and its
-// stores), needs no other buffer, and clusters never wait for one another.  A
-// turn's loads are issued before the stores of the turn before it, whose rows lie
-// in front of all that is still to be read; the addresses (two dependent table
-// lookups) are made a turn ahead.  Bound by HBM: 4 d bytes a row moved (32 x 4096
-// rows of 576 values: 60 us, 5.0 TB/s, random or consecutive, in place or not).
+// stores), needs no other buffer, and clusters never wait for one another.  The
+// addresses (two dependent table lookups) are made while the turn before is read,
+// and four blocks an SM overlap one another's loads and stores (turns double-
+// buffered in registers, at two blocks an SM, took 92 us for 33 x 4096 rows of 576
+// values against 62, and 14 against 9 for 8192 rows of one sequence).  Bound by
+// HBM: 4 d bytes a row moved (32 x 4096 rows: 60 us, 5.0 TB/s; 128 x 1024: 57 us, 5.3;
+// random or consecutive rows, in place or not).
 template <int UNITS>
-__global__ void __launch_bounds__(kKeepThreads) keep_rows_kernel(qcau_keep_args p, int spread, int* err) {
+__global__ void __launch_bounds__(kKeepThreads, 4) keep_rows_kernel(qcau_keep_args p, int spread, int* err) {
   constexpr int U = kKeepLoads;
   constexpr int kMaxRows = UNITS ? kKeepThreads * U / UNITS : 128;
   __shared__ int from[2][kMaxRows], to[2][kMaxRows];  // cache rows, or -1
@@ -376,22 +380,14 @@ __global__ void __launch_bounds__(kKeepThreads) keep_rows_kernel(qcau_keep_args 
       __syncthreads();
   };
   if (turns > 0) {
-    Turn even, odd;
+    Turn w;
     place(0);
     __syncthreads();
-    load(0, even);
-    if (turns > 1) place(1);
-    barrier();
-    for (int turn = 0; turn < turns; turn += 2) {
-      if (turn + 1 < turns) load(turn + 1, odd);
-      store(even);
-      if (turn + 2 < turns) place(turn + 2);
+    for (int turn = 0; turn < turns; turn++) {
+      load(turn, w);
+      if (turn + 1 < turns) place(turn + 1);
       barrier();
-      if (turn + 1 >= turns) break;
-      if (turn + 2 < turns) load(turn + 2, even);
-      store(odd);
-      if (turn + 3 < turns) place(turn + 3);
-      barrier();
+      store(w);
     }
   }
   if (bad) raise_dev_error(err, QCAU_DEVERR_INDEX);
@@ -427,16 +423,31 @@ cudaError_t launch_keep_rows(const qcau_keep_args& a, cudaStream_t st) {
   };
   // few rows (a commit): a block takes whole rows, up to 28 of 576 values a turn
   if (a.k <= 64 && units <= kKeepThreads) return run(keep_rows_kernel<0>, 1, 1);
-  // 128-byte slices, narrower ones (down to a 32-byte sector) while the blocks leave
-  // SMs idle; then clusters of up to 8 blocks a slice, while each block has several
-  // turns left (8192 rows kept of 1 sequence: 14 us, 31 unclustered; a cluster costs
-  // some 2 us, more than the one turn of 1024 rows)
-  const int64_t most = 2 * 148;
-  int64_t width = units % 8 == 0 ? 8 : units % 4 == 0 ? 4 : 2;
-  while (width > 2 && a.b * (units / width) * 2 <= most) width /= 2;
-  const int64_t turns = (a.k * width + kKeepThreads * kKeepLoads - 1) / (kKeepThreads * kKeepLoads);
-  int64_t spread = 1;
-  while (spread < 8 && turns >= 4 * spread && a.b * (units / width) * spread * 2 <= most) spread *= 2;
+  // Slices of 128 bytes or narrower (down to a 32-byte sector), in clusters of up to
+  // 8 blocks: the pair with the least estimated time (us) from B200 timings of 1 to
+  // 128 sequences: waves of four blocks per SM, each 6 us of set-up (2 more in a
+  // cluster) and 2 us a turn; and not below the bytes at 5.4 TB/s (less in fewer than
+  // 360 blocks, a quarter more time in slices under 128 bytes) and a last wave.
+  const double bytes_us = (double)a.b * (double)a.k * (double)a.d * 4 / 5.4e6;
+  int64_t width = 0, spread = 1;
+  double best = 1e300;
+  for (int64_t w = 8; w >= 2; w /= 2) {
+    if (units % w) continue;
+    const int64_t turns = (a.k * w + kKeepThreads * kKeepLoads - 1) / (kKeepThreads * kKeepLoads);
+    for (int64_t n = 1; n <= 8 && n <= turns; n++) {
+      const int64_t blocks = a.b * (units / w) * n, waves = (blocks + kKeepSlots - 1) / kKeepSlots;
+      const double wave = 6 + (n > 1 ? 2 : 0) + 2.0 * (double)((turns + n - 1) / n);
+      const double us = std::max((double)waves * wave,
+                                 bytes_us * (w == 8 ? 1.0 : 1.25) *
+                                         std::sqrt(std::max(1.0, 360.0 / (double)blocks)) +
+                                     (waves > 1 ? wave : 0.0));
+      if (us < best) {
+        best = us;
+        width = w;
+        spread = n;
+      }
+    }
+  }
   if (width == 8) return run(keep_rows_kernel<8>, units / 8, spread);
   if (width == 4) return run(keep_rows_kernel<4>, units / 4, spread);
   return run(keep_rows_kernel<2>, units / 2, spread);
