@@ -1488,7 +1488,7 @@ int check_tree(const TreeArgs& a, int64_t d_v, const char* name) {
   if (a.b >= 65536 || a.s >= (1 << 24) || a.h >= (1 << 24) || rows >= (1 << 24) ||
       a.max_len >= (1LL << 31) - 256 || a.max_pages * a.page_size >= (1LL << 31) ||
       a.num_pages >= (1LL << 31) / (a.page_size / 64) ||
-      a.b * ((rows + 63) / 64) * tiles >= (1LL << 31))
+      a.b * ((rows + 63) / 64) * tiles >= (1LL << 30))
     return fail(QCAU_ERR_UNSUPPORTED, who + ": batch too large for one call");
   QCAU_CHECK_ARG(((reinterpret_cast<uintptr_t>(a.q) | reinterpret_cast<uintptr_t>(a.cache)) & 15) == 0,
                  who + ": q and cache must be 16-byte aligned");

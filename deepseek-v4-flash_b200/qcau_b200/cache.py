@@ -258,7 +258,9 @@ class PagedKVCache:
     def truncate(self, seqs: Sequence[int], lengths: Sequence[int]) -> None:
         """Shorten sequences to their first lengths[i] tokens (the rows that
         keep_rows left after an eviction, or the tokens accepted at a drafting
-        step's end) and return the pages they no longer need."""
+        step's end) and return the pages they no longer need.  positions()
+        counts cached rows: after an eviction the caller's own count of tokens
+        gives the positions of new ones."""
         for s, n in zip(seqs, lengths):
             if not 0 <= n <= self._len[s]:
                 raise ValueError(f"sequence {s} has {self._len[s]} tokens, cannot keep {n}")
