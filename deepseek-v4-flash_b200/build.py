@@ -1,10 +1,11 @@
-"""Build libqcau_b200.so (all CUDA sources, sm_100a) in-tree with nvcc.
+"""Build libqcau_b200.so (all CUDA sources, sm_100a) in-tree with nvcc, and the
+Python binding of its short calls (csrc/bind.cpp, against torch's headers) with g++.
 
     python deepseek-v4-flash_b200/build.py [--jobs N] [--verbose-ptxas] [--force]
 
 Objects go to deepseek-v4-flash_b200/_build/, the shared library to
-deepseek-v4-flash_b200/qcau_b200/libqcau_b200.so.  A source is recompiled when
-it or any header under csrc/ or include/ is newer than its object.
+deepseek-v4-flash_b200/qcau_b200/libqcau_b200.so and _bind.so beside it.  A source
+is recompiled when it or any header under csrc/ or include/ is newer than its object.
 """
 from __future__ import annotations
 
@@ -13,6 +14,7 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
@@ -21,6 +23,7 @@ REPO = PKG_DIR.parent
 CSRC = PKG_DIR / "csrc"
 BUILD = PKG_DIR / "_build"
 LIB = PKG_DIR / "qcau_b200" / "libqcau_b200.so"
+BIND = PKG_DIR / "qcau_b200" / "_bind.so"
 SOURCES = ["capi.cu", "act_quant.cu", "rope_norm.cu", "fp8_gemm.cu", "bmm.cu",
            "attn_combine.cu", "attn_decode_sm100.cu", "attn_gather_sm100.cu", "kv_build.cu", "indexer.cu", "compress.cu",
            "indexer_score_sm100.cu", "attn_tree_sm100.cu", "attn_weights_sm100.cu", "evict.cu"]
@@ -69,7 +72,30 @@ def build(jobs: int = 8, verbose_ptxas: bool = False, force: bool = False) -> Pa
         r = subprocess.run(cmd, capture_output=True, text=True)
         if r.returncode != 0:
             raise RuntimeError(f"link failed:\n{r.stdout}\n{r.stderr}")
+    build_bind(force)
     return LIB
+
+
+def build_bind(force: bool = False) -> None:
+    """_bind.so: calls libqcau_b200.so (beside it) on torch tensors."""
+    src = CSRC / "bind.cpp"
+    if not force and BIND.exists() and BIND.stat().st_mtime >= max(src.stat().st_mtime,
+                                                                  _headers_mtime()):
+        return
+    import torch
+
+    root = Path(torch.__file__).resolve().parent
+    cuda = Path(nvcc()).resolve().parent.parent
+    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", "-DUSE_CUDA",
+           "-I", str(REPO / "include"), "-I", str(root / "include"),
+           "-I", str(root / "include" / "torch" / "csrc" / "api" / "include"),
+           "-I", str(cuda / "include"), "-I", sysconfig.get_paths()["include"], str(src),
+           "-o", str(BIND), "-L", str(root / "lib"), "-ltorch_python", "-ltorch_cuda", "-ltorch_cpu",
+           "-lc10_cuda", "-lc10", "-L", str(LIB.parent), f"-l:{LIB.name}", "-Wl,-rpath,$ORIGIN"]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"binding failed:\n{r.stdout}\n{r.stderr}")
 
 
 if __name__ == "__main__":

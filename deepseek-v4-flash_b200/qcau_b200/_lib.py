@@ -7,8 +7,6 @@ present, the call raises.
 from __future__ import annotations
 
 import ctypes
-import functools
-import struct
 from pathlib import Path
 
 import torch
@@ -47,6 +45,36 @@ class MlaDims(ctypes.Structure):
         ("max_pages", _I64), ("num_pages", _I64), ("max_seqlen", _I64), ("npos", _I64),
         ("softmax_scale", _F), ("w_scale_dtype", _I32), ("act_round_scale", _I32),
         ("out_dtype", _I32),
+    ]
+
+
+class TreeArgs(ctypes.Structure):
+    """qcau_tree_args of the header."""
+    _fields_ = [
+        *((n, _P) for n in ("q", "cache", "block_table", "seqlens", "tree_lens", "tree_mask",
+                            "attn_sink", "o", "lse", "sums", "workspace")),
+        *((n, _I64) for n in ("mask_seq_stride", "b", "s", "h", "d_qk", "d_v", "page_size",
+                              "max_pages", "num_pages", "max_seqlen", "sums_stride")),
+        ("workspace_bytes", ctypes.c_uint64), ("softmax_scale", _F), ("accumulate", _I32),
+    ]
+
+
+class SelectArgs(ctypes.Structure):
+    """qcau_select_args of the header."""
+    _fields_ = [
+        *((n, _P) for n in ("sums", "seqlens", "keep", "counts", "sums_out")),
+        *((n, _I64) for n in ("sums_stride", "out_stride", "b", "max_seqlen", "budget", "n_first",
+                              "n_recent")),
+    ]
+
+
+class KeepArgs(ctypes.Structure):
+    """qcau_keep_args of the header."""
+    _fields_ = [
+        *((n, _P) for n in ("cache", "block_table", "dst_cache", "dst_table", "keep", "counts",
+                            "start", "lens_out")),
+        *((n, _I64) for n in ("max_pages", "num_pages", "dst_max_pages", "dst_num_pages",
+                              "keep_stride", "b", "k", "d", "page_size")),
     ]
 
 
@@ -123,19 +151,12 @@ SIGNATURES = {
     "qcau_index_lists": ([_P, _I64, _I64, _I64, _I64, _I64, _I64, _P, _I64, _P], ctypes.c_int),
     "qcau_tree_mask": ([_P, _P, _I64, _I64, _P], ctypes.c_int),
     "qcau_tree_attn_workspace_size": ([_I64, _I64, _I64, _I64], _SZ),
-    "qcau_tree_attn": ([_P, _P], ctypes.c_int),
+    "qcau_tree_attn": ([ctypes.POINTER(TreeArgs), _P], ctypes.c_int),
     "qcau_attn_weight_sums_workspace_size": ([_I64, _I64, _I64, _I64], _SZ),
-    "qcau_attn_weight_sums": ([_P, _P], ctypes.c_int),
-    "qcau_evict_select": ([_P, _P], ctypes.c_int),
-    "qcau_keep_rows": ([_P, _P], ctypes.c_int),
+    "qcau_attn_weight_sums": ([ctypes.POINTER(TreeArgs), _P], ctypes.c_int),
+    "qcau_evict_select": ([ctypes.POINTER(SelectArgs), _P], ctypes.c_int),
+    "qcau_keep_rows": ([ctypes.POINTER(KeepArgs), _P], ctypes.c_int),
 }
-
-# Argument structs of the header, packed by struct (a twentieth of the time that
-# ctypes takes to convert as many arguments): qcau_tree_args, qcau_select_args
-# and qcau_keep_args; a NULL pointer is 0.
-pack_tree_args = struct.Struct("@11P11qQfi").pack
-pack_select_args = struct.Struct("@5P7q").pack
-pack_keep_args = struct.Struct("@8P9q").pack
 
 _lib = None
 
@@ -160,6 +181,23 @@ def lib() -> ctypes.CDLL:
     return _lib
 
 
+_bind = None
+
+
+def bind():
+    """The compiled binding of the short calls (csrc/bind.cpp).  Raises if it has
+    not been built."""
+    global _bind
+    if _bind is None:
+        try:
+            from . import _bind as module
+        except ImportError as e:
+            raise ImportError(f"{Path(__file__).resolve().parent / '_bind.so'} does not load: build "
+                              "it with `python deepseek-v4-flash_b200/build.py`") from e
+        _bind = module
+    return _bind
+
+
 def check(rc: int, what: str) -> None:
     """Map a qcau_status to the reference's exception types."""
     if rc == QCAU_OK:
@@ -174,32 +212,6 @@ def check(rc: int, what: str) -> None:
 
 def stream_ptr(device: torch.device | None = None) -> int:
     return torch.cuda.current_stream(device).cuda_stream
-
-
-def call_on(index: int, what: str, fn, args: bytes) -> None:
-    """check(fn(args, stream)) with device `index` current and its current stream.
-
-    For the short calls of a decode step: the device is switched only when
-    another one is current (the context manager alone costs about 2 us), and the
-    stream is read without building a Stream object."""
-    if index == torch._C._cuda_getDevice():
-        rc = fn(args, torch._C._cuda_getCurrentRawStream(index))
-    else:
-        with torch.cuda.device(index):
-            rc = fn(args, torch._C._cuda_getCurrentRawStream(index))
-    if rc != QCAU_OK:
-        check(rc, what)
-
-
-@functools.lru_cache(maxsize=1024)
-def workspace_size(name: str, *sizes: int) -> int:
-    """A *_workspace_size() of the library, which depends on the sizes alone."""
-    return getattr(lib(), name)(*sizes)
-
-
-def data(t: torch.Tensor | None) -> int:
-    """The address of a tensor as a packed argument: 0 for None."""
-    return 0 if t is None else t.data_ptr()
 
 
 def ptr(t: torch.Tensor | None) -> int | None:

@@ -113,50 +113,6 @@ def window_slots(bsz: int, seqlen: int, start_pos: int, window: int, ring_rows: 
     return out.to(torch.int32).reshape(-1)
 
 
-# The checks of the paged-cache operators are on the path of short decode steps:
-# each attribute is read once, and messages are made only to be raised.
-
-
-def _check_paged(what: str, index: int, cache: torch.Tensor, block_table: torch.Tensor):
-    """(pages, page, width, sequences, pages of a sequence) of a cache and its
-    block table on CUDA device `index`."""
-    if cache.get_device() != index or block_table.get_device() != index or index < 0:
-        require_cuda(cache, block_table)
-        raise ValueError(f"{what}: all tensors must be on one device")
-    shape, rows = cache.shape, block_table.shape
-    if len(shape) != 3 or cache.dtype != torch.bfloat16 or not cache.is_contiguous():
-        raise ValueError(f"{what}: the cache must be a contiguous bf16 [pages, page, width] tensor")
-    if len(rows) != 2 or block_table.dtype != torch.int32 or not block_table.is_contiguous():
-        raise ValueError(f"{what}: the block table must be a contiguous int32 [batch, pages] tensor")
-    return (*shape, *rows)
-
-
-def _check_ints(what: str, name: str, t: torch.Tensor, shape: tuple, index: int) -> None:
-    if t.dtype != torch.int32 or t.shape != shape or not t.is_contiguous() or t.get_device() != index:
-        raise ValueError(f"{what}: {name} must be a contiguous int32 {list(shape)} tensor on the "
-                         "device of the others")
-
-
-def _check_move(what: str, cache, block_table, dst_cache, dst_table):
-    """Where rows go to, checked with where they come from: (destination cache and
-    block table, the sizes of _check_paged, the destination's pages and pages of a
-    sequence)."""
-    index = cache.get_device()
-    sizes = _check_paged(what, index, cache, block_table)
-    num_pages, page, d, b, max_pages = sizes
-    if d % 16:
-        raise ValueError(f"{what}: the row width must be a multiple of 16")
-    if dst_cache is None and dst_table is None:
-        return cache, block_table, sizes, num_pages, max_pages
-    dc = cache if dst_cache is None else dst_cache
-    dt = block_table if dst_table is None else dst_table
-    dst_pages, dst_page, dst_d, dst_b, dst_max = _check_paged(what, index, dc, dt)
-    if dst_page != page or dst_d != d or dst_b != b:
-        raise ValueError(f"{what}: one row per sequence in both block tables, and caches of one page "
-                         "size and width are needed")
-    return dc, dt, sizes, dst_pages, dst_max
-
-
 def keep_rows(cache: torch.Tensor, block_table: torch.Tensor, keep: torch.Tensor,
               counts: torch.Tensor, *, start: Optional[torch.Tensor] = None,
               dst_cache: Optional[torch.Tensor] = None, dst_table: Optional[torch.Tensor] = None,
@@ -175,25 +131,7 @@ def keep_rows(cache: torch.Tensor, block_table: torch.Tensor, keep: torch.Tensor
     counts.  An offset out of range or out of order is not copied and raises the
     device error bit DEVERR_INDEX.
     """
-    move = _check_move("keep_rows", cache, block_table, dst_cache, dst_table)
-    index, b, k = cache.get_device(), move[2][3], keep.size(-1)
-    _check_ints("keep_rows", "keep", keep, (b, k), index)
-    _check_ints("keep_rows", "counts", counts, (b,), index)
-    if start is not None:
-        _check_ints("keep_rows", "start", start, (b,), index)
-    if seqlens is not None:
-        _check_ints("keep_rows", "seqlens", seqlens, (b,), index)
-    if k == 0:
-        raise ValueError("keep_rows: keep has no columns")
-    _launch_keep(index, cache, block_table, move, keep, k, counts, _lib.data(start), _lib.data(seqlens))
-
-
-def _launch_keep(index, cache, block_table, move, keep, k, counts, start, seqlens) -> None:
-    dc, dt, (num_pages, page, d, b, max_pages), dst_pages, dst_max = move
-    args = _lib.pack_keep_args(
-        cache.data_ptr(), block_table.data_ptr(), dc.data_ptr(), dt.data_ptr(), keep.data_ptr(),
-        counts.data_ptr(), start, seqlens, max_pages, num_pages, dst_max, dst_pages, k, b, k, d, page)
-    _lib.call_on(index, "keep_rows", lib().qcau_keep_rows, args)
+    _lib.bind().keep_rows(cache, block_table, keep, counts, start, dst_cache, dst_table, seqlens)
 
 
 class PagedKVCache:

@@ -39,7 +39,7 @@ def test_tree_attn_refusals():
                 ws_bytes=1 << 30, scale=0.07, accumulate=0)
 
     def call(**change):
-        return L.qcau_tree_attn(_lib.pack_tree_args(*{**good, **change}.values()), None)
+        return L.qcau_tree_attn(_lib.TreeArgs(*{**good, **change}.values()), None)
 
     _expect(L.qcau_tree_attn(None, None), ValueError, "NULL")
 
@@ -66,7 +66,7 @@ def test_weight_sums_refusals():
                 ws_bytes=0, scale=0.07, accumulate=0)
 
     def call(**change):
-        return L.qcau_attn_weight_sums(_lib.pack_tree_args(*{**good, **change}.values()), None)
+        return L.qcau_attn_weight_sums(_lib.TreeArgs(*{**good, **change}.values()), None)
 
     _expect(L.qcau_attn_weight_sums(None, None), ValueError, "NULL")
 
@@ -86,7 +86,7 @@ def test_select_and_keep_refusals():
                 first=2, recent=3)
 
     def select(**change):
-        return L.qcau_evict_select(_lib.pack_select_args(*{**good, **change}.values()), None)
+        return L.qcau_evict_select(_lib.SelectArgs(*{**good, **change}.values()), None)
 
     _expect(L.qcau_evict_select(None, None), ValueError, "NULL")
 
@@ -99,7 +99,7 @@ def test_select_and_keep_refusals():
                      num_pages=8, dst_max_pages=4, dst_num_pages=8, keep_stride=5, b=1, k=5, d=576, page=64)
 
     def rows(**change):
-        return L.qcau_keep_rows(_lib.pack_keep_args(*{**good_rows, **change}.values()), None)
+        return L.qcau_keep_rows(_lib.KeepArgs(*{**good_rows, **change}.values()), None)
 
     _expect(L.qcau_keep_rows(None, None), ValueError, "NULL")
 
