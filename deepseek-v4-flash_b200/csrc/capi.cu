@@ -1601,7 +1601,7 @@ int qcau_evict_select(const qcau_select_args* args, void* stream) {
                  "evict_select: the budget must hold n_first and n_recent tokens");
   QCAU_CHECK_ARG(t.sums_stride >= t.max_seqlen && (t.sums_out == nullptr || t.out_stride >= t.max_seqlen),
                  "evict_select: a row of sums must hold max_seqlen values");
-  if (t.b >= (1LL << 31) || t.max_seqlen >= (1LL << 31) - 65536 || t.budget >= (1LL << 31) - 65536)
+  if (t.b >= (1LL << 27) || t.max_seqlen >= (1LL << 30) || t.budget >= (1LL << 31) - 65536)
     return fail(QCAU_ERR_UNSUPPORTED, "evict_select: batch too large for one call");
   if (t.b == 0) return QCAU_OK;
   QCAU_CHECK_CUDA(launch_evict_select(t, to_stream(stream)));

@@ -65,7 +65,23 @@ struct SelShared {
   uint32_t count[32 * kSelWarps];  // kept-token counts per (j, warp): above the bar | at it << 16
   uint32_t scan[2][kSelWarps];
   int pick[3];
+  uint32_t total;                // this block's kept-token counts, packed as `count`
 };
+
+// Word of the same shared variable in block `rank` of the cluster.
+__device__ __forceinline__ uint32_t peer_u32(const void* p, int rank) {
+  uint32_t v;
+  asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(mapa_shared(smem_u32(p), rank)) : "memory");
+  return v;
+}
+__device__ __forceinline__ int2 peer_int2(const void* p, int rank) {
+  int2 v;
+  asm volatile("ld.shared::cluster.v2.u32 {%0, %1}, [%2];"
+               : "=r"(v.x), "=r"(v.y)
+               : "r"(mapa_shared(smem_u32(p), rank))
+               : "memory");
+  return v;
+}
 
 __device__ __forceinline__ void select_clear(SelShared* sh) {
   for (int i = threadIdx.x; i < 3 * kBins; i += kSelThreads) (&sh->hist[0][0])[i] = 0;
@@ -76,9 +92,10 @@ __device__ __forceinline__ void select_clear(SelShared* sh) {
 // the digits so far, and the bin that holds the budget-th key.  A bin that ends
 // exactly there ends the search.  visit(f) calls f(key) for each of the thread's
 // keys (0: none).  Starts behind select_clear and a barrier; a digit costs three
-// barriers, which is most of its time after the first.
+// barriers, which is most of its time after the first.  The `blocks` blocks of a
+// cluster add up their histograms, each for itself.
 template <typename Visit>
-__device__ __forceinline__ uint32_t select_bar(SelShared* sh, int budget, Visit visit) {
+__device__ __forceinline__ uint32_t select_bar(SelShared* sh, int budget, int blocks, Visit visit) {
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   uint32_t prefix = 0, known = 0;
   int want = budget;
@@ -90,10 +107,21 @@ __device__ __forceinline__ uint32_t select_bar(SelShared* sh, int budget, Visit 
       if (k != 0 && (k & known) == prefix)
         atomicAdd(&hist[(k >> shift) & ((1u << width) - 1u)], 1);
     });
-    __syncthreads();
     // thread i owns bins 2047 - 2i and 2046 - 2i
-    const int2 h = *reinterpret_cast<const int2*>(&hist[kBins - 2 - 2 * tid]);
-    const int h0 = h.y, h1 = h.x;
+    int h0 = 0, h1 = 0;
+    if (blocks > 1) {
+      cluster_sync();
+      for (int r = 0; r < blocks; r++) {
+        const int2 h = peer_int2(&hist[kBins - 2 - 2 * tid], r);
+        h0 += h.y;
+        h1 += h.x;
+      }
+    } else {
+      __syncthreads();
+      const int2 h = *reinterpret_cast<const int2*>(&hist[kBins - 2 - 2 * tid]);
+      h0 = h.y;
+      h1 = h.x;
+    }
     int inc = h0 + h1;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -119,28 +147,33 @@ __device__ __forceinline__ uint32_t select_bar(SelShared* sh, int budget, Visit 
   return prefix;
 }
 
-// One block per sequence, its keys in registers: value j of thread i is token
-// j * 1024 + i.  One read of the sums (all loads in flight at once, past the
-// length they read the last sum again); select_bar works on the registers and
-// shared-memory histograms; then each kept token's place is the number of kept
-// tokens before it, from ballots and one scan over (j, warp).  Latency-bound: a
-// sequence is one SM's work (64 KB at 16384 tokens).
-template <int V>
+// A cluster of `blocks` blocks per sequence, its keys in registers: value j of
+// thread i of block r is token (r V + j) * 1024 + i.  One read of the sums (all
+// loads in flight at once, past the length they read the last sum again);
+// select_bar works on the registers and shared-memory histograms (kCluster: more than
+// one block); then each kept
+// token's place is the number of kept tokens before it, from ballots, one scan over
+// (j, warp) and the totals of the blocks before.  Bound by the instructions of one
+// SM (16384 sums in one block: 10 us) and, split further, by latencies.
+template <int V, bool kCluster>
 __global__ void __launch_bounds__(kSelThreads)
-    evict_select_kernel(qcau_select_args p, int* err) {
+    evict_select_kernel(qcau_select_args p, int cluster, int* err) {
+  const int blocks = kCluster ? cluster : 1;
   __shared__ __align__(16) SelShared shared;
   SelShared* sh = &shared;
   select_clear(sh);
   cudaGridDependencySynchronize();
   cudaTriggerProgrammaticLaunchCompletion();  // the move of the rows may be launched; it waits
-  const int b = blockIdx.x, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int b = blockIdx.x / blocks, rank = blockIdx.x % blocks;
   const int max_len = (int)p.max_seqlen, budget = (int)p.budget;
   const int n_first = (int)p.n_first, n_recent = (int)p.n_recent;
+  const int token0 = rank * V * kSelThreads + tid;
   int len = p.seqlens[b];
   const float* src = p.sums + b * p.sums_stride;
   float x[V];
 #pragma unroll
-  for (int j = 0; j < V; j++) x[j] = src[min(j * kSelThreads + tid, max_len - 1)];
+  for (int j = 0; j < V; j++) x[j] = src[min(token0 + j * kSelThreads, max_len - 1)];
   if (len < 0 || len > max_len) {
     if (tid == 0) raise_dev_error(err, QCAU_DEVERR_INDEX);
     len = min(max(len, 0), max_len);
@@ -149,14 +182,14 @@ __global__ void __launch_bounds__(kSelThreads)
   uint32_t key[V];
 #pragma unroll
   for (int j = 0; j < V; j++) {
-    const int i = j * kSelThreads + tid;
+    const int i = token0 + j * kSelThreads;
     key[j] = i >= len ? 0u : i < n_first || i >= len - n_recent ? 0xffffffffu : sum_key(x[j]);
   }
   const int count = min(len, budget);
   uint32_t bar = 1;  // every token's key is above it
   __syncthreads();
-  if (len > budget)
-    bar = select_bar(sh, budget, [&](auto f) {
+  if (len > budget)  // the same in all blocks of the cluster
+    bar = select_bar(sh, budget, blocks, [&](auto f) {
 #pragma unroll
       for (int j = 0; j < V; j++) f(key[j]);
     });
@@ -180,11 +213,28 @@ __global__ void __launch_bounds__(kSelThreads)
   if (lane == 31) sh->scan[0][warp] = inc;
   __syncthreads();
   const uint32_t sums = sh->scan[0][lane];
-  const int total_gt = (int)(__reduce_add_sync(0xffffffffu, sums) & 0xffffu);
+  const uint32_t total = __reduce_add_sync(0xffffffffu, sums);
   if (tid < V * kSelWarps)
     sh->count[tid] = inc - mine + __reduce_add_sync(0xffffffffu, lane < warp ? sums : 0u);
+  int total_gt = (int)(total & 0xffffu), prior_gt = 0, prior_eq = 0;
+  // behind the barrier all sums of this sequence are read: sums_out may be sums
+  if (blocks > 1) {
+    if (tid == 0) sh->total = total;
+    cluster_sync();
+    total_gt = 0;
+    for (int r = 0; r < blocks; r++) {
+      const uint32_t t = peer_u32(&sh->total, r);
+      total_gt += (int)(t & 0xffffu);
+      if (r < rank) {
+        prior_gt += (int)(t & 0xffffu);
+        prior_eq += (int)(t >> 16);
+      }
+    }
+    cluster_arrive();  // no block leaves while another reads its shared memory
+  } else {
+    __syncthreads();
+  }
   const int ties = count - total_gt;  // of the tokens at the bar, the first ones
-  __syncthreads();  // the values of this sequence are all read: sums_out may be sums
   int32_t* kp = p.keep + (int64_t)b * budget;
   float* out = p.sums_out ? p.sums_out + b * p.out_stride : nullptr;
 #pragma unroll
@@ -192,17 +242,19 @@ __global__ void __launch_bounds__(kSelThreads)
     const uint32_t k = key[j], before = sh->count[j * kSelWarps + warp];
     const unsigned g = __ballot_sync(0xffffffffu, k > bar), e = __ballot_sync(0xffffffffu, k == bar);
     const unsigned lt = (1u << lane) - 1u;
-    const int before_eq = (int)(before >> 16) + __popc(e & lt);
-    const int pos = (int)(before & 0xffffu) + __popc(g & lt) + min(before_eq, ties);
+    const int before_eq = prior_eq + (int)(before >> 16) + __popc(e & lt);
+    const int pos = prior_gt + (int)(before & 0xffffu) + __popc(g & lt) + min(before_eq, ties);
     if (k > bar || (k == bar && before_eq < ties)) {
-      kp[pos] = j * kSelThreads + tid;
+      kp[pos] = token0 + j * kSelThreads;
       if (out) out[pos] = x[j];
     }
   }
-  for (int i = count + tid; i < budget; i += kSelThreads) kp[i] = -1;
+  const int step = blocks * kSelThreads, at = rank * kSelThreads + tid;
+  for (int i = count + at; i < budget; i += step) kp[i] = -1;
   if (out)
-    for (int i = count + tid; i < max_len; i += kSelThreads) out[i] = 0.f;
-  if (tid == 0) p.counts[b] = count;
+    for (int i = count + at; i < max_len; i += step) out[i] = 0.f;
+  if (at == 0) p.counts[b] = count;
+  if (blocks > 1) cluster_wait();
 }
 
 // Sequences longer than the registers hold: the sums are read again (from L2) for
@@ -233,7 +285,7 @@ __global__ void __launch_bounds__(kSelThreads)
   uint32_t bar = 1;
   int total_gt = len;  // tokens above the bar
   if (len > budget) {
-    bar = select_bar(sh, budget, [&](auto f) {
+    bar = select_bar(sh, budget, 1, [&](auto f) {
 #pragma unroll 8
       for (int i = tid; i < len; i += kSelThreads) f(rank_key(i, src[i]));
     });
@@ -404,14 +456,25 @@ cudaError_t launch_tree_mask(const int32_t* parents, uint8_t* mask, int64_t b, i
 }
 
 cudaError_t launch_evict_select(const qcau_select_args& a, cudaStream_t st) {
-  auto run = [&](auto kernel) {
-    return launch_early(kernel, dim3((unsigned)a.b), 1, kSelThreads, 0, st, a, device_error_word());
+  int* err = device_error_word();
+  // one block up to 8192 sums (7.5 us against 7.8 in two); then clusters of up to 8
+  // blocks of 4096, one block per SM in all (one sequence of 16384: 8.8 us, 11.1 in one
+  // block; of 32768: 11.7, 23.1); fuller ones for more sequences or longer ones (of
+  // 131072: 17.6 us, 174 where the sums are read again for each digit)
+  int64_t blocks = 1;
+  if (a.max_seqlen > 8 * kSelThreads)
+    while (blocks < 8 && blocks * 4 * kSelThreads < a.max_seqlen && 2 * blocks * a.b <= 148) blocks *= 2;
+  while (blocks < 8 && blocks * 32 * kSelThreads < a.max_seqlen) blocks *= 2;
+  const int64_t values = (a.max_seqlen + blocks * kSelThreads - 1) / (blocks * kSelThreads);
+  auto run = [&](auto single, auto clustered) {
+    return launch_early(blocks > 1 ? clustered : single, dim3((unsigned)(a.b * blocks)),
+                        (unsigned)blocks, kSelThreads, 0, st, a, (int)blocks, err);
   };
-  if (a.max_seqlen <= 4 * kSelThreads) return run(evict_select_kernel<4>);
-  if (a.max_seqlen <= 8 * kSelThreads) return run(evict_select_kernel<8>);
-  if (a.max_seqlen <= 16 * kSelThreads) return run(evict_select_kernel<16>);
-  if (a.max_seqlen <= 32 * kSelThreads) return run(evict_select_kernel<32>);
-  return run(evict_select_long_kernel);
+  if (values <= 4) return run(evict_select_kernel<4, false>, evict_select_kernel<4, true>);
+  if (values <= 8) return run(evict_select_kernel<8, false>, evict_select_kernel<8, true>);
+  if (values <= 16) return run(evict_select_kernel<16, false>, evict_select_kernel<16, true>);
+  if (values <= 32) return run(evict_select_kernel<32, false>, evict_select_kernel<32, true>);
+  return launch_early(evict_select_long_kernel, dim3((unsigned)a.b), 1, kSelThreads, 0, st, a, err);
 }
 
 cudaError_t launch_keep_rows(const qcau_keep_args& a, cudaStream_t st) {

@@ -133,7 +133,7 @@ def plain_select(sums, lens, budget, n_first, n_recent):
     return keep
 
 
-@pytest.mark.parametrize("width", [1, 65, 1024, 4096, 4097, 16384, 16385, 32768, 32769, 70001])
+@pytest.mark.parametrize("width", [1, 65, 1024, 4096, 4097, 8193, 16384, 16385, 32768, 32769, 70001, 270001])
 @pytest.mark.parametrize("kind", ["random", "ties", "equal", "specials"])
 def test_selection_equals_the_stable_sort(width, kind):
     g = torch.Generator().manual_seed(width)
@@ -166,6 +166,20 @@ def test_selection_equals_the_stable_sort(width, kind):
         again, _ = select_rows(dev, n, budget, n_first=first, n_recent=recent, sums_out=dev)
         assert torch.equal(again, keep) and torch.equal(torch.nan_to_num(dev, nan=7.0), torch.nan_to_num(out, nan=7.0))
     assert _lib.device_error() == 0
+
+
+@pytest.mark.parametrize("b,width", [(160, 5000), (80, 9000), (40, 20000), (160, 40000)])
+def test_selection_of_many_sequences(b, width):
+    """More sequences than SMs: one block each, or clusters of two and four."""
+    g = torch.Generator().manual_seed(b)
+    lens = torch.randint(1, width + 1, (b,), generator=g).tolist()
+    lens[0] = width
+    sums = torch.randint(0, 3000, (b, width), generator=g).float()
+    budget = width // 3
+    keep, counts = select_rows(sums.cuda(), torch.tensor(lens, dtype=torch.int32, device="cuda"), budget, n_first=2,
+                               n_recent=7)
+    assert torch.equal(keep.cpu(), plain_select(sums, lens, budget, 2, 7))
+    assert counts.tolist() == [min(n, budget) for n in lens]
 
 
 def test_lengths_out_of_range_are_flagged():
