@@ -47,6 +47,7 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kTile = 128;            // tokens per tile (two blocks of 64, one per CTA for K)
+using Cut = TreeCut<128, kTile>;
 constexpr int kKSlot = 24576;         // this CTA's 64 tokens x 3 chunks of 64 dims (one box)
 constexpr int kKSlots = 3;            // 9 chunks = 576 dims (8 = 512: the last box ends in zeros)
 constexpr int kVSlot = 32768;         // 64 tokens x this CTA's 256 dims (4 chunks, one box)
@@ -171,14 +172,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     tma_prefetch_desc(&tm_v);
   }
   cudaGridDependencySynchronize();
-  tree_plan_sums(p.sh, &sh->plan);
+  tree_plan_sums<Cut>(p.sh, &sh->plan);
   if (warp == 1) tmem_alloc<2>(&sh->tmem_base, kTmemCols);
   tc_fence_before();
   cluster_sync();
   tc_fence_after();
   const uint32_t tmem = sh->tmem_base;
 
-  const TreeRange range = tree_plan_range(p.sh, &sh->plan, pair, npairs);
+  const TreeRange range = tree_plan_range<Cut>(p.sh, &sh->plan, pair, npairs);
   cudaTriggerProgrammaticLaunchCompletion();  // the merge may be launched; it waits for this grid
 
   if (warp == 0) {
@@ -191,7 +192,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       bool ok = true;
       TreeCursor c = range.start;
       TreePiece u;
-      while (ok && tree_piece(p.sh, c, u)) {
+      while (ok && tree_piece<Cut>(p.sh, c, u)) {
         for (int t = u.t_begin; t < u.t_end && ok; t++, gt++) {
           const int blk = tree_block(p.sh, u, 2 * t + (int)rank);
           for (int i = 0; i < kKSlots; i++) {
@@ -233,7 +234,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     bool ok = true;
     TreeCursor c = range.start;
     TreePiece u;
-    while (ok && tree_piece(p.sh, c, u)) {
+    while (ok && tree_piece<Cut>(p.sh, c, u)) {
       const int base = u.q.len - u.q.n;
       for (int t = u.t_begin; t < u.t_end && ok; t++, gt++) {
 #pragma unroll
@@ -316,7 +317,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         const uint32_t idesc_qk = make_idesc(128, 128, kFmtBF16, kFmtBF16, false, false);
         const uint64_t q_desc = make_sdesc(q_addr, 16, 1024), k_desc = make_sdesc(k_addr, 16, 1024);
         int gt = 0, nu = 0;  // tiles, pieces
-        while (ok && tree_piece(p.sh, cur, u)) {
+        while (ok && tree_piece<Cut>(p.sh, cur, u)) {
           if (!(ok = mbar_wait(&sh->q_full, nu & 1, abort))) break;
           for (int t = u.t_begin; t < u.t_end && ok; t++, gt++) {
             const int sb = gt & 1;
@@ -357,7 +358,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         const uint32_t idesc_pv = make_idesc(128, 256, kFmtBF16, kFmtBF16, false, true);
         const uint64_t p_desc = make_sdesc(p_addr, 16, 1024), v_desc = make_sdesc(v_addr, 8192, 1024);
         int gt = 0, nu = 0;
-        while (ok && tree_piece(p.sh, cur, u)) {
+        while (ok && tree_piece<Cut>(p.sh, cur, u)) {
           // the first PV of a piece overwrites O: the previous epilogue has read it
           if (nu > 0 && !(ok = mbar_wait<true>(&sh->o_free, (nu - 1) & 1, abort))) break;
           for (int t = u.t_begin; t < u.t_end && ok; t++, gt++) {
@@ -417,7 +418,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     // (CTA c: sequence c mod b, together with the other CTAs of that sequence)
     const int parts = max((int)gridDim.x / p.sh.b, 1), part = blockIdx.x / p.sh.b;
     for (int b = blockIdx.x % p.sh.b; b < p.sh.b && part < parts; b += gridDim.x) {
-      const int64_t r0 = (int64_t)tree_seq(p.sh, b).n * p.sh.h;
+      const int64_t r0 = (int64_t)tree_seq<Cut>(p.sh, b).n * p.sh.h;
       uint4* o = reinterpret_cast<uint4*>(p.out + ((int64_t)b * seq_rows + r0) * 512);
       for (int64_t i = part * 128 + et; i < (seq_rows - r0) * 64; i += parts * 128)
         o[i] = make_uint4(0u, 0u, 0u, 0u);
@@ -431,7 +432,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     bool ok = true;
     TreeCursor c = range.start;
     TreePiece u;
-    while (ok && tree_piece(p.sh, c, u)) {
+    while (ok && tree_piece<Cut>(p.sh, c, u)) {
       const int base = u.q.len - u.q.n;
       const int my_row = u.g * 128 + (int)rank * 64 + hl;  // row of the sequence
       const bool mine = my_row < u.q.n * p.sh.h;
@@ -736,7 +737,7 @@ int64_t tree_pairs(const TreeArgs& a, int group_rows, int tile) {
   return n < 1 ? 1 : (n < kTreePairs ? n : kTreePairs);
 }
 
-TreeShape tree_shape(const TreeArgs& a, int group_rows, int tile, int64_t pairs) {
+TreeShape tree_shape(const TreeArgs& a, int group_rows, int64_t pairs) {
   TreeShape p{};
   p.table = a.block_table;
   p.seqlens = a.seqlens;
@@ -751,8 +752,6 @@ TreeShape tree_shape(const TreeArgs& a, int group_rows, int tile, int64_t pairs)
   p.h = (int)a.h;
   p.max_len = (int)a.max_len;
   p.page_blocks = (int)(a.page_size / 64);
-  p.tile = tile;
-  p.group_rows = group_rows;
   p.groups = (int)((a.s * a.h + group_rows - 1) / group_rows);
   // teams of `groups` pairs when they leave at most 4 of the 74 pairs idle
   p.team = p.groups > 1 && pairs == kTreePairs &&
@@ -763,12 +762,12 @@ TreeShape tree_shape(const TreeArgs& a, int group_rows, int tile, int64_t pairs)
 }
 
 size_t attn_tree_workspace(const TreeArgs& a) {
-  return (size_t)tree_pairs(a, 128, kTile) * (2 * 128 * (512 + 2) * 4 + 16);
+  return (size_t)tree_pairs(a, Cut::kGroupRows, kTile) * (2 * 128 * (512 + 2) * 4 + 16);
 }
 
 cudaError_t launch_attn_tree_sm100(const TreeArgs& a, void* ws, cudaStream_t st) {
   const int64_t rows = a.s * a.h;
-  const int64_t pairs = tree_pairs(a, 128, kTile);
+  const int64_t pairs = tree_pairs(a, Cut::kGroupRows, kTile);
   CUtensorMap tq, tk, tv;
   {
     // Q as [b][chunks][rows][64 values]: a CTA's 64 rows in one box
@@ -792,7 +791,7 @@ cudaError_t launch_attn_tree_sm100(const TreeArgs& a, void* ws, cudaStream_t st)
                  CU_TENSOR_MAP_SWIZZLE_128B))
     return cudaErrorInvalidValue;
   TreeParams p{};
-  p.sh = tree_shape(a, 128, kTile, pairs);
+  p.sh = tree_shape(a, Cut::kGroupRows, pairs);
   p.out = reinterpret_cast<__nv_bfloat16*>(a.o);
   p.lse = a.lse;
   p.sink = a.sink;

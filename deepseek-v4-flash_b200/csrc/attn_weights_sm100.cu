@@ -98,6 +98,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     attn_weights_sm100_kernel(const __grid_constant__ CUtensorMap tm_q,
                               const __grid_constant__ CUtensorMap tm_k, WeightsParams p) {
   using C = WeightsCfg<N>;
+  using Cut = TreeCut<N, C::kTile>;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t pad = (1024u - (smem_u32(smem_raw) & 1023u)) & 1023u;
   uint8_t* sQ = smem_raw + pad;
@@ -130,13 +131,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     tma_prefetch_desc(&tm_k);
   }
   cudaGridDependencySynchronize();
-  tree_plan_sums(p.sh, &sh->plan);
+  tree_plan_sums<Cut>(p.sh, &sh->plan);
   if (warp == 1) tmem_alloc<2>(&sh->tmem_base, C::kTmemCols);
   tc_fence_before();
   cluster_sync();
   tc_fence_after();
   const uint32_t tmem = sh->tmem_base;
-  const TreeRange range = tree_plan_range(p.sh, &sh->plan, pair, npairs);
+  const TreeRange range = tree_plan_range<Cut>(p.sh, &sh->plan, pair, npairs);
   cudaTriggerProgrammaticLaunchCompletion();
 
   if (warp == 0) {
@@ -149,7 +150,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       bool ok = true;
       TreeCursor c = range.start;
       TreePiece u;
-      while (ok && tree_piece(p.sh, c, u)) {
+      while (ok && tree_piece<Cut>(p.sh, c, u)) {
         for (int t = u.t_begin; t < u.t_end && ok; t++) {
           int blk[C::kBlocks];
 #pragma unroll
@@ -197,7 +198,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       bool ok = true;
       TreeCursor c = range.start;
       TreePiece u;
-      while (ok && tree_piece(p.sh, c, u)) {
+      while (ok && tree_piece<Cut>(p.sh, c, u)) {
         if (!(ok = mbar_wait(&sh->q_full, nu & 1, abort))) break;
         for (int t = u.t_begin; t < u.t_end && ok; t++, gt++) {
           const int sb = gt & 1;
@@ -264,7 +265,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     // positions that no token of the step can see: zero, unless sums are added to
     if (!p.accumulate)
       for (int b = blockIdx.x; b < p.sh.b; b += gridDim.x) {
-        const TreeSeq q = tree_seq(p.sh, b);
+        const TreeSeq q = tree_seq<Cut>(p.sh, b);
         for (int i = (q.n > 0 ? q.len : 0) + et; i < p.sh.max_len; i += 128)
           p.sums[b * p.sums_stride + i] = 0.f;
       }
@@ -273,7 +274,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     bool ok = true;
     TreeCursor c = range.start;
     TreePiece u;
-    while (ok && tree_piece(p.sh, c, u)) {
+    while (ok && tree_piece<Cut>(p.sh, c, u)) {
       const int base = u.q.len - u.q.n;
       const int col0 = u.g * N + half * C::kCols;  // first row of this thread's columns
       const int ncol = min(max(u.q.n * p.sh.h - col0, 0), C::kCols);
@@ -392,10 +393,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 }
 
 // The groups' partial sums of a token, in group order.
+// (Only groups of 256 rows leave several.)
 __global__ void __launch_bounds__(256) weights_combine_kernel(WeightsParams p) {
+  using Cut = TreeCut<256, WeightsCfg<256>::kTile>;
   cudaGridDependencySynchronize();
   const int b = blockIdx.y, tok = blockIdx.x * 256 + threadIdx.x;
-  const TreeSeq q = tree_seq(p.sh, b);
+  const TreeSeq q = tree_seq<Cut>(p.sh, b);
   if (q.groups < 2 || tok >= q.len) return;
   float w = 0.f;
 #pragma unroll 8
@@ -455,7 +458,7 @@ cudaError_t launch_attn_weights_sm100(const TreeArgs& a, void* ws, cudaStream_t 
       return cudaErrorInvalidValue;
   }
   WeightsParams p{};
-  p.sh = tree_shape(a, n, tile, pairs);
+  p.sh = tree_shape(a, n, pairs);
   // a row's start hides behind the K stream where HBM is the bound (64 x 4000 tokens
   // x 64 heads: 41.8 us against 43.2 with the cost)
   if (n < 256) p.sh.row_cost = 0;

@@ -3,7 +3,7 @@
 // attention and the attention weight sums.
 //
 // The query rows of a sequence (its n nodes x h heads) form groups of
-// `group_rows`; a (sequence, group) row has one tile per `tile` cached tokens.
+// kGroupRows; a (sequence, group) row has one tile per kTile cached tokens.
 // The tiles of all rows, laid end to end at the batch's own lengths (read on
 // the device, so a ragged batch is balanced too), are cut into equal ranges.  In
 // long ranges a row takes `row_cost` places in front of its tiles, for its Q
@@ -40,8 +40,6 @@ struct TreeShape {
   int64_t max_pages, num_pages, mask_stride;
   int b, s, h, max_len;
   int page_blocks;  // 64-token blocks of a page
-  int tile;         // tokens of a tile (a multiple of 64)
-  int group_rows;
   int groups;       // groups of a sequence at s nodes
   int team;         // 1: the team schedule may be used
   int min_tiles;    // tiles of a range, at least
@@ -50,7 +48,14 @@ struct TreeShape {
 
 // Host side (attn_tree_sm100.cu): CTA pairs of a launch, and its shape.
 int64_t tree_pairs(const TreeArgs& a, int group_rows, int tile);
-TreeShape tree_shape(const TreeArgs& a, int group_rows, int tile, int64_t pairs);
+TreeShape tree_shape(const TreeArgs& a, int group_rows, int64_t pairs);
+
+// The kernel's cut of the work: rows of a group, tokens of a tile (both constants,
+// so that what every role computes before its first load has no division by them).
+template <int kRows, int kTokens>
+struct TreeCut {
+  static constexpr int kGroupRows = kRows, kTile = kTokens;
+};
 
 struct TreeSeq {
   int len, n, tiles, groups;
@@ -58,14 +63,15 @@ struct TreeSeq {
 
 // Lengths of one sequence.  What the caller's arrays may not hold (a length
 // past max_len, more nodes than tokens or than s) is cut to what they may.
+template <typename Cut>
 __device__ __forceinline__ TreeSeq tree_seq(const TreeShape& p, int b) {
   TreeSeq q;
   const int len = p.seqlens[b], n = p.tree_lens ? p.tree_lens[b] : p.s;
   q.len = min(max(len, 0), p.max_len);
   q.n = min(min(max(n, 0), p.s), q.len);
   if (q.len != len || q.n != n) raise_dev_error(p.err, QCAU_DEVERR_INDEX);
-  q.groups = (q.n * p.h + p.group_rows - 1) / p.group_rows;
-  q.tiles = q.n > 0 ? (q.len + p.tile - 1) / p.tile : 0;
+  q.groups = (q.n * p.h + Cut::kGroupRows - 1) / Cut::kGroupRows;
+  q.tiles = q.n > 0 ? (q.len + Cut::kTile - 1) / Cut::kTile : 0;
   return q;
 }
 
@@ -98,9 +104,10 @@ struct TreePlanShared {
   int start_b, start_tile;             // first sequence of the range, and its first tile
 };
 
+template <typename Cut>
 __device__ __forceinline__ bool tree_piece(const TreeShape& p, TreeCursor& c, TreePiece& u) {
   while (c.x < c.x_end && c.b < p.b) {
-    u.q = tree_seq(p, c.b);
+    u.q = tree_seq<Cut>(p, c.b);
     const int rows = c.group >= 0 ? 1 : u.q.groups, places = u.q.tiles + c.extra;
     if (u.q.tiles == 0 || c.x >= c.first + places * rows) {
       c.first += u.q.tiles == 0 ? 0 : places * rows;
@@ -122,11 +129,12 @@ __device__ __forceinline__ bool tree_piece(const TreeShape& p, TreeCursor& c, Tr
 }
 
 // First half of the plan, before a barrier of the CTA: the batch's tiles.
+template <typename Cut>
 __device__ __forceinline__ void tree_plan_sums(const TreeShape& p, TreePlanShared* sh) {
   long long rows = 0, seqs = 0;
   int nrows = 0, nseqs = 0;
   for (int i = threadIdx.x; i < p.b; i += blockDim.x) {
-    const TreeSeq q = tree_seq(p, i);
+    const TreeSeq q = tree_seq<Cut>(p, i);
     rows += (long long)q.tiles * q.groups;
     seqs += q.tiles;
     nrows += q.groups;
@@ -164,6 +172,7 @@ __device__ __forceinline__ int tree_range_of(const TreeRange& r, int x) {
 
 // Second half, after that barrier (all threads of the CTA): this pair's range.
 // Every CTA sums the same lengths, so all take one plan.
+template <typename Cut>
 __device__ __forceinline__ TreeRange tree_plan_range(const TreeShape& p, TreePlanShared* sh,
                                                      int pair, int npairs) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, nwarps = blockDim.x >> 5;
@@ -200,7 +209,7 @@ __device__ __forceinline__ TreeRange tree_plan_range(const TreeShape& p, TreePla
       const int i = b0 + threadIdx.x;
       int w = 0;
       if (i < p.b) {
-        const TreeSeq q = tree_seq(p, i);
+        const TreeSeq q = tree_seq<Cut>(p, i);
         w = q.tiles > 0 ? (q.tiles + extra) * (team ? 1 : q.groups) : 0;
       }
       int inc = w;
@@ -236,12 +245,14 @@ __device__ __forceinline__ TreeRange tree_plan_range(const TreeShape& p, TreePla
 __device__ __forceinline__ int tree_block(const TreeShape& p, const TreePiece& u, int blk) {
   const int used = (u.q.len + 63) / 64;
   if (blk >= used) blk = used - 1;
-  const int64_t e = p.table[(int64_t)u.b * p.max_pages + blk / p.page_blocks];
+  // pages of one block, the usual ones, need no division
+  const int page = p.page_blocks == 1 ? blk : blk / p.page_blocks;
+  const int64_t e = p.table[(int64_t)u.b * p.max_pages + page];
   if (e < 0 || e >= p.num_pages) {
     raise_dev_error(p.err, QCAU_DEVERR_INDEX);
     return 0;
   }
-  return (int)(e * p.page_blocks + blk % p.page_blocks);
+  return (int)(e * p.page_blocks + blk - page * p.page_blocks);
 }
 
 // All lanes wait; the warp agrees on the outcome (timeouts are per lane).
