@@ -588,21 +588,24 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           const int64_t orow = u.b * seq_rows + my_row;
           uint8_t* po = reinterpret_cast<uint8_t*>(p.out + (u.b * seq_rows + warp_row) * 512 + 256 * half);
 #pragma unroll 1
-          for (int c = 0; c < 4; c++) {  // 64 dims
-            float v[64];
+          for (int c = 0; c < 4; c += 2) {  // 2 x 64 dims, loaded together
+            float v[2][64];
 #pragma unroll
-            for (int k = 0; k < 2; k++)
+            for (int k = 0; k < 4; k++)
               tmem_ld32(tmem + lane_base + kTmemO + 64 * c + 32 * k,
-                        *reinterpret_cast<float(*)[32]>(v + 32 * k));
+                        *reinterpret_cast<float(*)[32]>(&v[0][0] + 32 * k));
 #pragma unroll
-            for (int k = 0; k < 2; k++) tmem_ld_wait_regs(v + 32 * k);
+            for (int k = 0; k < 4; k++) tmem_ld_wait_regs(&v[0][0] + 32 * k);
 #pragma unroll
-            for (int k = 0; k < 8; k++)
-              put(k, make_uint4(pack_bf16(v[8 * k] * inv, v[8 * k + 1] * inv),
-                                pack_bf16(v[8 * k + 2] * inv, v[8 * k + 3] * inv),
-                                pack_bf16(v[8 * k + 4] * inv, v[8 * k + 5] * inv),
-                                pack_bf16(v[8 * k + 6] * inv, v[8 * k + 7] * inv)));
-            turn(po + 128 * c, 1024);
+            for (int j = 0; j < 2; j++) {
+#pragma unroll
+              for (int k = 0; k < 8; k++)
+                put(k, make_uint4(pack_bf16(v[j][8 * k] * inv, v[j][8 * k + 1] * inv),
+                                  pack_bf16(v[j][8 * k + 2] * inv, v[j][8 * k + 3] * inv),
+                                  pack_bf16(v[j][8 * k + 4] * inv, v[j][8 * k + 5] * inv),
+                                  pack_bf16(v[j][8 * k + 6] * inv, v[j][8 * k + 7] * inv)));
+              turn(po + 128 * (c + j), 1024);
+            }
           }
           if (p.lse && half == 0 && mine) p.lse[orow] = lse;
         } else {
@@ -611,15 +614,20 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           const int64_t prow0 = ((int64_t)pair * 2 + (first ? 1 : 0)) * 128 + rank * 64;
           uint8_t* po = reinterpret_cast<uint8_t*>(p.part_o + (prow0 + (quarter & 1) * 32) * 512 + 256 * half);
 #pragma unroll 1
-          for (int c = 0; c < 8; c++) {  // 32 dims
-            float v[32];
-            tmem_ld32(tmem + lane_base + kTmemO + c * 32, v);
-            tmem_ld_wait_regs(v);
+          for (int c = 0; c < 8; c += 4) {  // 4 x 32 dims, loaded together
+            float v[4][32];
 #pragma unroll
-            for (int k = 0; k < 8; k++)
-              put(k, make_uint4(__float_as_uint(v[4 * k]), __float_as_uint(v[4 * k + 1]),
-                                __float_as_uint(v[4 * k + 2]), __float_as_uint(v[4 * k + 3])));
-            turn(po + 128 * c, 2048);
+            for (int j = 0; j < 4; j++) tmem_ld32(tmem + lane_base + kTmemO + (c + j) * 32, v[j]);
+#pragma unroll
+            for (int j = 0; j < 4; j++) tmem_ld_wait_regs(v[j]);
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+#pragma unroll
+              for (int k = 0; k < 8; k++)
+                put(k, make_uint4(__float_as_uint(v[j][4 * k]), __float_as_uint(v[j][4 * k + 1]),
+                                  __float_as_uint(v[j][4 * k + 2]), __float_as_uint(v[j][4 * k + 3])));
+              turn(po + 128 * (c + j), 2048);
+            }
           }
           if (half == 0)
             *reinterpret_cast<float2*>(p.part_ml + (prow0 + hl) * 2) = make_float2(m_run, l_tot);
