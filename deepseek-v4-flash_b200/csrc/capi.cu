@@ -1472,7 +1472,7 @@ namespace {
 int check_tree(const TreeArgs& a, int64_t d_v, const char* name) {
   const std::string who(name);
   QCAU_CHECK_ARG(a.b >= 0 && a.s >= 1 && a.h >= 1 && a.page_size > 0 && a.max_pages > 0 &&
-                     a.num_pages > 0,
+                     a.num_pages > 0 && a.max_pages < (1LL << 31) && a.page_size < (1LL << 31),
                  who + ": bad shape");
   QCAU_CHECK_ARG(a.max_len >= 1 && a.max_len <= a.max_pages * a.page_size,
                  who + ": max_seqlen must be at least 1 and within the block table");
@@ -1493,6 +1493,11 @@ int check_tree(const TreeArgs& a, int64_t d_v, const char* name) {
   QCAU_CHECK_ARG(((reinterpret_cast<uintptr_t>(a.q) | reinterpret_cast<uintptr_t>(a.cache)) & 15) == 0,
                  who + ": q and cache must be 16-byte aligned");
   return QCAU_OK;
+}
+
+bool overlap(const void* x, int64_t x_bytes, const void* y, int64_t y_bytes) {
+  const uintptr_t a = reinterpret_cast<uintptr_t>(x), b = reinterpret_cast<uintptr_t>(y);
+  return a < b + (uintptr_t)y_bytes && b < a + (uintptr_t)x_bytes;
 }
 
 // The TreeArgs whose sizes decide the workspaces.
@@ -1559,6 +1564,9 @@ int qcau_tree_attn(const qcau_tree_args* args, void* stream) {
   int rc = check_tree(a, t.d_v, "tree_attn");
   if (rc) return rc;
   QCAU_CHECK_ARG((reinterpret_cast<uintptr_t>(t.o) & 15) == 0, "tree_attn: o must be 16-byte aligned");
+  // q is read by other blocks while rows of o are written
+  QCAU_CHECK_ARG(!overlap(t.q, t.b * t.s * t.h * t.d_qk * 2, t.o, t.b * t.s * t.h * 1024),
+                 "tree_attn: o must not overlap q");
   rc = check_tree_ws(attn_tree_workspace(a), t, "tree_attn");
   if (rc) return rc;
   if (t.b == 0) return QCAU_OK;
@@ -1624,6 +1632,9 @@ int qcau_keep_rows(const qcau_keep_args* args, void* stream) {
   if (t.b >= 65536 || t.k >= (1LL << 31) - 4096 || t.d >= (1LL << 24) || t.max_pages >= most ||
       t.dst_max_pages >= most || t.num_pages >= most || t.dst_num_pages >= most)
     return fail(QCAU_ERR_UNSUPPORTED, "keep_rows: batch too large for one call");
+  for (const int32_t* in : {t.start, t.counts})
+    QCAU_CHECK_ARG(t.b == 0 || !t.lens_out || !in || in == t.lens_out || !overlap(in, t.b * 4, t.lens_out, t.b * 4),
+                   "keep_rows: lens_out may be start or counts, but not overlap their other values");
   if (t.b == 0) return QCAU_OK;
   QCAU_CHECK_CUDA(launch_keep_rows(t, to_stream(stream)));
   return QCAU_OK;

@@ -337,6 +337,20 @@ constexpr int kKeepThreads = 256;
 constexpr int kKeepLoads = 8;  // 16-byte loads in flight per thread
 constexpr int64_t kKeepSlots = 4 * 148;  // blocks that run at once
 
+// Where the rows of sequence b go, and how many; refused: not within the block table.
+struct KeepRange {
+  int start, count;
+  bool refused;
+};
+__device__ __forceinline__ KeepRange keep_range(const qcau_keep_args& p, int b) {
+  KeepRange r;
+  r.start = p.start ? p.start[b] : 0;
+  r.count = p.counts[b];
+  const int room = (int)(p.dst_max_pages * p.page_size);
+  r.refused = r.count < 0 || r.count > p.k || r.start < 0 || r.start > room - r.count;
+  return r;
+}
+
 // A cluster of `spread` blocks moves one column slice of UNITS x 16 bytes (0:
 // whole rows) of all kept rows of sequence b, in order, spread x some rows a turn:
 // keep is strictly ascending, so row start + i comes from itself or from a later
@@ -361,12 +375,10 @@ __global__ void __launch_bounds__(kKeepThreads, 4) keep_rows_kernel(qcau_keep_ar
   const int rows = UNITS ? kMaxRows : min(kMaxRows, kKeepThreads * U / row_units);  // a turn
   const int unit0 = UNITS ? blockIdx.x / spread * UNITS : 0;
   const int share = blockIdx.x % spread;  // this block's rows of a turn
-  const int start = p.start ? p.start[b] : 0, page = (int)p.page_size;
-  const int room = (int)(p.max_pages * p.page_size), dst_room = (int)(p.dst_max_pages * p.page_size);
-  int count = p.counts[b];
-  const bool refused = count < 0 || count > p.k || start < 0 || start > dst_room - count;
-  bool bad = refused;
-  if (refused) count = 0;
+  const KeepRange range = keep_range(p, b);
+  const int start = range.start, count = range.refused ? 0 : range.count;
+  const int page = (int)p.page_size, room = (int)(p.max_pages * p.page_size);
+  bool bad = range.refused;
   const int32_t* keep = p.keep + b * p.keep_stride;
   const int32_t* stab = p.block_table + b * p.max_pages;
   const int32_t* dtab = p.dst_table + b * p.dst_max_pages;
@@ -376,11 +388,12 @@ __global__ void __launch_bounds__(kKeepThreads, 4) keep_rows_kernel(qcau_keep_ar
       const int i = (turn * spread + share) * rows + r;
       int f = -1, t = -1;
       if (i < count) {
-        const int k = keep[i], before = i > 0 ? keep[i - 1] : -1, at = start + k, row = start + i;
+        const int k = keep[i], before = i > 0 ? keep[i - 1] : -1;
         // ascending: behind its predecessor, hence never before its own place
         if (k < i || k <= before || k >= room - start) {
           bad = true;
         } else if (!(same && k == i)) {
+          const int at = start + k, row = start + i;
           const int64_t sp = stab[at / page], dp = dtab[row / page];
           if (sp < 0 || sp >= p.num_pages || dp < 0 || dp >= p.dst_num_pages) {
             bad = true;
@@ -443,7 +456,19 @@ __global__ void __launch_bounds__(kKeepThreads, 4) keep_rows_kernel(qcau_keep_ar
     }
   }
   if (bad) raise_dev_error(err, QCAU_DEVERR_INDEX);
-  if (p.lens_out && !refused && blockIdx.x == 0 && tid == 0) p.lens_out[b] = start + count;
+  if (p.lens_out && blockIdx.x == 0) {
+    __syncthreads();  // start and counts, either of which lens_out may be, are read
+    if (tid == 0 && !range.refused) p.lens_out[b] = start + count;
+  }
+}
+
+// lens_out where it is start or counts, which all the blocks of a sequence read.
+__global__ void __launch_bounds__(256) keep_lens_kernel(qcau_keep_args p) {
+  cudaGridDependencySynchronize();
+  const int b = blockIdx.x * 256 + threadIdx.x;
+  if (b >= p.b) return;
+  const KeepRange r = keep_range(p, b);
+  if (!r.refused) p.lens_out[b] = r.start + r.count;
 }
 
 }  // namespace
@@ -480,9 +505,15 @@ cudaError_t launch_evict_select(const qcau_select_args& a, cudaStream_t st) {
 cudaError_t launch_keep_rows(const qcau_keep_args& a, cudaStream_t st) {
   int* err = device_error_word();
   const int64_t units = a.d / 8;  // 16-byte units of a row
+  const bool late = a.lens_out && (a.lens_out == a.start || a.lens_out == a.counts);
   auto run = [&](auto kernel, int64_t slices, int64_t spread) {
-    return launch_early(kernel, dim3((unsigned)(slices * spread), (unsigned)a.b), (unsigned)spread,
-                        kKeepThreads, 0, st, a, (int)spread, err);
+    const bool two = late && slices * spread > 1;
+    qcau_keep_args rows = a;
+    if (two) rows.lens_out = nullptr;
+    cudaError_t e = launch_early(kernel, dim3((unsigned)(slices * spread), (unsigned)a.b), (unsigned)spread,
+                                 kKeepThreads, 0, st, rows, (int)spread, err);
+    if (e != cudaSuccess || !two) return e;
+    return launch_early(keep_lens_kernel, dim3((unsigned)((a.b + 255) / 256)), 1, 256, 0, st, a);
   };
   // few rows (a commit): a block takes whole rows, up to 28 of 576 values a turn
   if (a.k <= 64 && units <= kKeepThreads) return run(keep_rows_kernel<0>, 1, 1);

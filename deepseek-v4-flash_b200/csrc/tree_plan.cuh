@@ -62,11 +62,12 @@ struct TreeSeq {
 };
 
 // Lengths of one sequence.  What the caller's arrays may not hold (a length
-// past max_len, more nodes than tokens or than s) is cut to what they may.
+// past max_len, more nodes than tokens or than s) is cut to what they may.  A
+// sequence of no tokens, an idle slot of the cache, has no nodes where none are given.
 template <typename Cut>
 __device__ __forceinline__ TreeSeq tree_seq(const TreeShape& p, int b) {
   TreeSeq q;
-  const int len = p.seqlens[b], n = p.tree_lens ? p.tree_lens[b] : p.s;
+  const int len = p.seqlens[b], n = p.tree_lens ? p.tree_lens[b] : len == 0 ? 0 : p.s;
   q.len = min(max(len, 0), p.max_len);
   q.n = min(min(max(n, 0), p.s), q.len);
   if (q.len != len || q.n != n) raise_dev_error(p.err, QCAU_DEVERR_INDEX);

@@ -128,7 +128,7 @@ def keep_rows(cache: torch.Tensor, block_table: torch.Tensor, keep: torch.Tensor
     dst_table name where the rows go (None: cache / block_table), either other
     memory or pages that block_table does not use.  Pages that are written must
     belong to one sequence only.  seqlens [b] int32, when given, becomes start +
-    counts.  An offset out of range or out of order is not copied and raises the
+    counts (it may be start or counts itself).  An offset out of range or out of order is not copied and raises the
     device error bit DEVERR_INDEX.
     """
     _lib.bind().keep_rows(cache, block_table, keep, counts, start, dst_cache, dst_table, seqlens)
@@ -199,6 +199,8 @@ class PagedKVCache:
         step's end) and return the pages they no longer need.  positions()
         counts cached rows: after an eviction the caller's own count of tokens
         gives the positions of new ones."""
+        if len(seqs) != len(lengths) or len(set(seqs)) != len(seqs):
+            raise ValueError("one length for each sequence, and each sequence once, are needed")
         for s, n in zip(seqs, lengths):
             if not 0 <= n <= self._len[s]:
                 raise ValueError(f"sequence {s} has {self._len[s]} tokens, cannot keep {n}")

@@ -53,7 +53,8 @@ def tree_attn(q: torch.Tensor, cache: torch.Tensor, block_table: torch.Tensor,
     q [b, s, h, d] bf16 (d = 576 or 512, the cache's width; any s and h), cache
     [pages, page, d] bf16 (page a multiple of 64), block_table [b, max_pages]
     int32, seqlens [b] int32: cached tokens, of which the last tree_lens[i]
-    (None: s) are the tree's nodes in the cache.  Node t attends to all tokens
+    (None: s, or none where seqlens[i] is 0, an idle slot) are the tree's nodes
+    in the cache.  Node t attends to all tokens
     before the tree and to node j when mask[i, t, j]; mask is bool [b, s, s],
     or [s, s] for all sequences, or None for a chain (j <= t).  attn_sink [h].
 
@@ -75,7 +76,7 @@ def commit(cache: torch.Tensor, block_table: torch.Tensor, base_lens: torch.Tens
     path [b, k] int32: the accepted nodes from the root down (ascending, as a
     node comes after its parent; values past accepted[i] are ignored), accepted
     [b] int32: how many (0: none).  seqlens [b], when given, becomes base_lens
-    + accepted; PagedKVCache.truncate returns the pages of the rest.
+    + accepted (it may be base_lens itself); PagedKVCache.truncate returns the pages of the rest.
     """
     if base_lens is None:
         raise ValueError("commit: base_lens is needed")

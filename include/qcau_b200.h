@@ -594,8 +594,8 @@ int qcau_wait_flags(const uint32_t* flags, int64_t n, uint32_t epoch, void* stre
  * 512 values of a row), block_table [b, max_pages] int32.
  *
  * The drafted tokens' rows are in the cache: sequence i has seqlens[i] <=
- * max_seqlen cached tokens of which the last n = tree_lens[i] (NULL: s, and
- * n <= s, n <= seqlens[i]) are the nodes of its tree; node t is token
+ * max_seqlen cached tokens of which the last n = tree_lens[i] (n <= s, n <=
+ * seqlens[i]; NULL: s, or none in a sequence of no tokens) are the nodes of its tree; node t is token
  * base + t, base = seqlens[i] - n.  Node t attends to all tokens before
  * base, and to token base + j when tree_mask[i][t][j] != 0 (bytes [b, s, s]
  * with mask_seq_stride s * s, or one mask [s, s] for all with stride 0;
@@ -610,7 +610,7 @@ int qcau_wait_flags(const uint32_t* flags, int64_t n, uint32_t epoch, void* stre
  *   raises QCAU_DEVERR_INDEX and ends the chain.
  * tree_attn: q [b, s, h, d_qk], o [b, s, h, 512] bf16, lse [b, s, h] fp32 or
  *   NULL: the natural logarithm of the softmax denominator, the sink's term
- *   (attn_sink [h] fp32 or NULL) included.  Any h and s.  Rows that see
+ *   (attn_sink [h] fp32 or NULL) included.  Any h and s; o may not overlap q.  Rows that see
  *   nothing get o = 0 and lse = the sink's value (-inf without one); rows of
  *   nodes t >= n get o = 0 and lse = -inf.  P is rounded to bf16 before P.V
  *   as in sparse_attn.
@@ -630,8 +630,8 @@ int qcau_wait_flags(const uint32_t* flags, int64_t n, uint32_t epoch, void* stre
  *   keep[i][j] in cache, j < counts[i] <= k (start NULL: 0).  keep is strictly
  *   ascending; keep [b, keep_stride].  dst_cache / dst_table may be cache /
  *   block_table (in place, with no other buffer); pages that are written must
- *   belong to one sequence.  lens_out [b] int32 (or NULL) := start[i] +
- *   counts[i].  Entries out of range or out of order are skipped and raise
+ *   belong to one sequence.  lens_out [b] int32 (or NULL; may be start or
+ *   counts) := start[i] + counts[i].  Entries out of range or out of order are skipped and raise
  *   QCAU_DEVERR_INDEX.  page_size any, d a multiple of 16.  Evicting: keep
  *   from evict_select.  Ending a drafting step: start = base, keep = the
  *   accepted path's nodes.

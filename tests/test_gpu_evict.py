@@ -362,3 +362,47 @@ def test_empty_batch():
     assert keep.shape == (0, 5) and lens.shape == (0,)
     keep_rows(cache, table, keep, lens)
     assert tree_mask(torch.zeros(0, 4, dtype=torch.int32, device="cuda")).shape == (0, 4, 4)
+
+
+def test_a_step_with_idle_slots():
+    """A decode step of a cache whose other slots are empty: no error, sums of 0
+    there, nothing kept."""
+    pc = PagedKVCache(num_pages=16, max_seqs=4, max_pages=6)
+    g = torch.Generator().manual_seed(8)
+    slots = pc.append([1, 3], [300, 130])
+    pc.cache.view(-1, 576)[slots.long()] = torch.randn(430, 576, generator=g).to(torch.bfloat16).cuda()
+    q = torch.randn(4, 1, 16, 576, generator=g).to(torch.bfloat16).cuda()
+    o, lse = tree_attn(q, pc.cache, pc.block_table, pc.seqlens, softmax_scale=SCALE, return_lse=True)
+    sums = attn_weight_sums(q, pc.cache, pc.block_table, pc.seqlens, lse, softmax_scale=SCALE)
+    total = sums.sum(1)
+    assert total[[0, 2]].eq(0).all() and o[[0, 2]].eq(0).all()
+    # 16 rows' weights, 1 in all each: an exponent is off by 2^-19 of sum |q k| * scale
+    # (576 * 0.64 * 0.073 = 27) plus 2^-20 * (1 + lse), under 2^-13; sums lose less
+    assert (total[[1, 3]] - 16).abs().max() < 16 * 2.0 ** -12
+    before = pc.cache.clone()
+    keep, lens = evict(pc.cache, pc.block_table, pc.seqlens, sums, 128, n_first=4, n_recent=16)
+    torch.cuda.synchronize()
+    assert lens.tolist() == [0, 128, 0, 128] and keep[[0, 2]].eq(-1).all()
+    for i in (1, 3):
+        rows = R.gather(before, pc.block_table, i, 300)
+        assert torch.equal(R.gather(pc.cache, pc.block_table, i, 128), rows[keep[i].long()])
+    assert _lib.device_error() == 0
+
+
+def test_sums_of_pages_far_into_a_cache():
+    """Rows whose offsets pass 32 bits: a cache of 5 GB."""
+    pages, d = 68000, 576
+    cache = torch.empty(pages, 64, d, dtype=torch.bfloat16, device="cuda")
+    assert cache.numel() > 2 ** 31 and cache.numel() * 2 > 2 ** 32
+    at = [pages - 1, 5, pages - 2, 60000, 0, pages - 4]
+    small = torch.randn(6, 64, d, device="cuda").to(torch.bfloat16)
+    cache[at] = small
+    table = torch.tensor([at], dtype=torch.int32, device="cuda")
+    near = torch.arange(6, dtype=torch.int32, device="cuda").view(1, 6)
+    lens = torch.tensor([350], dtype=torch.int32, device="cuda")
+    for h in (16, 128, 400):
+        q = torch.randn(1, 1, h, d, device="cuda").to(torch.bfloat16)
+        lse = tree_attn(q, small, near, lens, softmax_scale=SCALE, return_lse=True)[1]
+        w = attn_weight_sums(q, cache, table, lens, lse, softmax_scale=SCALE)
+        assert torch.equal(w, attn_weight_sums(q, small, near, lens, lse, softmax_scale=SCALE))
+    assert _lib.device_error() == 0

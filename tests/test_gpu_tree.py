@@ -389,3 +389,99 @@ def test_empty_batch():
                        torch.zeros(0, 2, dtype=torch.int32, device="cuda"),
                        torch.zeros(0, dtype=torch.int32, device="cuda"), softmax_scale=SCALE, return_lse=True)
     assert o.shape == (0, 3, 16, 512) and lse.shape == (0, 3, 16)
+
+
+def test_idle_slots_have_no_nodes():
+    """Without tree_lens a sequence of no tokens, an idle slot of a cache, has no
+    nodes: zeros, -inf, and no error; the others as if it were not there."""
+    x = build(dict(lens=[200, 300], nodes=[4, 4], s=4, h=16, mask="tree"))
+    want, want_lse = tree_attn(x["q"], x["cache"], x["table"], x["seqlens"], x["mask"], softmax_scale=SCALE, return_lse=True)
+    q = torch.cat([x["q"][:1], torch.full_like(x["q"][:1], float("nan")), x["q"][1:]])
+    table = torch.stack([x["table"][0], torch.full_like(x["table"][0], -1), x["table"][1]])
+    mask = torch.stack([x["mask"][0], x["mask"][0], x["mask"][1]])
+    lens = torch.tensor([200, 0, 300], dtype=torch.int32, device="cuda")
+    o, lse = tree_attn(q, x["cache"], table, lens, mask, softmax_scale=SCALE, return_lse=True)
+    torch.cuda.synchronize()
+    assert _lib.device_error() == 0
+    assert torch.equal(o[[0, 2]], want) and torch.equal(lse[[0, 2]], want_lse)
+    assert o[1].eq(0).all() and lse[1].eq(-math.inf).all()
+
+
+def test_two_calls_at_once():
+    """Calls on two streams share nothing."""
+    xs = [build(dict(lens=[4000, 3000], nodes=[12, 10], s=12, h=16, mask="tree"), seed=3),
+          build(dict(lens=[6000], nodes=[3], s=3, h=64), seed=4)]
+
+    def call(x):
+        return tree_attn(x["q"], x["cache"], x["table"], x["seqlens"], x["mask"], softmax_scale=SCALE, tree_lens=x["tree_lens"])
+
+    want = [call(x) for x in xs]
+    streams = [torch.cuda.Stream() for _ in xs]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(20):
+        for k, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                got[k].append(call(xs[k]))
+    torch.cuda.synchronize()
+    for k in range(2):
+        assert all(torch.equal(g, want[k]) for g in got[k])
+    assert _lib.device_error() == 0
+
+
+@pytest.mark.parametrize("k", [5, 300])
+@pytest.mark.parametrize("into", ["start", "counts"])
+def test_lengths_may_be_updated_in_place(k, into):
+    b, page, d = 6, 64, 576
+    base, taken = [0, 1, 63, 192, 133, 70], [0, k, 1, 3, k // 2, k]
+    cache, table, rows = R.paged([n + k for n in base], d, page, max_pages=(192 + k) // page + 1, seed=k, stale=9.0)
+    g = torch.Generator().manual_seed(k)
+    path = torch.full((b, k), -7, dtype=torch.int32)
+    want = cache.clone()
+    for i in range(b):
+        nodes = torch.sort(torch.randperm(k, generator=g)[:taken[i]]).values
+        path[i, :taken[i]] = nodes.to(torch.int32)
+        for j, node in enumerate(nodes.tolist()):
+            p = base[i] + j
+            want[table[i, p // page], p % page] = rows[i][base[i] + node].cuda()
+    start = torch.tensor(base, dtype=torch.int32, device="cuda")
+    counts = torch.tensor(taken, dtype=torch.int32, device="cuda")
+    lens = start if into == "start" else counts
+    commit(cache, table, start, path.cuda(), counts, seqlens=lens)
+    torch.cuda.synchronize()
+    assert torch.equal(cache, want)
+    assert lens.tolist() == [x + y for x, y in zip(base, taken)]
+    assert _lib.device_error() == 0
+
+
+def test_pages_far_into_a_cache():
+    """Rows whose offsets pass 32 bits: a cache of 5 GB, the sequence in its last
+    pages and its first."""
+    pages, d, s, h = 68000, 576, 4, 16
+    cache = torch.empty(pages, 64, d, dtype=torch.bfloat16, device="cuda")
+    assert cache.numel() > 2 ** 31 and cache.numel() * 2 > 2 ** 32
+    at = [pages - 1, 5, pages - 2, 60000, 0, pages - 4]
+    small, _, _ = R.paged([6 * 64], d, 64, seed=2, stale=0.0)
+    small = small[:6].contiguous()
+    small.nan_to_num_(0.0)
+    cache[at] = small
+    table = torch.tensor([at], dtype=torch.int32, device="cuda")
+    near = torch.arange(6, dtype=torch.int32, device="cuda").view(1, 6)
+    lens = torch.tensor([350], dtype=torch.int32, device="cuda")
+    q = torch.randn(1, s, h, d, device="cuda").to(torch.bfloat16)
+    o = tree_attn(q, cache, table, lens, softmax_scale=SCALE)
+    assert torch.equal(o, tree_attn(q, small, near, lens, softmax_scale=SCALE))
+    for k in (40, 200):
+        keep = torch.sort(torch.randperm(340)[:k]).values.to(torch.int32).view(1, k).cuda()
+        n = torch.tensor([k], dtype=torch.int32, device="cuda")
+        keep_rows(cache, table, keep, n)
+        keep_rows(small, near, keep, n)
+        torch.cuda.synchronize()
+        assert torch.equal(cache[at], small)
+    assert _lib.device_error() == 0
+
+
+def test_output_over_the_queries_is_refused():
+    x = build(dict(lens=[200], nodes=[4], s=4, h=16, d=512))
+    with pytest.raises(ValueError, match="overlap"):
+        tree_attn(x["q"], x["cache"], x["table"], x["seqlens"], softmax_scale=SCALE, out=x["q"])

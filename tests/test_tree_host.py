@@ -130,3 +130,37 @@ def test_truncate_returns_pages():
         with pytest.raises(ValueError):
             pc.truncate([0, 1], [0, bad])
     assert pc.length(1) == 100
+
+
+def test_truncate_takes_each_sequence_once():
+    """A second, longer length of a sequence would name pages already returned."""
+    pc = PagedKVCache(num_pages=12, max_seqs=2, max_pages=8, width=16, device="cpu")
+    pc.append([0, 1], [300, 100])
+    for seqs, lengths in (([0, 0], [10, 200]), ([0, 1], [10]), ([0], [10, 20])):
+        with pytest.raises(ValueError):
+            pc.truncate(seqs, lengths)
+        assert pc.length(0) == 300 and pc.free_pages == 5
+
+
+@no_device
+def test_overlapping_results_are_refused():
+    L = _lib.lib()
+    step = dict(q=P[0], cache=P[1], table=P[2], seqlens=P[3], nodes=0, mask=0, sink=0, o=P[0] + 512, lse=0, sums=0, ws=P[5],
+                stride=0, b=1, s=1, h=2, d=512, dv=512, page=64, max_pages=4, num_pages=8, most=200, sums_stride=0,
+                ws_bytes=1 << 30, scale=0.07, accumulate=0)
+    for o in (P[0], P[0] + 2032, P[0] - 2032):
+        _expect(L.qcau_tree_attn(_lib.TreeArgs(*{**step, "o": o}.values()), None), ValueError, "overlap")
+    rows = dict(cache=P[0], table=P[1], dst=P[0], dst_table=P[1], keep=P[2], counts=P[3], start=P[4], lens=0, max_pages=4,
+                num_pages=8, dst_max_pages=4, dst_num_pages=8, keep_stride=5, b=3, k=5, d=576, page=64)
+    for lens in (P[3] + 4, P[3] - 8, P[4] + 8, P[4] - 4):
+        _expect(L.qcau_keep_rows(_lib.KeepArgs(*{**rows, "lens": lens}.values()), None), ValueError, "overlap")
+
+
+@no_device
+def test_sizes_past_64_bits_are_refused():
+    L = _lib.lib()
+    step = dict(q=P[0], cache=P[1], table=P[2], seqlens=P[3], nodes=0, mask=0, sink=0, o=P[4], lse=0, sums=0, ws=P[5],
+                stride=0, b=1, s=1, h=2, d=576, dv=512, page=64, max_pages=4, num_pages=8, most=200, sums_stride=0,
+                ws_bytes=1 << 30, scale=0.07, accumulate=0)
+    for change in (dict(max_pages=(1 << 58) + 4), dict(page=(1 << 62) + 64, max_pages=8)):
+        _expect(L.qcau_tree_attn(_lib.TreeArgs(*{**step, **change}.values()), None), ValueError, "bad shape")
