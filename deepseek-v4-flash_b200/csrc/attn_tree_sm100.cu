@@ -52,7 +52,8 @@ constexpr int kKSlot = 24576;         // this CTA's 64 tokens x 3 chunks of 64 d
 constexpr int kKSlots = 3;            // 9 chunks = 576 dims (8 = 512: the last box ends in zeros)
 constexpr int kVSlot = 32768;         // 64 tokens x this CTA's 256 dims (4 chunks, one box)
 constexpr int kVSlots = 2;            // the tile's two blocks
-constexpr int kQBytes = 9 * 8192;     // 64 rows x 576 bf16 (9 chunks of 64 rows)
+constexpr int kQBox = 3 * 8192;       // 64 rows x 3 chunks
+constexpr int kQBytes = 3 * kQBox;    // 64 rows x 576 bf16
 constexpr int kPBytes = 2 * 8192;     // 64 rows x 128 tokens bf16 (2 chunks of 64 tokens)
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
@@ -62,18 +63,16 @@ constexpr uint32_t kTmemS = 256;      // 2 buffers x 64 columns
 constexpr uint32_t kTmemCols = 512;
 
 struct TreeShared {
-  uint64_t kfull[kKSlots];   // leader: K slot landed in both CTAs
+  uint64_t kfull[kKSlots];   // leader: K slot (and a third of a new piece's Q) landed in both CTAs
   uint64_t kempty[kKSlots];  // both: K slot consumed by QK (the last slot: s_full)
   uint64_t vfull[kVSlots];   // leader: V slot ready in both CTAs
   uint64_t vempty[kVSlots];  // both: V slot consumed by PV (the last slot: p_free)
   uint64_t vtail;            // local: a V slot that is cleaned before use has landed
-  uint64_t q_full;           // leader: Q landed in both CTAs
   uint64_t s_full[2];        // both: S(t) ready
   uint64_t s_free[2];        // leader: the 8 softmax warps have read S(t)
   uint64_t p_full;           // leader: the 8 softmax warps wrote P(t) / corrected O
   uint64_t p_free;           // both: PV(t) done with P and O
   uint64_t o_full;           // both: last PV of the piece done
-  uint64_t q_empty;          // both: last QK of the piece done (Q may be reloaded)
   uint64_t o_free;           // leader: the 8 epilogue warps have read O
   uint64_t xbar[2];          // local: the 4 softmax warps exchanged tile maxima
   uint64_t lbar;             // local: denominator exchange
@@ -151,7 +150,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       mbar_init(&sh->vempty[i], 1);
     }
     mbar_init(&sh->vtail, 1);
-    mbar_init(&sh->q_full, 1);
     for (int i = 0; i < 2; i++) {
       mbar_init(&sh->s_full[i], 1);
       mbar_init(&sh->s_free[i], 8);
@@ -160,7 +158,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     mbar_init(&sh->p_full, 8);
     mbar_init(&sh->p_free, 1);
     mbar_init(&sh->o_full, 1);
-    mbar_init(&sh->q_empty, 1);
     mbar_init(&sh->o_free, 8);
     mbar_init(&sh->lbar, 4);
     sh->abort = 0;
@@ -187,8 +184,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     if (lane == 0) {
       int last_use[kKSlots];
       for (int i = 0; i < kKSlots; i++) last_use[i] = -1;
-      const uint32_t q_full_l = mapa_shared(smem_u32(&sh->q_full), 0);
-      int gt = 0, nq = 0;  // tiles; pieces whose Q was issued
+      int gt = 0;  // tiles
       bool ok = true;
       TreeCursor c = range.start;
       TreePiece u;
@@ -203,25 +199,22 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             } else if (!(ok = mbar_wait(&sh->kempty[i], (gt & 1) ^ 1, abort))) {
               break;
             }
-            if (leader) mbar_arrive_expect_tx(&sh->kfull[i], 2 * kKSlot);
+            // a piece's first tile brings its Q (rows past the sequence's: zeros) along,
+            // the box's three chunks at a time: the MMAs that freed the slot were the
+            // last to read the previous piece's
+            const bool with_q = t == u.t_begin;
+            const uint32_t bar = mapa_shared(smem_u32(&sh->kfull[i]), 0);
+            if (leader) mbar_arrive_expect_tx(&sh->kfull[i], 2 * (kKSlot + (with_q ? kQBox : 0)));
             last_use[i] = gt;
-            tma_load_4d_pair(sK + i * kKSlot, &tm_k, mapa_shared(smem_u32(&sh->kfull[i]), 0), 0, 0,
-                             3 * i, blk);
-            if (i == 0 && t == u.t_begin) {
-              // the piece's rows (past the sequence's: zeros), behind its first K
-              // box: free once the previous piece's last QK has completed
-              if (nq > 0 && !(ok = mbar_wait(&sh->q_empty, (nq - 1) & 1, abort))) break;
-              if (leader) mbar_arrive_expect_tx(&sh->q_full, 2 * p.chunks * 8192);
-              tma_load_4d_pair(sQ, &tm_q, q_full_l, 0, u.g * 128 + 64 * (int)rank, 0, u.b);
-              nq++;
-            }
+            if (with_q)
+              tma_load_4d_pair(sQ + i * kQBox, &tm_q, bar, 0, u.g * 128 + 64 * (int)rank, 3 * i, u.b);
+            tma_load_4d_pair(sK + i * kKSlot, &tm_k, bar, 0, 0, 3 * i, blk);
           }
         }
       }
       if (*abort && leader) {
         // the leader's full barriers count both CTAs' copies: drain them all
         volatile int never = 0;
-        if (nq > 0) mbar_wait<true>(&sh->q_full, (nq - 1) & 1, &never);
         for (int i = 0; i < kKSlots; i++)
           if (last_use[i] >= 0) mbar_wait<true>(&sh->kfull[i], last_use[i] & 1, &never);
       }
@@ -316,9 +309,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       if (warp == 1) {
         const uint32_t idesc_qk = make_idesc(128, 128, kFmtBF16, kFmtBF16, false, false);
         const uint64_t q_desc = make_sdesc(q_addr, 16, 1024), k_desc = make_sdesc(k_addr, 16, 1024);
-        int gt = 0, nu = 0;  // tiles, pieces
+        int gt = 0;  // tiles
         while (ok && tree_piece<Cut>(p.sh, cur, u)) {
-          if (!(ok = mbar_wait(&sh->q_full, nu & 1, abort))) break;
           for (int t = u.t_begin; t < u.t_end && ok; t++, gt++) {
             const int sb = gt & 1;
             if (gt >= 2 && !(ok = mbar_wait<true>(&sh->s_free[sb], ((gt >> 1) - 1) & 1, abort)))
@@ -350,9 +342,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
               last_phase = (gt >> 1) & 1;
             }
           }
-          // both CTAs' Q may be reloaded once the piece's QK MMAs have completed
-          if (ok) tc_commit_pair(&sh->q_empty, 3);
-          nu++;
         }
       } else {
         const uint32_t idesc_pv = make_idesc(128, 256, kFmtBF16, kFmtBF16, false, true);
@@ -778,11 +767,11 @@ cudaError_t launch_attn_tree_sm100(const TreeArgs& a, void* ws, cudaStream_t st)
   const int64_t pairs = tree_pairs(a, Cut::kGroupRows, kTile);
   CUtensorMap tq, tk, tv;
   {
-    // Q as [b][chunks][rows][64 values]: a CTA's 64 rows in one box
+    // Q as [b][chunks][rows][64 values]: three chunks of a CTA's 64 rows in a box
     const uint64_t row = (uint64_t)a.d_qk * 2;
     const uint64_t dims[4] = {64, (uint64_t)rows, (uint64_t)(a.d_qk / 64), (uint64_t)a.b};
     const uint64_t strides[3] = {row, 128, (uint64_t)rows * row};
-    const uint32_t box[4] = {64, 64, (uint32_t)(a.d_qk / 64), 1};
+    const uint32_t box[4] = {64, 64, 3, 1};
     if (!make_tmap(&tq, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, a.q, dims, strides, box,
                    CU_TENSOR_MAP_SWIZZLE_128B))
       return cudaErrorInvalidValue;

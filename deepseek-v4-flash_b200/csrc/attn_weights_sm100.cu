@@ -50,7 +50,9 @@ struct WeightsCfg {
   static constexpr int kTile = 128 * kBlocks;       // tokens of a pair's tile (MMA M)
   static constexpr int kStage = kBlocks * kBlockBox;
   static constexpr int kStages = 3;
+  static_assert(kStages == kBoxes, "Q's thirds are released by the stages of one tile");
   static constexpr int kQChunk = N / 2 * 128;  // N/2 rows x 64 dims bf16
+  static constexpr int kQBox = 3 * kQChunk;
   // TMEM: M = 128 puts a token's first N/2 columns in lanes 0-63 and the rest in
   // lanes 64-127; M = 256 all N in its one lane
   static constexpr int kCols = N == 256 ? 128 : N;
@@ -64,7 +66,6 @@ struct WeightsCfg {
 template <int N>
 struct WeightsShared {
   uint64_t kfull[WeightsCfg<N>::kStages], kempty[WeightsCfg<N>::kStages];
-  uint64_t q_full, q_empty;
   uint64_t s_full[2], s_free[2];
   uint64_t xbar[2][4];  // M = 128: halves of a token's sum handed over: 2 warp pairs x 4 buffers
   float xsum[4][64];
@@ -116,8 +117,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       mbar_init(&sh->kfull[i], 1);
       mbar_init(&sh->kempty[i], 1);
     }
-    mbar_init(&sh->q_full, 1);
-    mbar_init(&sh->q_empty, 1);
     for (int i = 0; i < 2; i++) {
       mbar_init(&sh->s_full[i], 1);
       mbar_init(&sh->s_free[i], 8);
@@ -145,8 +144,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     if (lane == 0) {
       int last_use[C::kStages];
       for (int i = 0; i < C::kStages; i++) last_use[i] = -1;
-      const uint32_t q_full_l = mapa_shared(smem_u32(&sh->q_full), 0);
-      int n = 0, nq = 0;  // boxes issued; pieces whose Q was issued
+      int n = 0;  // stages issued
       bool ok = true;
       TreeCursor c = range.start;
       TreePiece u;
@@ -159,29 +157,25 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           for (int i = 0; i < kBoxes; i++, n++) {
             const int slot = n % C::kStages, use = n / C::kStages;
             if (!(ok = mbar_wait(&sh->kempty[slot], (use & 1) ^ 1, abort))) break;
-            if (leader) mbar_arrive_expect_tx(&sh->kfull[slot], 2 * C::kStage);
+            // a piece's first tile brings its Q (rows past the sequence's: zeros) along,
+            // the stage's three chunks at a time: the MMAs that freed the stage were the
+            // last to read the previous piece's (a ring holds one tile)
+            const bool with_q = t == u.t_begin;
+            if (leader) mbar_arrive_expect_tx(&sh->kfull[slot], 2 * (C::kStage + (with_q ? C::kQBox : 0)));
             last_use[slot] = use;
             const uint32_t bar = mapa_shared(smem_u32(&sh->kfull[slot]), 0);
+            if (with_q)
+              tma_load_4d_pair(sQ + i * C::kQBox, &tm_q, bar, 0, u.g * N + N / 2 * (int)rank, 3 * i, u.b);
 #pragma unroll
             for (int j = 0; j < C::kBlocks; j++)
               tma_load_5d_pair(sK + (size_t)slot * C::kStage + j * kBlockBox, &tm_k, bar, 0, 0, 3 * i,
                                0, blk[j]);
-          }
-          if (ok && t == u.t_begin) {
-            // the piece's rows, behind its first tile: K streams on while the last
-            // MMAs of the previous piece, which still read Q, complete
-            if (nq > 0 && !(ok = mbar_wait(&sh->q_empty, (nq - 1) & 1, abort))) break;
-            if (leader) mbar_arrive_expect_tx(&sh->q_full, 2 * p.chunks * C::kQChunk);
-            // (rows past the sequence's are zero-filled)
-            tma_load_4d_pair(sQ, &tm_q, q_full_l, 0, u.g * N + N / 2 * (int)rank, 0, u.b);
-            nq++;
           }
         }
       }
       if (*abort && leader) {
         // the leader's full barriers count both CTAs' copies: drain them all
         volatile int never = 0;
-        if (nq > 0) mbar_wait<true>(&sh->q_full, (nq - 1) & 1, &never);
         for (int i = 0; i < C::kStages; i++)
           if (last_use[i] >= 0) mbar_wait<true>(&sh->kfull[i], last_use[i] & 1, &never);
       }
@@ -192,14 +186,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       const uint32_t idesc = make_idesc(C::kTile, N, kFmtBF16, kFmtBF16, false, false);
       const uint64_t k_desc = make_sdesc(smem_u32(sK), 16, 3072);
       const uint64_t q_desc = make_sdesc(smem_u32(sQ), 16, 1024);
-      int n = 0, gt = 0, nu = 0;  // boxes, tiles, pieces
+      int n = 0, gt = 0;  // stages, tiles
       uint64_t* last_bar = nullptr;
       int last_phase = 0;
       bool ok = true;
       TreeCursor c = range.start;
       TreePiece u;
       while (ok && tree_piece<Cut>(p.sh, c, u)) {
-        if (!(ok = mbar_wait(&sh->q_full, nu & 1, abort))) break;
         for (int t = u.t_begin; t < u.t_end && ok; t++, gt++) {
           const int sb = gt & 1;
           if (gt >= 2 && !(ok = mbar_wait<true>(&sh->s_free[sb], ((gt >> 1) - 1) & 1, abort)))
@@ -239,8 +232,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             last_phase = (gt >> 1) & 1;
           }
         }
-        if (ok) tc_commit_pair(&sh->q_empty, 3);
-        nu++;
       }
       if (*abort && last_bar != nullptr) {
         // the MMAs issued so far finish before TMEM and the slots go away
@@ -437,11 +428,11 @@ cudaError_t launch_attn_weights_sm100(const TreeArgs& a, void* ws, cudaStream_t 
   const int64_t rows = a.s * a.h, pairs = tree_pairs(a, n, tile);
   CUtensorMap tq, tk;
   {
-    // Q as [b][chunks][rows][64 values]: a CTA's rows in one box
+    // Q as [b][chunks][rows][64 values]: three chunks of a CTA's rows in a box
     const uint64_t row = (uint64_t)a.d_qk * 2;
     const uint64_t dims[4] = {64, (uint64_t)rows, (uint64_t)(a.d_qk / 64), (uint64_t)a.b};
     const uint64_t strides[3] = {row, 128, (uint64_t)rows * row};
-    const uint32_t box[4] = {64, (uint32_t)n / 2, (uint32_t)(a.d_qk / 64), 1};
+    const uint32_t box[4] = {64, (uint32_t)n / 2, 3, 1};
     if (!make_tmap(&tq, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, a.q, dims, strides, box,
                    CU_TENSOR_MAP_SWIZZLE_128B))
       return cudaErrorInvalidValue;
