@@ -129,9 +129,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     tma_prefetch_desc(&tm_q);
     tma_prefetch_desc(&tm_k);
   }
+  if (warp == 1) tmem_alloc<2>(&sh->tmem_base, C::kTmemCols);
   cudaGridDependencySynchronize();
   tree_plan_sums<Cut>(p.sh, &sh->plan);
-  if (warp == 1) tmem_alloc<2>(&sh->tmem_base, C::kTmemCols);
   tc_fence_before();
   cluster_sync();
   tc_fence_after();
