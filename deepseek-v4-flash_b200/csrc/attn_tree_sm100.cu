@@ -168,16 +168,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     tma_prefetch_desc(&tm_k);
     tma_prefetch_desc(&tm_v);
   }
-  cudaGridDependencySynchronize();
-  tree_plan_sums<Cut>(p.sh, &sh->plan);
   if (warp == 1) tmem_alloc<2>(&sh->tmem_base, kTmemCols);
   tc_fence_before();
   cluster_sync();
   tc_fence_after();
   const uint32_t tmem = sh->tmem_base;
-
-  const TreeRange range = tree_plan_range<Cut>(p.sh, &sh->plan, pair, npairs);
-  cudaTriggerProgrammaticLaunchCompletion();  // the merge may be launched; it waits for this grid
+  cudaGridDependencySynchronize();
+  const TreeRange range = tree_plan<Cut>(p.sh, &sh->plan, pair, npairs);
 
   if (warp == 0) {
     // ------------------------------------------------ Q and K producer (both CTAs)
@@ -402,6 +399,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     const uint32_t p_full_l = mapa_shared(smem_u32(&sh->p_full), 0);
     const uint32_t o_free_l = mapa_shared(smem_u32(&sh->o_free), 0);
 
+    cudaTriggerProgrammaticLaunchCompletion();  // the merge may be launched; it waits for this grid
     // the rows of nodes that a sequence does not have: zero, log-sum-exp -inf
     const int64_t seq_rows = (int64_t)p.sh.s * p.sh.h;
     // (CTA c: sequence c mod b, together with the other CTAs of that sequence)
@@ -657,6 +655,7 @@ static_assert(kMaxPieces >= kTreePairs, "a row's pieces fit the merge");
 
 __global__ void __launch_bounds__(256) tree_combine_kernel(TreeParams p) {
   cudaGridDependencySynchronize();
+  cudaTriggerProgrammaticLaunchCompletion();
   const int pair = blockIdx.x, lane = threadIdx.x & 31;
   const int4 own = p.desc[pair];
   const int local = blockIdx.y * 8 + (threadIdx.x >> 5);
@@ -725,13 +724,11 @@ __global__ void __launch_bounds__(256) tree_combine_kernel(TreeParams p) {
 
 }  // namespace
 
-// As many pairs as there can be ranges of kTreeMinTiles tiles, up to one per
-// two SMs.
+// As many pairs as there can be tiles, up to one per two SMs.
 int64_t tree_pairs(const TreeArgs& a, int group_rows, int tile) {
   const int64_t groups = (a.s * a.h + group_rows - 1) / group_rows;
   const int64_t tiles = a.b * groups * ((a.max_len + tile - 1) / tile);
-  const int64_t n = tiles / kTreeMinTiles;
-  return n < 1 ? 1 : (n < kTreePairs ? n : kTreePairs);
+  return tiles < 1 ? 1 : (tiles < kTreePairs ? tiles : kTreePairs);
 }
 
 TreeShape tree_shape(const TreeArgs& a, int group_rows, int64_t pairs) {
@@ -753,7 +750,6 @@ TreeShape tree_shape(const TreeArgs& a, int group_rows, int64_t pairs) {
   // teams of `groups` pairs when they leave at most 4 of the 74 pairs idle
   p.team = p.groups > 1 && pairs == kTreePairs &&
            kTreePairs / p.groups * p.groups >= kTreePairs - 4;
-  p.min_tiles = kTreeMinTiles;
   p.row_cost = kTreeRowCost;
   return p;
 }

@@ -130,14 +130,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     tma_prefetch_desc(&tm_k);
   }
   if (warp == 1) tmem_alloc<2>(&sh->tmem_base, C::kTmemCols);
-  cudaGridDependencySynchronize();
-  tree_plan_sums<Cut>(p.sh, &sh->plan);
   tc_fence_before();
   cluster_sync();
   tc_fence_after();
   const uint32_t tmem = sh->tmem_base;
-  const TreeRange range = tree_plan_range<Cut>(p.sh, &sh->plan, pair, npairs);
-  cudaTriggerProgrammaticLaunchCompletion();
+  cudaGridDependencySynchronize();
+  const TreeRange range = tree_plan<Cut>(p.sh, &sh->plan, pair, npairs);
 
   if (warp == 0) {
     // ------------------------------------------------ producer (both CTAs)
@@ -253,6 +251,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     const int64_t seq_rows = (int64_t)p.sh.s * p.sh.h;
     float* neg = sh->neg[warp - 2];
 
+    cudaTriggerProgrammaticLaunchCompletion();  // the next kernel may be launched; it waits for this grid
     // positions that no token of the step can see: zero, unless sums are added to
     if (!p.accumulate)
       for (int b = blockIdx.x; b < p.sh.b; b += gridDim.x) {
@@ -388,6 +387,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 __global__ void __launch_bounds__(256) weights_combine_kernel(WeightsParams p) {
   using Cut = TreeCut<256, WeightsCfg<256>::kTile>;
   cudaGridDependencySynchronize();
+  cudaTriggerProgrammaticLaunchCompletion();
   const int b = blockIdx.y, tok = blockIdx.x * 256 + threadIdx.x;
   const TreeSeq q = tree_seq<Cut>(p.sh, b);
   if (q.groups < 2 || tok >= q.len) return;

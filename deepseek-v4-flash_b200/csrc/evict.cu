@@ -369,6 +369,7 @@ __global__ void __launch_bounds__(kKeepThreads, 4) keep_rows_kernel(qcau_keep_ar
   constexpr int kMaxRows = UNITS ? kKeepThreads * U / UNITS : 128;
   __shared__ int from[2][kMaxRows], to[2][kMaxRows];  // cache rows, or -1
   cudaGridDependencySynchronize();
+  cudaTriggerProgrammaticLaunchCompletion();
   const int b = blockIdx.y, tid = threadIdx.x;
   const int row_units = (int)(p.d / 8);
   const int units = UNITS ? UNITS : row_units;             // of this block's slice

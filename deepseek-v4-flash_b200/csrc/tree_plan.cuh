@@ -18,7 +18,6 @@
 namespace qcau {
 
 constexpr int kTreePairs = 74;  // CTA pairs of a B200 (148 SMs)
-constexpr int kTreeMinTiles = 1;
 // 32 sequences x up to 8 nodes x 128 heads, ragged: 132.6 us with 0, 126.6 with 1,
 // 124.7 with 2, 124.8 with 3.
 constexpr int kTreeRowCost = 2;
@@ -42,7 +41,6 @@ struct TreeShape {
   int page_blocks;  // 64-token blocks of a page
   int groups;       // groups of a sequence at s nodes
   int team;         // 1: the team schedule may be used
-  int min_tiles;    // tiles of a range, at least
   int row_cost;     // what starting a row costs, in tiles (long ranges only)
 };
 
@@ -87,6 +85,7 @@ struct TreePiece {
 // takes the same walk.
 struct TreeCursor {
   int b, first;  // current sequence and its first place in the list
+  TreeSeq q;     // the current sequence
   int x, x_end;
   int extra;     // places in front of a row's tiles
   int group;     // team schedule: this pair's group; else -1
@@ -98,24 +97,24 @@ struct TreeRange {
   int tsize;  // pairs between a range and the next one of the same group
 };
 
-struct TreePlanShared {
-  long long sum_rows[8], sum_seqs[8];  // per warp (up to 8): tiles of all rows, of all sequences
-  int num_rows[8], num_seqs[8];        // per warp: rows, sequences that have tiles
-  int scan[8];                         // per warp: tiles of a run of sequences
-  int start_b, start_tile;             // first sequence of the range, and its first tile
+struct TreePlanShared {  // batches of more than 32 sequences
+  int4 sums[8];              // per warp (up to 8): tiles of all rows, of all sequences; rows, sequences
+  int scan[8];               // per warp: places of a run of sequences
+  int start_b, start_first;  // first sequence of the range, and its first place
+  TreeSeq start;
 };
 
 template <typename Cut>
 __device__ __forceinline__ bool tree_piece(const TreeShape& p, TreeCursor& c, TreePiece& u) {
   while (c.x < c.x_end && c.b < p.b) {
-    u.q = tree_seq<Cut>(p, c.b);
+    u.q = c.q;
     const int rows = c.group >= 0 ? 1 : u.q.groups, places = u.q.tiles + c.extra;
     if (u.q.tiles == 0 || c.x >= c.first + places * rows) {
       c.first += u.q.tiles == 0 ? 0 : places * rows;
-      c.b++;
+      if (++c.b < p.b) c.q = tree_seq<Cut>(p, c.b);
       continue;
     }
-    const int k = (c.x - c.first) / places;
+    const int k = rows == 1 ? 0 : (int)((unsigned)(c.x - c.first) / (unsigned)places);
     u.b = c.b;
     u.g = c.group >= 0 ? c.group : k;
     u.row0 = c.first + k * places + c.extra;
@@ -129,115 +128,150 @@ __device__ __forceinline__ bool tree_piece(const TreeShape& p, TreeCursor& c, Tr
   return false;
 }
 
-// First half of the plan, before a barrier of the CTA: the batch's tiles.
-template <typename Cut>
-__device__ __forceinline__ void tree_plan_sums(const TreeShape& p, TreePlanShared* sh) {
-  long long rows = 0, seqs = 0;
-  int nrows = 0, nseqs = 0;
-  for (int i = threadIdx.x; i < p.b; i += blockDim.x) {
-    const TreeSeq q = tree_seq<Cut>(p, i);
-    rows += (long long)q.tiles * q.groups;
-    seqs += q.tiles;
-    nrows += q.groups;
-    nseqs += q.tiles > 0 ? 1 : 0;
-  }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    rows += __shfl_xor_sync(0xffffffffu, rows, o);
-    seqs += __shfl_xor_sync(0xffffffffu, seqs, o);
-  }
-  nrows = __reduce_add_sync(0xffffffffu, nrows);
-  nseqs = __reduce_add_sync(0xffffffffu, nseqs);
-  if ((threadIdx.x & 31) == 0) {
-    sh->sum_rows[threadIdx.x >> 5] = rows;
-    sh->sum_seqs[threadIdx.x >> 5] = seqs;
-    sh->num_rows[threadIdx.x >> 5] = nrows;
-    sh->num_seqs[threadIdx.x >> 5] = nseqs;
-  }
-  if (threadIdx.x == 0) {
-    sh->start_b = p.b;
-    sh->start_tile = 0;
-  }
+// floor(x / n) of small numbers, n <= kTreePairs and x < 2^14: (x + 1/2) / n is at
+// least 1/148 from an integer, far more than its rounding.
+__device__ __forceinline__ int tree_div_small(int x, float inv_n) {
+  return (int)(((float)x + 0.5f) * inv_n);
 }
 
 // First place of range i: floor(i total / nranges), in 32 bits (nranges is small).
-__device__ __forceinline__ int tree_cut(const TreeRange& r, int i) {
-  const int q = r.total / r.nranges, rem = r.total - q * r.nranges;
-  return i * q + i * rem / r.nranges;
+__device__ __forceinline__ int tree_cut(int total, int nranges, int i) {
+  const int q = (unsigned)total / (unsigned)nranges, rem = total - q * nranges;
+  return i * q + tree_div_small(i * rem, __fdividef(1.f, (float)nranges));
 }
 
 // The range that place x belongs to: the largest i with tree_cut(i) <= x.
 __device__ __forceinline__ int tree_range_of(const TreeRange& r, int x) {
-  return (int)(((int64_t)(x + 1) * r.nranges - 1) / r.total);
+  // off by one at most
+  int i = min((int)((float)x * (float)r.nranges / (float)r.total), r.nranges - 1);
+  if (tree_cut(r.total, r.nranges, i) > x) return i - 1;
+  if (i + 1 < r.nranges && tree_cut(r.total, r.nranges, i + 1) <= x) i++;
+  return i;
 }
 
-// Second half, after that barrier (all threads of the CTA): this pair's range.
-// Every CTA sums the same lengths, so all take one plan.
-template <typename Cut>
-__device__ __forceinline__ TreeRange tree_plan_range(const TreeShape& p, TreePlanShared* sh,
-                                                     int pair, int npairs) {
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, nwarps = blockDim.x >> 5;
-  long long rows = 0, seqs = 0;
-  int nrows = 0, nseqs = 0;
-  for (int w = 0; w < nwarps; w++) {
-    rows += sh->sum_rows[w];
-    seqs += sh->sum_seqs[w];
-    nrows += sh->num_rows[w];
-    nseqs += sh->num_seqs[w];
-  }
+// The cut of a batch of `rows` tiles (of `seqs` sequences' tiles; nrows rows of nseqs
+// sequences that have tiles): this pair's range, but for its first sequence.
+__device__ __forceinline__ TreeRange tree_plan_cut(const TreeShape& p, int rows, int seqs, int nrows, int nseqs,
+                                                   int pair, int npairs) {
   TreeRange r;
   // a team runs every group on every sequence's tiles: not worth it where the
   // trees' own sizes leave a tenth of them empty
-  const bool team = p.team && rows * 10 >= seqs * p.groups * 9;
+  const bool team = p.team && (int64_t)rows * 10 >= (int64_t)seqs * p.groups * 9;
   r.tsize = team ? p.groups : 1;
-  r.total = (int)(team ? seqs : rows);
-  r.nranges = max(1, min(npairs / r.tsize, r.total / p.min_tiles));
+  r.total = team ? seqs : rows;
+  r.range = team ? pair / p.groups : pair;
+  r.start.group = team ? pair - r.range * p.groups : -1;
+  r.nranges = max(1, min(team ? npairs / p.groups : npairs, r.total));
   // ranges of 8 tiles or more: the rows' starts count too
   const int extra = r.total >= 8 * r.nranges ? p.row_cost : 0;
   r.total += extra * (team ? nseqs : nrows);
   r.start.extra = extra;
-  r.range = pair / r.tsize;
   const bool busy = r.range < r.nranges;
-  r.start.x = busy ? tree_cut(r, r.range) : 0;
-  r.start.x_end = busy ? tree_cut(r, r.range + 1) : 0;
-  r.start.group = team ? pair % r.tsize : -1;
-  r.start.b = 0;
-  r.start.first = 0;
-  if (p.b > 1) {
-    // the sequence that place start.x belongs to: prefix sums of a block's worth of sequences
-    int before = 0;
-    for (int b0 = 0; b0 < p.b; b0 += blockDim.x) {
-      const int i = b0 + threadIdx.x;
-      int w = 0;
-      if (i < p.b) {
-        const TreeSeq q = tree_seq<Cut>(p, i);
-        w = q.tiles > 0 ? (q.tiles + extra) * (team ? 1 : q.groups) : 0;
-      }
-      int inc = w;
+  r.start.x = busy ? tree_cut(r.total, r.nranges, r.range) : 0;
+  r.start.x_end = busy ? tree_cut(r.total, r.nranges, r.range + 1) : 0;
+  return r;
+}
+
+// Places of a sequence in the list.
+__device__ __forceinline__ int tree_places(const TreeRange& r, const TreeSeq& q) {
+  return q.tiles > 0 ? (q.tiles + r.start.extra) * (r.start.group >= 0 ? 1 : q.groups) : 0;
+}
+
+__device__ __forceinline__ int warp_scan(int x) {  // inclusive
 #pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int v = __shfl_up_sync(0xffffffffu, inc, o);
-        if (lane >= o) inc += v;
-      }
-      if (lane == 31) sh->scan[warp] = inc;
-      __syncthreads();
-      int prior = before, all = before;
-      for (int k = 0; k < nwarps; k++) {
-        if (k < warp) prior += sh->scan[k];
-        all += sh->scan[k];
-      }
-      const int lo = prior + inc - w;
-      if (w > 0 && lo <= r.start.x && r.start.x < lo + w) {
-        sh->start_b = i;
-        sh->start_tile = lo;
-      }
-      __syncthreads();
-      before = all;
-      if (before > r.start.x) break;
-    }
-    r.start.b = sh->start_b;
-    r.start.first = sh->start_tile;
+  for (int o = 1; o < 32; o <<= 1) {
+    const int v = __shfl_up_sync(0xffffffffu, x, o);
+    if ((threadIdx.x & 31) >= o) x += v;
   }
+  return x;
+}
+
+// This pair's range (all threads of the CTA).  Every CTA sums the same lengths, so
+// all take one plan.
+//
+// A short call waits for the plan alone, so it goes without what can be spared:
+// divisions (a handful of them was half a microsecond), a second read of the
+// lengths, the wait for the block table, whose start is brought near meanwhile (all
+// of it in a short call), and up to 32 sequences without barriers, each warp for itself.
+template <typename Cut>
+__device__ __forceinline__ TreeRange tree_plan(const TreeShape& p, TreePlanShared* sh, int pair, int npairs) {
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, nwarps = blockDim.x >> 5;
+  if (tid * 32 < p.b * p.max_pages) {
+    int first;
+    asm volatile("ld.global.b32 %0, [%1];" : "=r"(first) : "l"(p.table + tid * 32));
+  }
+  if (p.b <= 32) {
+    TreeSeq q{};
+    if (lane < p.b) q = tree_seq<Cut>(p, lane);
+    const int rows = __reduce_add_sync(0xffffffffu, q.tiles * q.groups);
+    const int seqs = __reduce_add_sync(0xffffffffu, q.tiles);
+    const int nrows = __reduce_add_sync(0xffffffffu, q.groups);
+    TreeRange r = tree_plan_cut(p, rows, seqs, nrows, __popc(__ballot_sync(0xffffffffu, q.tiles > 0)), pair, npairs);
+    const int w = tree_places(r, q), lo = p.b > 1 ? warp_scan(w) - w : 0;
+    const unsigned at = __ballot_sync(0xffffffffu, lo <= r.start.x && r.start.x < lo + w);
+    const int i = at ? __ffs(at) - 1 : 0;
+    r.start.b = at ? i : p.b;
+    r.start.first = __shfl_sync(0xffffffffu, lo, i);
+    r.start.q.len = __shfl_sync(0xffffffffu, q.len, i);
+    r.start.q.n = __shfl_sync(0xffffffffu, q.n, i);
+    r.start.q.tiles = __shfl_sync(0xffffffffu, q.tiles, i);
+    r.start.q.groups = __shfl_sync(0xffffffffu, q.groups, i);
+    return r;
+  }
+  int rows = 0, seqs = 0, nrows = 0, nseqs = 0;
+  for (int i = tid; i < p.b; i += blockDim.x) {
+    const TreeSeq q = tree_seq<Cut>(p, i);
+    rows += q.tiles * q.groups;
+    seqs += q.tiles;
+    nrows += q.groups;
+    nseqs += q.tiles > 0 ? 1 : 0;
+  }
+  rows = __reduce_add_sync(0xffffffffu, rows);
+  seqs = __reduce_add_sync(0xffffffffu, seqs);
+  nrows = __reduce_add_sync(0xffffffffu, nrows);
+  nseqs = __reduce_add_sync(0xffffffffu, nseqs);
+  if (lane == 0) sh->sums[warp] = make_int4(rows, seqs, nrows, nseqs);
+  if (tid == 0) {
+    sh->start_b = p.b;
+    sh->start_first = 0;
+    sh->start = TreeSeq{};
+  }
+  __syncthreads();
+  rows = seqs = nrows = nseqs = 0;
+  for (int w = 0; w < nwarps; w++) {
+    rows += sh->sums[w].x;
+    seqs += sh->sums[w].y;
+    nrows += sh->sums[w].z;
+    nseqs += sh->sums[w].w;
+  }
+  TreeRange r = tree_plan_cut(p, rows, seqs, nrows, nseqs, pair, npairs);
+  // the sequence that place start.x belongs to: prefix sums of a block's worth of sequences
+  int before = 0;
+  for (int b0 = 0; b0 < p.b; b0 += blockDim.x) {
+    const int i = b0 + tid;
+    TreeSeq q{};
+    if (i < p.b) q = tree_seq<Cut>(p, i);
+    const int w = tree_places(r, q), inc = warp_scan(w);
+    if (lane == 31) sh->scan[warp] = inc;
+    __syncthreads();
+    int prior = before, all = before;
+    for (int k = 0; k < nwarps; k++) {
+      if (k < warp) prior += sh->scan[k];
+      all += sh->scan[k];
+    }
+    const int lo = prior + inc - w;
+    if (lo <= r.start.x && r.start.x < lo + w) {
+      sh->start_b = i;
+      sh->start_first = lo;
+      sh->start = q;
+    }
+    __syncthreads();
+    before = all;
+    if (before > r.start.x) break;
+  }
+  r.start.b = sh->start_b;
+  r.start.first = sh->start_first;
+  r.start.q = sh->start;
   return r;
 }
 
