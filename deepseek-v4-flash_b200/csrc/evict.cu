@@ -87,7 +87,12 @@ __device__ __forceinline__ void select_clear(SelShared* sh) {
   for (int i = threadIdx.x; i < 3 * kBins; i += kSelThreads) (&sh->hist[0][0])[i] = 0;
 }
 
-// The budget-th largest key, or a value that exactly `budget` keys reach: three
+struct Bar {
+  uint32_t key;  // tokens above it are kept,
+  bool tied;     // and as many at it as still fit (false: none)
+};
+
+// The bar that `budget` of more keys than that pass: three
 // digits of 11, 11 and 10 bits from the top, a histogram of the keys that share
 // the digits so far, and the bin that holds the budget-th key.  A bin that ends
 // exactly there ends the search.  visit(f) calls f(key) for each of the thread's
@@ -95,7 +100,7 @@ __device__ __forceinline__ void select_clear(SelShared* sh) {
 // barriers, which is most of its time after the first.  The `blocks` blocks of a
 // cluster add up their histograms, each for itself.
 template <typename Visit>
-__device__ __forceinline__ uint32_t select_bar(SelShared* sh, int budget, int blocks, Visit visit) {
+__device__ __forceinline__ Bar select_bar(SelShared* sh, int budget, int blocks, Visit visit) {
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   uint32_t prefix = 0, known = 0;
   int want = budget;
@@ -141,10 +146,10 @@ __device__ __forceinline__ uint32_t select_bar(SelShared* sh, int budget, int bl
     __syncthreads();
     prefix |= (uint32_t)sh->pick[0] << shift;
     known |= ((1u << width) - 1u) << shift;
-    if (sh->pick[2] == want) break;
+    if (sh->pick[2] == want) return {prefix - 1, false};
     want -= sh->pick[1];
   }
-  return prefix;
+  return {prefix, true};
 }
 
 // A cluster of `blocks` blocks per sequence, its keys in registers: value j of
@@ -186,7 +191,7 @@ __global__ void __launch_bounds__(kSelThreads)
     key[j] = i >= len ? 0u : i < n_first || i >= len - n_recent ? 0xffffffffu : sum_key(x[j]);
   }
   const int count = min(len, budget);
-  uint32_t bar = 1;  // every token's key is above it
+  Bar bar = {1, false};  // every token's key is above it
   __syncthreads();
   if (len > budget)  // the same in all blocks of the cluster
     bar = select_bar(sh, budget, blocks, [&](auto f) {
@@ -196,8 +201,8 @@ __global__ void __launch_bounds__(kSelThreads)
   // tokens above the bar and at it, per (j, warp)
 #pragma unroll
   for (int j = 0; j < V; j++) {
-    const unsigned g = __ballot_sync(0xffffffffu, key[j] > bar);
-    const unsigned e = __ballot_sync(0xffffffffu, key[j] == bar);
+    const unsigned g = __ballot_sync(0xffffffffu, key[j] > bar.key);
+    const unsigned e = bar.tied ? __ballot_sync(0xffffffffu, key[j] == bar.key) : 0;
     if (lane == 0) sh->count[j * kSelWarps + warp] = __popc(g) | __popc(e) << 16;
   }
   __syncthreads();
@@ -240,11 +245,17 @@ __global__ void __launch_bounds__(kSelThreads)
 #pragma unroll
   for (int j = 0; j < V; j++) {
     const uint32_t k = key[j], before = sh->count[j * kSelWarps + warp];
-    const unsigned g = __ballot_sync(0xffffffffu, k > bar), e = __ballot_sync(0xffffffffu, k == bar);
+    const unsigned g = __ballot_sync(0xffffffffu, k > bar.key);
     const unsigned lt = (1u << lane) - 1u;
-    const int before_eq = prior_eq + (int)(before >> 16) + __popc(e & lt);
-    const int pos = prior_gt + (int)(before & 0xffffu) + __popc(g & lt) + min(before_eq, ties);
-    if (k > bar || (k == bar && before_eq < ties)) {
+    int pos = prior_gt + (int)(before & 0xffffu) + __popc(g & lt);
+    bool kept = k > bar.key;
+    if (bar.tied) {
+      const unsigned e = __ballot_sync(0xffffffffu, k == bar.key);
+      const int before_eq = prior_eq + (int)(before >> 16) + __popc(e & lt);
+      pos += min(before_eq, ties);
+      kept = kept || (k == bar.key && before_eq < ties);
+    }
+    if (kept) {
       kp[pos] = token0 + j * kSelThreads;
       if (out) out[pos] = x[j];
     }
@@ -288,7 +299,7 @@ __global__ void __launch_bounds__(kSelThreads)
     bar = select_bar(sh, budget, 1, [&](auto f) {
 #pragma unroll 8
       for (int i = tid; i < len; i += kSelThreads) f(rank_key(i, src[i]));
-    });
+    }).key;  // (not tied: as many are above it as are kept)
     int n = 0;
 #pragma unroll 8
     for (int i = tid; i < len; i += kSelThreads) n += rank_key(i, src[i]) > bar;
@@ -364,12 +375,11 @@ __device__ __forceinline__ KeepRange keep_range(const qcau_keep_args& p, int b) 
 // HBM: 4 d bytes a row moved (32 x 4096 rows: 60 us, 5.0 TB/s; 128 x 1024: 57 us, 5.3;
 // random or consecutive rows, in place or not).
 template <int UNITS>
-__global__ void __launch_bounds__(kKeepThreads, 4) keep_rows_kernel(qcau_keep_args p, int spread, int* err) {
+__global__ void __launch_bounds__(kKeepThreads, UNITS ? 4 : 1) keep_rows_kernel(qcau_keep_args p, int spread, int* err) {
   constexpr int U = kKeepLoads;
   constexpr int kMaxRows = UNITS ? kKeepThreads * U / UNITS : 128;
   __shared__ int from[2][kMaxRows], to[2][kMaxRows];  // cache rows, or -1
   cudaGridDependencySynchronize();
-  cudaTriggerProgrammaticLaunchCompletion();
   const int b = blockIdx.y, tid = threadIdx.x;
   const int row_units = (int)(p.d / 8);
   const int units = UNITS ? UNITS : row_units;             // of this block's slice
@@ -384,28 +394,46 @@ __global__ void __launch_bounds__(kKeepThreads, 4) keep_rows_kernel(qcau_keep_ar
   const int32_t* stab = p.block_table + b * p.max_pages;
   const int32_t* dtab = p.dst_table + b * p.dst_max_pages;
   const bool same = p.cache == p.dst_cache && p.block_table == p.dst_table;
+  // the addresses of a turn's rows: both lookups of all of a thread's rows at a time
+  constexpr int kPlaces = (kMaxRows + kKeepThreads - 1) / kKeepThreads;
   auto place = [&](int turn) {
-    for (int r = tid; r < rows; r += kKeepThreads) {
-      const int i = (turn * spread + share) * rows + r;
-      int f = -1, t = -1;
-      if (i < count) {
-        const int k = keep[i], before = i > 0 ? keep[i - 1] : -1;
+    const int i0 = (turn * spread + share) * rows;
+    int k[kPlaces], before[kPlaces], f[kPlaces], t[kPlaces], f_at[kPlaces], t_at[kPlaces];
+#pragma unroll
+    for (int j = 0; j < kPlaces; j++) {
+      const int r = tid + j * kKeepThreads, i = i0 + r;
+      const bool live = r < rows && i < count;
+      k[j] = live ? keep[i] : -1;
+      before[j] = live && i > 0 ? keep[i - 1] : -1;
+    }
+#pragma unroll
+    for (int j = 0; j < kPlaces; j++) {
+      const int r = tid + j * kKeepThreads, i = i0 + r;
+      f[j] = t[j] = -1;
+      f_at[j] = t_at[j] = 0;
+      if (r < rows && i < count) {
         // ascending: behind its predecessor, hence never before its own place
-        if (k < i || k <= before || k >= room - start) {
+        if (k[j] < i || k[j] <= before[j] || k[j] >= room - start) {
           bad = true;
-        } else if (!(same && k == i)) {
-          const int at = start + k, row = start + i;
-          const int64_t sp = stab[at / page], dp = dtab[row / page];
-          if (sp < 0 || sp >= p.num_pages || dp < 0 || dp >= p.dst_num_pages) {
-            bad = true;
-          } else {
-            f = (int)sp * page + at % page;
-            t = (int)dp * page + row % page;
-          }
+        } else if (!(same && k[j] == i)) {
+          const unsigned at = start + k[j], row = start + i, fp = at / (unsigned)page, tp = row / (unsigned)page;
+          f[j] = stab[fp];
+          t[j] = dtab[tp];
+          f_at[j] = at - fp * page;
+          t_at[j] = row - tp * page;
+          bad = bad || f[j] < 0 || t[j] < 0;
         }
       }
-      from[turn & 1][r] = f;
-      to[turn & 1][r] = t;
+    }
+#pragma unroll
+    for (int j = 0; j < kPlaces; j++) {
+      const int r = tid + j * kKeepThreads;
+      if (f[j] >= p.num_pages || t[j] >= p.dst_num_pages) bad = true;
+      const bool move = f[j] >= 0 && t[j] >= 0 && f[j] < p.num_pages && t[j] < p.dst_num_pages;
+      if (r < rows) {
+        from[turn & 1][r] = move ? f[j] * page + f_at[j] : -1;
+        to[turn & 1][r] = move ? t[j] * page + t_at[j] : -1;
+      }
     }
   };
   const uint4* src = reinterpret_cast<const uint4*>(p.cache);
