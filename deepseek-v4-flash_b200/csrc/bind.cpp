@@ -1,7 +1,7 @@
 // bind.cpp -- Python binding of the draft-tree and eviction calls
 // (include/qcau_b200.h) on torch tensors: checks, outputs, workspace and call.
 //
-// These are calls of single decode steps, short enough on the GPU (9 to 17 us) that
+// These are calls of single decode steps, short enough on the GPU (6 to 17 us) that
 // a binding through ctypes, whose checks read each tensor attribute from Python,
 // took as long as the kernels (a tree attention 17.5 us of host time, an eviction
 // 17.2, a commit's move 8).  The functions take their arguments by position; the

@@ -512,9 +512,9 @@ cudaError_t launch_tree_mask(const int32_t* parents, uint8_t* mask, int64_t b, i
 cudaError_t launch_evict_select(const qcau_select_args& a, cudaStream_t st) {
   int* err = device_error_word();
   // one block up to 8192 sums (7.5 us against 7.8 in two); then clusters of up to 8
-  // blocks of 4096, one block per SM in all (one sequence of 16384: 8.8 us, 11.1 in one
-  // block; of 32768: 11.7, 23.1); fuller ones for more sequences or longer ones (of
-  // 131072: 17.6 us, 174 where the sums are read again for each digit)
+  // blocks of 4096, one block per SM in all (one sequence of 16384: 8.5 us, 11.1 in one
+  // block; of 32768: 11.6, 23.1); fuller ones for more sequences or longer ones (of
+  // 131072: 17.3 us, 174 where the sums are read again for each digit)
   int64_t blocks = 1;
   if (a.max_seqlen > 8 * kSelThreads)
     while (blocks < 8 && blocks * 4 * kSelThreads < a.max_seqlen && 2 * blocks * a.b <= 148) blocks *= 2;
