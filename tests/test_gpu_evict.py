@@ -406,3 +406,20 @@ def test_sums_of_pages_far_into_a_cache():
         w = attn_weight_sums(q, cache, table, lens, lse, softmax_scale=SCALE)
         assert torch.equal(w, attn_weight_sums(q, small, near, lens, lse, softmax_scale=SCALE))
     assert _lib.device_error() == 0
+
+
+@pytest.mark.parametrize("b,s,h", [(32, 1, 16), (33, 1, 16), (100, 2, 64), (40, 5, 64), (257, 1, 8)])
+def test_sums_of_many_sequences(b, s, h):
+    g = torch.Generator().manual_seed(b)
+    lens = [0 if i % 5 == 3 else int(torch.randint(1, 900, (1,), generator=g)) for i in range(b)]
+    x = build(dict(lens=lens, nodes=[min(n, 1 + i % s) for i, n in enumerate(lens)], s=s, h=h, mask="tree"))
+    lse = tree_attn(x["q"], x["cache"], x["table"], x["seqlens"], x["mask"], softmax_scale=SCALE,
+                    tree_lens=x["tree_lens"], return_lse=True)[1]
+    got = attn_weight_sums(x["q"], x["cache"], x["table"], x["seqlens"], lse, x["mask"], softmax_scale=SCALE,
+                           tree_lens=x["tree_lens"])
+    torch.cuda.synchronize()
+    live = [i for i, n in enumerate(lens) if n]
+    some = dict(rows=[x["rows"][i] for i in live], nodes=[x["nodes"][i] for i in live], q=x["q"][live], mask=x["mask"][live])
+    check_sums(some, lse[live], got[live])
+    assert got[[i for i, n in enumerate(lens) if not n]].eq(0).all()
+    assert _lib.device_error() == 0

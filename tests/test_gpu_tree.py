@@ -485,3 +485,21 @@ def test_output_over_the_queries_is_refused():
     x = build(dict(lens=[200], nodes=[4], s=4, h=16, d=512))
     with pytest.raises(ValueError, match="overlap"):
         tree_attn(x["q"], x["cache"], x["table"], x["seqlens"], softmax_scale=SCALE, out=x["q"])
+
+
+@pytest.mark.parametrize("b", [31, 32, 33, 100, 257])
+def test_batches_around_the_plan_s_sizes(b):
+    """Up to 32 sequences each warp plans for itself, above them the block does, above
+    256 in several runs; idle slots among them."""
+    g = torch.Generator().manual_seed(b)
+    lens = [0 if i % 5 == 3 else int(torch.randint(1, 700, (1,), generator=g)) for i in range(b)]
+    x = build(dict(lens=lens, nodes=[min(n, 1 + i % 3) for i, n in enumerate(lens)], s=3, h=8, mask="tree"))
+    o, lse = tree_attn(x["q"], x["cache"], x["table"], x["seqlens"], x["mask"], softmax_scale=SCALE,
+                       tree_lens=x["tree_lens"], return_lse=True)
+    torch.cuda.synchronize()
+    live = [i for i, n in enumerate(lens) if n]
+    check_attention(o[live], lse[live], x["q"][live], [x["rows"][i] for i in live], [x["nodes"][i] for i in live],
+                    x["mask"][live], None, SCALE)
+    idle = [i for i, n in enumerate(lens) if not n]
+    assert o[idle].eq(0).all() and lse[idle].eq(-math.inf).all()
+    assert _lib.device_error() == 0

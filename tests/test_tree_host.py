@@ -164,3 +164,31 @@ def test_sizes_past_64_bits_are_refused():
                 ws_bytes=1 << 30, scale=0.07, accumulate=0)
     for change in (dict(max_pages=(1 << 58) + 4), dict(page=(1 << 62) + 64, max_pages=8)):
         _expect(L.qcau_tree_attn(_lib.TreeArgs(*{**step, **change}.values()), None), ValueError, "bad shape")
+
+
+def test_the_binding_refuses_host_tensors_and_other_types():
+    """The compiled binding loads without a device, and refuses before any device work."""
+    from qcau_b200 import evict as E
+    from qcau_b200 import tree as T
+
+    q = torch.zeros(1, 2, 4, 576, dtype=torch.bfloat16)
+    cache, table = torch.zeros(2, 64, 576, dtype=torch.bfloat16), torch.zeros(1, 2, dtype=torch.int32)
+    lens, sums = torch.ones(1, dtype=torch.int32), torch.zeros(1, 128)
+    with pytest.raises(ValueError, match="CUDA"):
+        T.tree_attn(q, cache, table, lens, softmax_scale=0.07)
+    with pytest.raises(ValueError, match="CUDA"):
+        E.attn_weight_sums(q, cache, table, lens, torch.zeros(1, 2, 4), softmax_scale=0.07)
+    with pytest.raises(ValueError, match="CUDA"):
+        E.select_rows(sums, lens, 10)
+    with pytest.raises(ValueError, match="CUDA"):
+        E.evict(cache, table, lens, sums, 10)
+    with pytest.raises(ValueError, match="CUDA"):
+        T.commit(cache, table, lens, table, lens)
+    with pytest.raises(TypeError, match="q must be a tensor"):
+        T.tree_attn(None, cache, table, lens, softmax_scale=0.07)
+    with pytest.raises(TypeError, match="mask must be a tensor or None"):
+        T.tree_attn(q, cache, table, lens, 3, softmax_scale=0.07)
+    with pytest.raises(TypeError, match="softmax_scale"):
+        T.tree_attn(q, cache, table, lens, softmax_scale="x")
+    with pytest.raises(ValueError, match="base_lens"):
+        T.commit(cache, table, None, table, lens)
