@@ -450,9 +450,9 @@ cudaError_t launch_attn_weights_sm100(const TreeArgs& a, void* ws, cudaStream_t 
   }
   WeightsParams p{};
   p.sh = tree_shape(a, n, pairs);
-  // a row's start hides behind the K stream where HBM is the bound (64 x 4000 tokens
-  // x 64 heads: 41.8 us against 43.2 with the cost)
-  if (n < 256) p.sh.row_cost = 0;
+  // a row's start hides behind the K stream (64 x 4000 tokens x 64 heads: 41.8 us against
+  // 43.2 with a cost of 2 tiles; 4 x 16 nodes x 64 heads x 8000: 38.3, 39.7 with 1)
+  p.sh.row_cost = 0;
   p.lse = a.lse;
   p.sums = a.sums;
   p.sums_stride = a.sums_stride;
