@@ -38,6 +38,8 @@
 // their descendants see, values that are not finite.
 // Every wait is bounded; a timeout raises QCAU_DEVERR_TIMEOUT, drains the
 // copies in flight, frees TMEM and returns.
+#include <algorithm>
+
 #include "common.cuh"
 #include "kernels.h"
 #include "tree_plan.cuh"
@@ -644,16 +646,18 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   if (threadIdx.x == 0 && *abort) raise_dev_error(p.sh.err, QCAU_DEVERR_TIMEOUT);
 }
 
-// Merge of the rows that several ranges share: block (pair, j) takes rows
-// [8 j, 8 j + 8) of the group whose pieces start at that pair, one warp a row:
-// M = max m_i, L = sum l_i 2^(m_i - M), O = sum O_i 2^(m_i - M), then the sink
-// and the normalisation.  Latency-bound (2 KB a row and piece): the descriptor
-// holds all that the loads need, and the states and the first four pieces' O are
-// read together.
+// Merge of the rows that several ranges share: M = max m_i, L = sum l_i 2^(m_i - M),
+// O = sum O_i 2^(m_i - M), then the sink and the normalisation.  2 KB a row and
+// piece, from L2: 44 MB for 74 groups of 128 rows of two or three pieces.
+//
+// Many groups: block (pair, j) takes rows [8 j, 8 j + 8) of the group whose pieces
+// start at that pair, one warp a row, two pieces at a time so that four blocks fit an
+// SM (23 sequences of 13 nodes x 64 heads x 1536: 83.6 us, 85.7 with four at a time
+// and two blocks).
 constexpr int kMaxPieces = 96;  // at least kTreePairs
 static_assert(kMaxPieces >= kTreePairs, "a row's pieces fit the merge");
 
-__global__ void __launch_bounds__(256) tree_combine_kernel(TreeParams p) {
+__global__ void __launch_bounds__(256, 4) tree_combine_kernel(TreeParams p) {
   cudaGridDependencySynchronize();
   cudaTriggerProgrammaticLaunchCompletion();
   const int pair = blockIdx.x, lane = threadIdx.x & 31;
@@ -664,10 +668,10 @@ __global__ void __launch_bounds__(256) tree_combine_kernel(TreeParams p) {
   auto slot = [&](int i) -> int64_t {
     return ((int64_t)(pair + i * step) * 2 + (i == 0 ? 1 : 0)) * 128 + local;
   };
-  float4 f[4][4];
+  float4 f[2][4];
   auto load = [&](int i0) {
 #pragma unroll
-    for (int j = 0; j < 4; j++) {
+    for (int j = 0; j < 2; j++) {
       const float4* src = reinterpret_cast<const float4*>(p.part_o + slot(i0 + j) * 512) + lane;
 #pragma unroll
       for (int k = 0; k < 4; k++)
@@ -695,10 +699,10 @@ __global__ void __launch_bounds__(256) tree_combine_kernel(TreeParams p) {
   float a[16];
 #pragma unroll
   for (int j = 0; j < 16; j++) a[j] = 0.f;
-  for (int i0 = 0; i0 < pieces; i0 += 4) {
+  for (int i0 = 0; i0 < pieces; i0 += 2) {
     if (i0 > 0) load(i0);
 #pragma unroll
-    for (int j = 0; j < 4; j++) {
+    for (int j = 0; j < 2; j++) {
       const int i = i0 + j;  // past the pieces: weight 0 of zeros
       const float wr = i < 32 ? w[0] : i < 64 ? w[1] : w[2];
       const float wi = __shfl_sync(0xffffffffu, wr, i & 31);
@@ -720,6 +724,141 @@ __global__ void __launch_bounds__(256) tree_combine_kernel(TreeParams p) {
     out[32 * k] = make_uint2(pack_bf16(a[4 * k] * inv, a[4 * k + 1] * inv),
                              pack_bf16(a[4 * k + 2] * inv, a[4 * k + 3] * inv));
   if (p.lse && lane == 0) p.lse[orow] = lse;
+}
+
+// Few groups (one sequence, or some short trees), whose rows are cut into many pieces:
+// every warp finds the shared rows in the descriptors, and rows go to as many of a
+// block's warps as leave the blocks busy, all 8 for one group, which share out the
+// row's pieces and read four at a time.
+constexpr int kFewBlocks = 2 * 148;  // that run at once
+
+__global__ void __launch_bounds__(256, 2) tree_combine_few_kernel(TreeParams p, int npairs) {
+  constexpr int kFlight = 4;
+  __shared__ __align__(16) float so[8][512];
+  __shared__ float2 sml[8];
+  cudaGridDependencySynchronize();
+  cudaTriggerProgrammaticLaunchCompletion();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  // the shared rows, pair by pair: this lane's three pairs and their places in the list
+  static_assert(kTreePairs <= 96, "three descriptors a lane");
+  int4 own[3];
+  int first[3], rows[3], total = 0;
+#pragma unroll
+  for (int k = 0; k < 3; k++)
+    own[k] = 32 * k + lane < npairs ? p.desc[32 * k + lane] : make_int4(-1, 0, 0, 0);
+#pragma unroll
+  for (int k = 0; k < 3; k++) {
+    rows[k] = own[k].x >= 0 ? min(own[k].z - own[k].y * 128, 128) : 0;
+    const int inc = warp_scan(rows[k]);
+    first[k] = total + inc - rows[k];
+    total += __shfl_sync(0xffffffffu, inc, 31);
+  }
+  int split = 8;  // warps of a row
+  while (split > 1 && total * split > (int)gridDim.x * 8) split >>= 1;
+  const int part = warp & (split - 1), per_block = 8 / split;
+  for (int item0 = blockIdx.x * per_block; item0 < total; item0 += gridDim.x * per_block) {
+    const int item = item0 + warp / split;
+    int pair = -1, b = 0, g = 0, pieces = 0, step = 0, local = 0;
+#pragma unroll
+    for (int k = 0; k < 3; k++) {
+      const unsigned at = __ballot_sync(0xffffffffu, first[k] <= item && item < first[k] + rows[k]);
+      if (at) {
+        const int l = __ffs(at) - 1;
+        pair = 32 * k + l;
+        b = __shfl_sync(0xffffffffu, own[k].x, l);
+        g = __shfl_sync(0xffffffffu, own[k].y, l);
+        const int w = __shfl_sync(0xffffffffu, own[k].w, l);
+        pieces = w & 0xffff;
+        step = w >> 16;
+        local = item - __shfl_sync(0xffffffffu, first[k], l);
+      }
+    }
+    const int row = g * 128 + local;
+    const float sink = pair >= 0 && p.sink ? p.sink[row % p.sh.h] : -INFINITY;
+    float M = -INFINITY, L = 0.f, a[16];
+#pragma unroll
+    for (int j = 0; j < 16; j++) a[j] = 0.f;
+    for (int i0 = part; i0 < pieces; i0 += kFlight * split) {
+      float m[kFlight], l[kFlight];
+      float4 f[kFlight][4];
+      float top = M;
+#pragma unroll
+      for (int j = 0; j < kFlight; j++) {
+        // (past the last piece: that one again, at no weight, so that no branch parts the loads)
+        const int i = min(i0 + j * split, pieces - 1);
+        const int64_t slot = ((int64_t)(pair + i * step) * 2 + (i == 0 ? 1 : 0)) * 128 + local;
+        const float4* src = reinterpret_cast<const float4*>(p.part_o + slot * 512) + lane;
+        const float2 ml = reinterpret_cast<const float2*>(p.part_ml)[slot];
+        m[j] = i0 + j * split < pieces ? ml.x : -INFINITY;
+        l[j] = ml.y;
+#pragma unroll
+        for (int k = 0; k < 4; k++) f[j][k] = src[32 * k];
+      }
+#pragma unroll
+      for (int j = 0; j < kFlight; j++) top = fmaxf(top, m[j]);
+      const float w = M == -INFINITY ? 0.f : exp2f(M - top);
+      M = top;
+      L *= w;
+#pragma unroll
+      for (int j = 0; j < 16; j++) a[j] *= w;
+#pragma unroll
+      for (int j = 0; j < kFlight; j++) {
+        if (i0 + j * split >= pieces) break;
+        const float wj = m[j] == -INFINITY ? 0.f : exp2f(m[j] - top);
+        L = fmaf(l[j], wj, L);
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+          a[4 * k] = fmaf(f[j][k].x, wj, a[4 * k]);
+          a[4 * k + 1] = fmaf(f[j][k].y, wj, a[4 * k + 1]);
+          a[4 * k + 2] = fmaf(f[j][k].z, wj, a[4 * k + 2]);
+          a[4 * k + 3] = fmaf(f[j][k].w, wj, a[4 * k + 3]);
+        }
+      }
+    }
+    const int64_t orow = (int64_t)b * p.sh.s * p.sh.h + row;
+    uint2* out = reinterpret_cast<uint2*>(p.out + orow * 512);
+    float inv, lse;
+    if (split == 1) {
+      if (pair < 0) continue;
+      tree_norm(M, L, sink, inv, lse);
+#pragma unroll
+      for (int k = 0; k < 4; k++)
+        out[lane + 32 * k] = make_uint2(pack_bf16(a[4 * k] * inv, a[4 * k + 1] * inv),
+                                        pack_bf16(a[4 * k + 2] * inv, a[4 * k + 3] * inv));
+    } else {
+      // the row's warps, of which each then adds up its share of the dims
+#pragma unroll
+      for (int k = 0; k < 4; k++)
+        reinterpret_cast<float4*>(so[warp])[lane + 32 * k] = make_float4(a[4 * k], a[4 * k + 1], a[4 * k + 2], a[4 * k + 3]);
+      if (lane == 0) sml[warp] = make_float2(M, L);
+      __syncthreads();
+      const int w0 = warp - part;
+      const float2 ml = lane < split ? sml[w0 + lane] : make_float2(-INFINITY, 0.f);
+      M = warp_max(ml.x);
+      const float w = ml.x == -INFINITY ? 0.f : exp2f(ml.x - M);
+      L = warp_sum(ml.y * w);
+      float wj[8];
+#pragma unroll
+      for (int j = 0; j < 8; j++) wj[j] = __shfl_sync(0xffffffffu, w, j);
+      tree_norm(M, L, sink, inv, lse);
+      const int units = 128 / split;
+      for (int u = part * units + lane; pair >= 0 && u < (part + 1) * units; u += 32) {
+        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+          if (j >= split) break;
+          const float4 x = reinterpret_cast<const float4*>(so[w0 + j])[u];
+          o.x = fmaf(x.x, wj[j], o.x);
+          o.y = fmaf(x.y, wj[j], o.y);
+          o.z = fmaf(x.z, wj[j], o.z);
+          o.w = fmaf(x.w, wj[j], o.w);
+        }
+        out[u] = make_uint2(pack_bf16(o.x * inv, o.y * inv), pack_bf16(o.z * inv, o.w * inv));
+      }
+      __syncthreads();
+    }
+    if (p.lse && pair >= 0 && part == 0 && lane == 0) p.lse[orow] = lse;
+  }
 }
 
 }  // namespace
@@ -799,7 +938,15 @@ cudaError_t launch_attn_tree_sm100(const TreeArgs& a, void* ws, cudaStream_t st)
   e = launch_early(attn_tree_sm100_kernel, dim3((unsigned)(2 * pairs)), 1, kThreads, kSmemBytes, st,
                    tq, tk, tv, p);
   if (e != cudaSuccess || pairs == 1) return e;  // one pair: no row is shared
-  return launch_early(tree_combine_kernel, dim3((unsigned)pairs, 16), 1, 256, 0, st, p);
+  // the merge by how many groups share the pairs (one sequence of 8 nodes x 16 heads x 8192:
+  // 18.5 us with the merge of few groups, 28.6 with the other; of 23 sequences of up to 7
+  // groups, 512 wide, 56.4 and 54.0)
+  const int64_t groups = a.b * p.sh.groups;
+  if (4 * groups > pairs)
+    return launch_early(tree_combine_kernel, dim3((unsigned)pairs, 16), 1, 256, 0, st, p);
+  const int64_t shared_rows = groups * std::min<int64_t>(rows, 128);  // at most a row a block
+  return launch_early(tree_combine_few_kernel, dim3((unsigned)std::min<int64_t>(shared_rows, kFewBlocks)), 1,
+                      256, 0, st, p, (int)pairs);
 }
 
 }  // namespace qcau

@@ -503,3 +503,18 @@ def test_batches_around_the_plan_s_sizes(b):
     idle = [i for i, n in enumerate(lens) if not n]
     assert o[idle].eq(0).all() and lse[idle].eq(-math.inf).all()
     assert _lib.device_error() == 0
+
+
+@pytest.mark.parametrize("b,s,h,most", [(1, 3, 5, 5000), (1, 8, 16, 12000), (3, 8, 16, 6000), (5, 8, 16, 3000), (9, 4, 32, 2500),
+                                        (18, 8, 16, 1500), (19, 8, 16, 1500), (2, 33, 8, 4000)])
+def test_rows_cut_into_many_pieces(b, s, h, most):
+    """Few groups of rows over all ranges: their merge gives a row eight warps, four,
+    two or one."""
+    g = torch.Generator().manual_seed(most)
+    lens = [most] + [int(torch.randint(s, most, (1,), generator=g)) for _ in range(b - 1)]
+    x = build(dict(lens=lens, nodes=[s - i % 2 for i in range(b)], s=s, h=h, mask="tree", sink=b % 2 == 1), seed=b)
+    o, lse = tree_attn(x["q"], x["cache"], x["table"], x["seqlens"], x["mask"], softmax_scale=SCALE,
+                       tree_lens=x["tree_lens"], attn_sink=x["sink"], return_lse=True)
+    torch.cuda.synchronize()
+    check_attention(o, lse, x["q"], x["rows"], x["nodes"], x["mask"], x["sink"], SCALE)
+    assert _lib.device_error() == 0
