@@ -436,22 +436,40 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         const bool full = tok0 + 64 <= base;
         uint32_t bits[2] = {0xffffffffu, 0xffffffffu};
         if (!full) {
-          auto sees = [&](int tok, int node) -> bool {
-            if (tok >= u.q.len || node < 0) return false;
-            if (tok < base) return true;
-            return mask ? mask[(int64_t)node * p.sh.s + tok - base] != 0 : tok - base <= node;
-          };
-          unsigned left = 0xffffffffu;  // one ballot pair per node among the warp's rows
+          // A ballot pair per node among the warp's rows; the masks of two nodes are read
+          // together, from a valid address wherever the token lies, so that no branch
+          // parts the loads (one tree of 64 nodes x 1 head x 2000 tokens: 16.4 us, 23.5
+          // one by one)
+          constexpr int kNodes = 2;
+          const int j0 = tok0 + lane - base, j1 = j0 + 32;  // this lane's two tokens, as nodes
+          const bool live0 = j0 < u.q.n, live1 = j1 < u.q.n;
+          unsigned left = __ballot_sync(0xffffffffu, mine);
+          bits[0] = bits[1] = 0;
           while (left) {
-            const int node = __shfl_sync(0xffffffffu, my_t, __ffs(left) - 1);
-            const unsigned b0 = __ballot_sync(0xffffffffu, sees(tok0 + lane, node));
-            const unsigned b1 = __ballot_sync(0xffffffffu, sees(tok0 + 32 + lane, node));
-            const unsigned same = __ballot_sync(0xffffffffu, my_t == node);
-            if (my_t == node) {
-              bits[0] = b0;
-              bits[1] = b1;
+            unsigned same[kNodes];
+            uint8_t m0[kNodes], m1[kNodes];
+#pragma unroll
+            for (int k = 0; k < kNodes; k++) {
+              const int node = __shfl_sync(0xffffffffu, my_t, left ? __ffs(left) - 1 : 0);
+              same[k] = left & __ballot_sync(0xffffffffu, my_t == node);
+              left &= ~same[k];
+              m0[k] = j0 <= node;  // a chain
+              m1[k] = j1 <= node;
+              if (mask) {
+                const uint8_t* row = mask + (int64_t)max(node, 0) * p.sh.s;
+                m0[k] = row[min(max(j0, 0), p.sh.s - 1)];
+                m1[k] = row[min(max(j1, 0), p.sh.s - 1)];
+              }
             }
-            left &= ~same;
+#pragma unroll
+            for (int k = 0; k < kNodes; k++) {
+              const unsigned b0 = __ballot_sync(0xffffffffu, live0 && (j0 < 0 || m0[k] != 0));
+              const unsigned b1 = __ballot_sync(0xffffffffu, live1 && (j1 < 0 || m1[k] != 0));
+              if (same[k] >> lane & 1u) {
+                bits[0] = b0;
+                bits[1] = b1;
+              }
+            }
           }
         }
         if (!(ok = tree_warp_wait(&sh->s_full[sb], (gt >> 1) & 1, abort))) break;
