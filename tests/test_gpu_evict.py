@@ -423,3 +423,15 @@ def test_sums_of_many_sequences(b, s, h):
     check_sums(some, lse[live], got[live])
     assert got[[i for i, n in enumerate(lens) if not n]].eq(0).all()
     assert _lib.device_error() == 0
+
+
+@pytest.mark.parametrize("s,h,n", [(60, 1, 500), (64, 4, 200), (37, 1, 40), (90, 2, 300), (70, 3, 129)])
+def test_sums_of_trees_of_few_heads(s, h, n):
+    """Many nodes in a group of rows, their masks read several at a time."""
+    x = build(dict(lens=[n, max(s, n // 2)], nodes=[min(s, n), min(s, max(s, n // 2)) - 3], s=s, h=h, mask="any"))
+    lse = lse_of(x)
+    got = attn_weight_sums(x["q"], x["cache"], x["table"], x["seqlens"], lse, x["mask"], softmax_scale=SCALE,
+                           tree_lens=x["tree_lens"])
+    torch.cuda.synchronize()
+    check_sums(x, lse, got)
+    assert _lib.device_error() == 0
