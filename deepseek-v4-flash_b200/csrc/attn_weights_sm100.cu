@@ -23,7 +23,7 @@
 // its time, and the MMAs took longer than the loads (B200, 32 x 16384 tokens x
 // 128 heads: 117 us, 98.6 us with a third of them).  The M operand of 128 tokens
 // is two boxes of 64 tokens x 3 chunks laid out [8 rows][chunk][8 groups], which
-// makes its 8-row groups 3072 bytes apart across both.  With more rows, N is 256
+// makes its 8-row groups 3 KB apart across both.  With more rows, N is 256
 // (K is read half as often, from L2, and N = 256 needs fewer operand bytes) and
 // M 128: Q takes 147 KB, and 72 KB of ring hold one 128-token tile.
 //
@@ -182,7 +182,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     // ------------------------------------------------ MMA issuer (pair leader)
     if (leader && lane == 0) {
       const uint32_t idesc = make_idesc(C::kTile, N, kFmtBF16, kFmtBF16, false, false);
-      const uint64_t k_desc = make_sdesc(smem_u32(sK), 16, 3072);
+      const uint64_t k_desc = make_sdesc(smem_u32(sK), 16, 3 * 1024);
       const uint64_t q_desc = make_sdesc(smem_u32(sQ), 16, 1024);
       int n = 0, gt = 0;  // stages, tiles
       uint64_t* last_bar = nullptr;
