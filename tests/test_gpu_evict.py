@@ -435,3 +435,41 @@ def test_sums_of_trees_of_few_heads(s, h, n):
     torch.cuda.synchronize()
     check_sums(x, lse, got)
     assert _lib.device_error() == 0
+
+
+def test_calls_in_a_row_see_what_ran_before_them():
+    """Launches overlap the kernels before them; inputs that change between calls, by
+    kernels of torch and of this package, are read as they then are."""
+    g = torch.Generator().manual_seed(12)
+    b, s, h, most = 3, 4, 16, 2000
+    x = build(dict(lens=[most] * b, nodes=[s] * b, s=s, h=h, mask="tree"), stale=0.0)
+    q, lens, nodes = x["q"].clone(), x["seqlens"].clone(), x["tree_lens"].clone()
+    steps = [(torch.randint(s, most + 1, (b,), generator=g).to(torch.int32).cuda(),
+              torch.randn(q.shape, generator=g).to(torch.bfloat16).cuda()) for _ in range(12)]
+
+    def step(n, qs, cache):
+        lens.copy_(n)
+        q.copy_(qs)
+        o, lse = tree_attn(q, cache, x["table"], lens, x["mask"], softmax_scale=SCALE, tree_lens=nodes, return_lse=True)
+        w = attn_weight_sums(q, cache, x["table"], lens, lse, x["mask"], softmax_scale=SCALE, tree_lens=nodes)
+        keep, counts = evict(cache, x["table"], lens, w, 500, n_first=2, n_recent=8)
+        o2 = tree_attn(q, cache, x["table"], counts, x["mask"], softmax_scale=SCALE, tree_lens=nodes)
+        return o, lse, w, keep, counts, o2
+
+    caches = [x["cache"].clone(), x["cache"].clone()]
+    slow = []
+    for n, qs in steps:
+        caches[0].copy_(x["cache"])
+        out = step(n, qs, caches[0])
+        torch.cuda.synchronize()
+        slow.append([t.clone() for t in out] + [caches[0].clone()])
+    fast = []
+    for _ in range(3):
+        for k, (n, qs) in enumerate(steps):
+            caches[1].copy_(x["cache"])
+            fast.append((k, [*step(n, qs, caches[1]), caches[1].clone()]))
+    torch.cuda.synchronize()
+    for k, got in fast:
+        for a, c in zip(got, slow[k]):
+            assert torch.equal(a, c), k
+    assert _lib.device_error() == 0
