@@ -374,10 +374,11 @@ PyObject* evict(PyObject*, PyObject* const* a, Py_ssize_t n) {
 
 PyObject* keep_rows(PyObject*, PyObject* const* a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
-  TORCH_CHECK_TYPE(n == 8, "keep_rows takes 8 arguments");
+  TORCH_CHECK_TYPE(n == 9, "keep_rows takes 9 arguments");
   const Tensor *cache = tensor_arg(a[0], "cache"), *table = tensor_arg(a[1], "block_table");
   const Tensor *keep = tensor_arg(a[2], "keep"), *counts = tensor_arg(a[3], "counts");
   const Tensor *start = tensor_arg(a[4], "start", true), *lens = tensor_arg(a[7], "seqlens", true);
+  const Tensor* sums = tensor_arg(a[8], "sums", true);
   const int index = cuda_index(*cache);
   qcau_keep_args k = check_move("keep_rows", index, *cache, *table, tensor_arg(a[5], "dst_cache", true),
                                 tensor_arg(a[6], "dst_table", true));
@@ -391,7 +392,14 @@ PyObject* keep_rows(PyObject*, PyObject* const* a, Py_ssize_t n) {
   k.counts = data<int32_t>(counts);
   k.start = data<int32_t>(start);
   k.lens_out = data<int32_t>(lens);
-  run(index, "keep_rows", [&](cudaStream_t st) { return qcau_keep_rows(&k, st); });
+  if (sums) {
+    const Sums s = check_sums("keep_rows", *sums, index, k.b);
+    run(index, "keep_rows", [&](cudaStream_t st) {
+      return qcau_keep_rows_sums(&k, data<float>(sums), s.stride, s.n, st);
+    });
+  } else {
+    run(index, "keep_rows", [&](cudaStream_t st) { return qcau_keep_rows(&k, st); });
+  }
   Py_RETURN_NONE;
   END_HANDLE_TH_ERRORS
 }

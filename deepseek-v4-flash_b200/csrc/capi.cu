@@ -1525,6 +1525,26 @@ TreeArgs tree_args(const qcau_tree_args& t) {
   return a;
 }
 
+int check_keep(const qcau_keep_args& t) {
+  QCAU_CHECK_ARG(t.b == 0 || (t.cache && t.block_table && t.dst_cache && t.dst_table && t.keep && t.counts),
+                 "keep_rows: NULL pointer");
+  QCAU_CHECK_ARG(t.b >= 0 && t.k >= 1 && t.keep_stride >= t.k && t.page_size > 0 && t.max_pages > 0 &&
+                     t.num_pages > 0 && t.dst_max_pages > 0 && t.dst_num_pages > 0,
+                 "keep_rows: bad shape");
+  QCAU_CHECK_ARG(t.d > 0 && t.d % 16 == 0, "keep_rows: the row width must be a multiple of 16");
+  QCAU_CHECK_ARG(((reinterpret_cast<uintptr_t>(t.cache) | reinterpret_cast<uintptr_t>(t.dst_cache)) & 15) == 0,
+                 "keep_rows: the caches must be 16-byte aligned");
+  // the kernel counts rows in 32 bits
+  const int64_t most = (1LL << 31) / t.page_size;
+  if (t.b >= 65536 || t.k >= (1LL << 31) - 4096 || t.d >= (1LL << 24) || t.max_pages >= most ||
+      t.dst_max_pages >= most || t.num_pages >= most || t.dst_num_pages >= most)
+    return fail(QCAU_ERR_UNSUPPORTED, "keep_rows: batch too large for one call");
+  for (const int32_t* in : {t.start, t.counts})
+    QCAU_CHECK_ARG(t.b == 0 || !t.lens_out || !in || in == t.lens_out || !overlap(in, t.b * 4, t.lens_out, t.b * 4),
+                   "keep_rows: lens_out may be start or counts, but not overlap their other values");
+  return QCAU_OK;
+}
+
 int check_tree_ws(size_t need, const qcau_tree_args& t, const char* who) {
   if (t.workspace_bytes < need || (need && !t.workspace))
     return fail(QCAU_ERR_WORKSPACE,
@@ -1619,23 +1639,24 @@ int qcau_evict_select(const qcau_select_args* args, void* stream) {
 int qcau_keep_rows(const qcau_keep_args* args, void* stream) {
   QCAU_CHECK_ARG(args != nullptr, "keep_rows: NULL arguments");
   const qcau_keep_args& t = *args;
-  QCAU_CHECK_ARG(t.b == 0 || (t.cache && t.block_table && t.dst_cache && t.dst_table && t.keep && t.counts),
-                 "keep_rows: NULL pointer");
-  QCAU_CHECK_ARG(t.b >= 0 && t.k >= 1 && t.keep_stride >= t.k && t.page_size > 0 && t.max_pages > 0 &&
-                     t.num_pages > 0 && t.dst_max_pages > 0 && t.dst_num_pages > 0,
-                 "keep_rows: bad shape");
-  QCAU_CHECK_ARG(t.d > 0 && t.d % 16 == 0, "keep_rows: the row width must be a multiple of 16");
-  QCAU_CHECK_ARG(((reinterpret_cast<uintptr_t>(t.cache) | reinterpret_cast<uintptr_t>(t.dst_cache)) & 15) == 0,
-                 "keep_rows: the caches must be 16-byte aligned");
-  // the kernel counts rows in 32 bits
-  const int64_t most = (1LL << 31) / t.page_size;
-  if (t.b >= 65536 || t.k >= (1LL << 31) - 4096 || t.d >= (1LL << 24) || t.max_pages >= most ||
-      t.dst_max_pages >= most || t.num_pages >= most || t.dst_num_pages >= most)
-    return fail(QCAU_ERR_UNSUPPORTED, "keep_rows: batch too large for one call");
-  for (const int32_t* in : {t.start, t.counts})
-    QCAU_CHECK_ARG(t.b == 0 || !t.lens_out || !in || in == t.lens_out || !overlap(in, t.b * 4, t.lens_out, t.b * 4),
-                   "keep_rows: lens_out may be start or counts, but not overlap their other values");
+  const int rc = check_keep(t);
+  if (rc) return rc;
   if (t.b == 0) return QCAU_OK;
+  QCAU_CHECK_CUDA(launch_keep_rows(t, to_stream(stream)));
+  return QCAU_OK;
+}
+
+int qcau_keep_rows_sums(const qcau_keep_args* args, float* sums, int64_t sums_stride, int64_t positions,
+                        void* stream) {
+  QCAU_CHECK_ARG(args != nullptr, "keep_rows: NULL arguments");
+  const qcau_keep_args& t = *args;
+  const int rc = check_keep(t);
+  if (rc) return rc;
+  QCAU_CHECK_ARG(t.b == 0 || sums, "keep_rows: NULL pointer");
+  QCAU_CHECK_ARG(positions >= 1 && sums_stride >= positions, "keep_rows: a row of sums must hold its positions");
+  if (positions >= (1LL << 31) - 2048) return fail(QCAU_ERR_UNSUPPORTED, "keep_rows: batch too large for one call");
+  if (t.b == 0) return QCAU_OK;
+  QCAU_CHECK_CUDA(launch_keep_sums(t, sums, sums_stride, positions, to_stream(stream)));
   QCAU_CHECK_CUDA(launch_keep_rows(t, to_stream(stream)));
   return QCAU_OK;
 }

@@ -8,6 +8,7 @@
 //    order; among equal sums the lowest positions.
 //  * keep_rows: row start + keep[i] of a sequence to row start + i, for i in
 //    order, through the block table (in place, or into another cache).
+//  * keep_sums: the same move of the sequence's weight sums, 0 behind them.
 #include <algorithm>
 #include <cmath>
 
@@ -491,6 +492,44 @@ __global__ void __launch_bounds__(kKeepThreads, UNITS ? 4 : 1) keep_rows_kernel(
   }
 }
 
+constexpr int kSumThreads = 1024;
+
+// The weight sums of the rows that keep_rows moves, one block a sequence: sum start +
+// keep[i] to place start + i, then 0 from the last kept one to the row's end.  In place:
+// keep is strictly ascending, so a chunk of i reads at or behind the places that it
+// writes, and the barrier between its loads and its stores is all that is needed.
+// Bound by latency at a drafting step's few nodes, then by one SM's stores of zeros
+// (4 bytes a position).
+__global__ void __launch_bounds__(kSumThreads)
+    keep_sums_kernel(qcau_keep_args p, float* sums, int64_t stride, int64_t positions, int* err) {
+  cudaGridDependencySynchronize();
+  cudaTriggerProgrammaticLaunchCompletion();  // the move of the rows may be launched; it waits
+  const int b = blockIdx.x, tid = threadIdx.x, n = (int)positions;
+  const KeepRange range = keep_range(p, b);
+  if (range.refused) return;  // keep_rows raises the error
+  const int start = range.start, count = range.count;
+  const int32_t* keep = p.keep + b * p.keep_stride;
+  float* row = sums + b * stride;
+  bool bad = false;
+  for (int i0 = 0; i0 < count; i0 += kSumThreads) {
+    const int i = i0 + tid;
+    bool move = false;
+    float x = 0.f;
+    if (i < count) {
+      const int k = keep[i], before = i > 0 ? keep[i - 1] : -1;
+      // what keep_rows moves, and within the row of sums
+      move = k >= i && k > before && k < n - start;
+      bad = bad || !move;
+      if (move) x = row[start + k];
+    }
+    __syncthreads();
+    if (move) row[start + i] = x;
+  }
+  __syncthreads();  // the sums are read: the rest may be cleared
+  for (int i = start + count + tid; i < n; i += kSumThreads) row[i] = 0.f;
+  if (bad) raise_dev_error(err, QCAU_DEVERR_INDEX);
+}
+
 // lens_out where it is start or counts, which all the blocks of a sequence read.
 __global__ void __launch_bounds__(256) keep_lens_kernel(qcau_keep_args p) {
   cudaGridDependencySynchronize();
@@ -529,6 +568,12 @@ cudaError_t launch_evict_select(const qcau_select_args& a, cudaStream_t st) {
   if (values <= 16) return run(evict_select_kernel<16, false>, evict_select_kernel<16, true>);
   if (values <= 32) return run(evict_select_kernel<32, false>, evict_select_kernel<32, true>);
   return launch_early(evict_select_long_kernel, dim3((unsigned)a.b), 1, kSelThreads, 0, st, a, err);
+}
+
+cudaError_t launch_keep_sums(const qcau_keep_args& a, float* sums, int64_t stride, int64_t positions,
+                             cudaStream_t st) {
+  return launch_early(keep_sums_kernel, dim3((unsigned)a.b), 1, kSumThreads, 0, st, a, sums, stride, positions,
+                      device_error_word());
 }
 
 cudaError_t launch_keep_rows(const qcau_keep_args& a, cudaStream_t st) {

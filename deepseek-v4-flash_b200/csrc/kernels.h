@@ -284,5 +284,8 @@ cudaError_t launch_tree_mask(const int32_t* parents, uint8_t* mask, int64_t b, i
 // (evict.cu).
 cudaError_t launch_evict_select(const qcau_select_args& a, cudaStream_t st);
 cudaError_t launch_keep_rows(const qcau_keep_args& a, cudaStream_t st);
+// The weight sums of the same rows: runs before launch_keep_rows, which may write start or counts.
+cudaError_t launch_keep_sums(const qcau_keep_args& a, float* sums, int64_t stride, int64_t positions,
+                             cudaStream_t st);
 
 }  // namespace qcau

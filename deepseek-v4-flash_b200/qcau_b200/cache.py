@@ -116,7 +116,7 @@ def window_slots(bsz: int, seqlen: int, start_pos: int, window: int, ring_rows: 
 def keep_rows(cache: torch.Tensor, block_table: torch.Tensor, keep: torch.Tensor,
               counts: torch.Tensor, *, start: Optional[torch.Tensor] = None,
               dst_cache: Optional[torch.Tensor] = None, dst_table: Optional[torch.Tensor] = None,
-              seqlens: Optional[torch.Tensor] = None) -> None:
+              seqlens: Optional[torch.Tensor] = None, sums: Optional[torch.Tensor] = None) -> None:
     """Bring each sequence of a paged cache down to a choice of its rows.
 
     Row start[i] + j of sequence i becomes its row start[i] + keep[i, j], for
@@ -128,10 +128,13 @@ def keep_rows(cache: torch.Tensor, block_table: torch.Tensor, keep: torch.Tensor
     dst_table name where the rows go (None: cache / block_table), either other
     memory or pages that block_table does not use.  Pages that are written must
     belong to one sequence only.  seqlens [b] int32, when given, becomes start +
-    counts (it may be start or counts itself).  An offset out of range or out of order is not copied and raises the
+    counts (it may be start or counts itself).  sums [b, positions] fp32, when
+    given, are the weight sums of the sequences' rows (evict.attn_weight_sums):
+    those of the kept rows move with them, in place, and 0 follows to the row's
+    end.  An offset out of range or out of order is not copied and raises the
     device error bit DEVERR_INDEX.
     """
-    _lib.bind().keep_rows(cache, block_table, keep, counts, start, dst_cache, dst_table, seqlens)
+    _lib.bind().keep_rows(cache, block_table, keep, counts, start, dst_cache, dst_table, seqlens, sums)
 
 
 class PagedKVCache:

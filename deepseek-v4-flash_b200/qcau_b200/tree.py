@@ -69,7 +69,7 @@ def tree_attn(q: torch.Tensor, cache: torch.Tensor, block_table: torch.Tensor,
 
 def commit(cache: torch.Tensor, block_table: torch.Tensor, base_lens: torch.Tensor,
            path: torch.Tensor, accepted: torch.Tensor, *,
-           seqlens: Optional[torch.Tensor] = None) -> None:
+           seqlens: Optional[torch.Tensor] = None, sums: Optional[torch.Tensor] = None) -> None:
     """End a drafting step: the rows of each sequence's accepted path move up
     behind its base_lens[i] tokens, in place.
 
@@ -77,7 +77,12 @@ def commit(cache: torch.Tensor, block_table: torch.Tensor, base_lens: torch.Tens
     node comes after its parent; values past accepted[i] are ignored), accepted
     [b] int32: how many (0: none).  seqlens [b], when given, becomes base_lens
     + accepted (it may be base_lens itself); PagedKVCache.truncate returns the pages of the rest.
+    sums [b, positions] fp32: the running weight sums of a cache that is also
+    bounded by eviction (evict.attn_weight_sums, which has the step's weights
+    added before this call).  The accepted nodes' sums move with their rows, and
+    0 follows to the row's end, so that the tokens that come next inherit
+    nothing from rejected nodes.
     """
     if base_lens is None:
         raise ValueError("commit: base_lens is needed")
-    bind().keep_rows(cache, block_table, path, accepted, base_lens, None, None, seqlens)
+    bind().keep_rows(cache, block_table, path, accepted, base_lens, None, None, seqlens, sums)

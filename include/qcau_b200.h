@@ -635,6 +635,10 @@ int qcau_wait_flags(const uint32_t* flags, int64_t n, uint32_t epoch, void* stre
  *   QCAU_DEVERR_INDEX.  page_size any, d a multiple of 16.  Evicting: keep
  *   from evict_select.  Ending a drafting step: start = base, keep = the
  *   accepted path's nodes.
+ * keep_rows_sums: keep_rows, and the weight sums of the same rows, in place:
+ *   sums[i][start[i] + j] := sums[i][start[i] + keep[i][j]], then 0 from
+ *   start[i] + counts[i] to positions.  sums [b, sums_stride] fp32; without it
+ *   the tokens that come next would add to what rejected nodes received.
  * ---------------------------------------------------------------------- */
 typedef struct {
     const void* q;
@@ -688,6 +692,8 @@ size_t qcau_attn_weight_sums_workspace_size(int64_t b, int64_t s, int64_t h,
 int qcau_attn_weight_sums(const qcau_tree_args* args, void* stream);
 int qcau_evict_select(const qcau_select_args* args, void* stream);
 int qcau_keep_rows(const qcau_keep_args* args, void* stream);
+int qcau_keep_rows_sums(const qcau_keep_args* args, float* sums, int64_t sums_stride,
+                        int64_t positions, void* stream);
 
 #ifdef __cplusplus
 }

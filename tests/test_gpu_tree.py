@@ -518,3 +518,64 @@ def test_rows_cut_into_many_pieces(b, s, h, most):
     torch.cuda.synchronize()
     check_attention(o, lse, x["q"], x["rows"], x["nodes"], x["mask"], x["sink"], SCALE)
     assert _lib.device_error() == 0
+
+
+@pytest.mark.parametrize("k,width,into", [(5, 300, None), (70, 271, None), (300, 600, "start"), (2500, 3000, None)])
+def test_commit_moves_the_sums_with_the_rows(k, width, into):
+    """The accepted nodes' sums follow their rows and nothing stays of the others,
+    in rows of a wider buffer; the cache is moved as without sums."""
+    b, page, d = 5, 64, 64
+    base = [0, 1, 63, 192, 133]
+    taken = [0, k, 1, min(k, 3), k // 2]
+    cache, table, _ = R.paged([n + k for n in base], d, page, max_pages=(192 + k) // page + 1, seed=k, stale=9.0)
+    g = torch.Generator().manual_seed(k)
+    path = torch.full((b, k), -7, dtype=torch.int32)
+    wide = torch.rand(b, width + 9, generator=g)
+    want = wide.clone()
+    want[:, :width] = 0
+    for i in range(b):
+        nodes = torch.sort(torch.randperm(min(k, width - base[i]), generator=g)[:taken[i]]).values
+        taken[i] = len(nodes)
+        path[i, :taken[i]] = nodes.to(torch.int32)
+        want[i, :base[i]] = wide[i, :base[i]]
+        want[i, base[i]:base[i] + taken[i]] = wide[i, base[i] + nodes]
+    other, sums = cache.clone(), wide.cuda()
+    start = torch.tensor(base, dtype=torch.int32, device="cuda")
+    counts = torch.tensor(taken, dtype=torch.int32, device="cuda")
+    commit(other, table, start, path.cuda(), counts)
+    lens = start if into else torch.zeros_like(start)
+    commit(cache, table, start, path.cuda(), counts, seqlens=lens, sums=sums[:, :width])
+    torch.cuda.synchronize()
+    assert torch.equal(sums.cpu(), want) and torch.equal(cache, other)
+    assert lens.tolist() == [x + y for x, y in zip(base, taken)]
+    assert _lib.device_error() == 0
+
+
+def test_sums_of_a_path_out_of_order_or_range_are_flagged():
+    """What is not moved raises the error bit; a refused sequence's sums stay, and the
+    next one's move."""
+    cache, table, _ = R.paged([200, 200], 64, 64, seed=1, stale=0.0)
+    for path, count, start in (([3, 2], 2, 10), ([-1, 2], 2, 10), ([0, 90], 2, 10), ([0, 1], 3, 10), ([0, 1], -1, 10),
+                               ([0, 1], 2, 255), ([0, 1], 2, 120)):
+        sums = torch.rand(2, 100, device="cuda")
+        before = sums.clone()
+        keep = torch.tensor([path, [0, 4]], dtype=torch.int32, device="cuda")
+        keep_rows(cache, table, keep, torch.tensor([count, 2], dtype=torch.int32, device="cuda"),
+                  start=torch.tensor([start, 7], dtype=torch.int32, device="cuda"), sums=sums)
+        torch.cuda.synchronize()
+        assert _lib.device_error() == _lib.DEVERR_INDEX, (path, count, start)
+        if not 0 <= count <= 2 or start > 100:
+            assert torch.equal(sums[0], before[0])
+        assert torch.equal(sums[1, :8], before[1, :8]) and sums[1, 8] == before[1, 11] and sums[1, 9:].eq(0).all()
+
+
+def test_commit_refuses_other_sums():
+    cache, table, _ = R.paged([200], 64, 64, seed=1, stale=0.0)
+    one = torch.ones(1, dtype=torch.int32, device="cuda")
+    path = torch.zeros(1, 2, dtype=torch.int32, device="cuda")
+    for sums in (torch.zeros(1, 100), torch.zeros(2, 100, device="cuda"), torch.zeros(100, device="cuda"),
+                 torch.zeros(1, 100, device="cuda", dtype=torch.float64), torch.zeros(1, 0, device="cuda")):
+        with pytest.raises(ValueError):
+            commit(cache, table, one, path, one, sums=sums)
+    with pytest.raises(TypeError):
+        commit(cache, table, one, path, one, sums=3)

@@ -192,3 +192,22 @@ def test_the_binding_refuses_host_tensors_and_other_types():
         T.tree_attn(q, cache, table, lens, softmax_scale="x")
     with pytest.raises(ValueError, match="base_lens"):
         T.commit(cache, table, None, table, lens)
+
+
+@no_device
+def test_keep_rows_sums_refusals():
+    L = _lib.lib()
+    good = dict(cache=P[0], table=P[1], dst=P[0], dst_table=P[1], keep=P[2], counts=P[3], start=0, lens=0, max_pages=4,
+                num_pages=8, dst_max_pages=4, dst_num_pages=8, keep_stride=5, b=1, k=5, d=576, page=64)
+
+    def call(sums=P[4], stride=100, n=100, **change):
+        return L.qcau_keep_rows_sums(_lib.KeepArgs(*{**good, **change}.values()), sums, stride, n, None)
+
+    _expect(L.qcau_keep_rows_sums(None, P[4], 100, 100, None), ValueError, "NULL")
+    for change, exc, text in ((dict(sums=0), ValueError, "NULL"), (dict(stride=99), ValueError, "row of sums"),
+                              (dict(n=0), ValueError, "row of sums"), (dict(n=1 << 31, stride=1 << 31), NotImplementedError, "too large"),
+                              (dict(keep=0), ValueError, "NULL"), (dict(k=6), ValueError, "bad shape"),
+                              (dict(d=24), ValueError, "multiple of 16"), (dict(cache=P[0] + 2), ValueError, "aligned"),
+                              (dict(b=70000), NotImplementedError, "too large")):
+        _expect(call(**change), exc, text)
+    assert call(b=0) == 0
