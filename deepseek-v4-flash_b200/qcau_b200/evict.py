@@ -2,12 +2,25 @@
 
 Every decode (or verification) step adds to each cached token the attention
 weight it received; when a sequence is over its budget, its first tokens, its
-most recent ones and those of the largest sums stay:
+most recent ones and those of the largest sums stay.  A step with draft trees
+(without mask and commit: a decode step, s = 1) of a PagedKVCache pc, sums
+[sequences, positions] starting at 0:
 
-    o, lse = tree_attn(q, cache, block_table, seqlens, softmax_scale=scale, return_lse=True)
-    attn_weight_sums(q, cache, block_table, seqlens, lse, softmax_scale=scale, sums=sums)
-    ...
-    keep, lens = evict(cache, block_table, seqlens, sums, budget, n_first=4, n_recent=256)
+    base = pc.seqlens.clone()
+    slots = pc.append(seqs, [s] * len(seqs))  # kv_build writes the drafted rows there
+    mask = tree_mask(parents)
+    o, lse = tree_attn(q, pc.cache, pc.block_table, pc.seqlens, mask, softmax_scale=scale,
+                       return_lse=True)
+    # the lengths, rows and nodes that lse belongs to: before the step's end
+    attn_weight_sums(q, pc.cache, pc.block_table, pc.seqlens, lse, mask, softmax_scale=scale,
+                     sums=sums)
+    # a path of each tree is accepted; its rows and their sums move up
+    commit(pc.cache, pc.block_table, base, path, accepted, seqlens=pc.seqlens, sums=sums)
+    pc.truncate(seqs, lengths)
+    # sequences over the budget come down to it
+    keep, lens = evict(pc.cache, pc.block_table, pc.seqlens, sums, budget, n_first=first,
+                       n_recent=recent)
+    pc.truncate(seqs, [int(lens[i]) for i in seqs])
 
 The latent row of a token is shared by all heads, so one choice is made per
 sequence.  Rows keep the rotation of the position they were written at: a
@@ -32,8 +45,9 @@ def attn_weight_sums(q: torch.Tensor, cache: torch.Tensor, block_table: torch.Te
     over the step's query tokens and heads.
 
     q, cache, block_table, seqlens, mask, tree_lens, max_seqlen as tree_attn
-    takes them, lse [b, s, h] fp32 as it returned them (q [b, 1, h, d] and no
-    mask: a decode step).  Returns sums [b, max_seqlen] fp32, 0 where no query
+    took them, lse [b, s, h] fp32 as it returned them (q [b, 1, h, d] and no
+    mask: a decode step): the call belongs between the attention and the step's
+    end, whose commit moves the rows and changes the lengths.  Returns sums [b, max_seqlen] fp32, 0 where no query
     sees; with `sums` given ([b, at least max_seqlen], rows may be strided) the
     weights are added to it instead, at positions below seqlens, and it is
     returned.  The same inputs give the same bits.

@@ -11,6 +11,9 @@ behind the sequence:
     ...                                             # accept a path per sequence
     commit(cache, block_table, base_lens, path, accepted, seqlens=seqlens)
 
+(On a cache that is bounded by its attention weights, qcau_b200.evict shows where
+their sums come in between.)
+
 The reference has no speculative decoding; the attention is its sparse_attn
 (Deepseek_origin/inference/kernel.py:276-352) with every cached token in place
 of the index list and the tree in place of causality.
