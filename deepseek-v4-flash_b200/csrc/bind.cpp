@@ -16,7 +16,6 @@
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 
-#include <algorithm>
 #include <string>
 
 #include "qcau_b200.h"
@@ -267,7 +266,7 @@ PyObject* attn_weight_sums(PyObject*, PyObject* const* a, Py_ssize_t n) {
 
 // ---------------------------------------------------------------- selection and moves
 
-// Selection of sequences `b`; the outputs are allocated by select_run.
+// Selection of sequences `b`; select_outputs allocates the outputs.
 qcau_select_args check_select(const char* what, int index, const Tensor& sums, const Tensor& seqlens, int64_t b,
                               const Tensor* sums_out) {
   qcau_select_args s{};
@@ -288,13 +287,13 @@ qcau_select_args check_select(const char* what, int index, const Tensor& sums, c
   return s;
 }
 
-void select_run(int index, qcau_select_args& s, const Tensor& seqlens, Tensor& keep, Tensor& counts) {
+// The outputs of a selection.
+void select_outputs(qcau_select_args& s, const Tensor& seqlens, Tensor& keep, Tensor& counts) {
   TORCH_CHECK_VALUE(s.budget >= 1, "evict_select: the budget must be at least 1");
   keep = at::empty({s.b, s.budget}, seqlens.options());
   counts = at::empty_like(seqlens);
   s.keep = data<int32_t>(&keep);
   s.counts = data<int32_t>(&counts);
-  run(index, "evict_select", [&](cudaStream_t st) { return qcau_evict_select(&s, st); });
 }
 
 // Where rows come from and go to.
@@ -340,7 +339,8 @@ PyObject* select_rows(PyObject*, PyObject* const* a, Py_ssize_t n) {
   s.n_first = int_arg(a[3], "n_first");
   s.n_recent = int_arg(a[4], "n_recent");
   Tensor keep, counts;
-  select_run(index, s, *seqlens, keep, counts);
+  select_outputs(s, *seqlens, keep, counts);
+  run(index, "evict_select", [&](cudaStream_t st) { return qcau_evict_select(&s, st); });
   return pair(std::move(keep), std::move(counts));
   END_HANDLE_TH_ERRORS
 }
@@ -352,22 +352,16 @@ PyObject* evict(PyObject*, PyObject* const* a, Py_ssize_t n) {
   const Tensor *seqlens = tensor_arg(a[2], "seqlens"), *sums = tensor_arg(a[3], "sums");
   const Tensor* sums_out = tensor_arg(a[9], "sums_out", true);
   const int index = cuda_index(*cache);
-  // every refusal comes before the sums are touched
   qcau_keep_args k = check_move("evict", index, *cache, *table, tensor_arg(a[7], "dst_cache", true),
                                 tensor_arg(a[8], "dst_table", true));
   qcau_select_args s = check_select("evict", index, *sums, *seqlens, k.b, sums_out ? sums_out : sums);
   s.budget = int_arg(a[4], "budget");
   s.n_first = int_arg(a[5], "n_first");
   s.n_recent = int_arg(a[6], "n_recent");
-  TORCH_CHECK_VALUE(s.max_seqlen <= k.max_pages * k.page_size &&
-                        std::min(s.budget, s.max_seqlen) <= k.dst_max_pages * k.page_size,
-                    "evict: a block table does not hold the positions of sums, or the budget");
   Tensor keep, counts;
-  select_run(index, s, *seqlens, keep, counts);
-  k.keep = s.keep;
-  k.counts = s.counts;
-  k.keep_stride = k.k = s.budget;
-  run(index, "keep_rows", [&](cudaStream_t st) { return qcau_keep_rows(&k, st); });
+  select_outputs(s, *seqlens, keep, counts);
+  // (refuses before the selection is launched, which changes the sums)
+  run(index, "evict", [&](cudaStream_t st) { return qcau_evict(&s, &k, st); });
   return pair(std::move(keep), std::move(counts));
   END_HANDLE_TH_ERRORS
 }

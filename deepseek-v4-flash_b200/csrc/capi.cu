@@ -1525,6 +1525,19 @@ TreeArgs tree_args(const qcau_tree_args& t) {
   return a;
 }
 
+int check_select(const qcau_select_args& t) {
+  QCAU_CHECK_ARG(t.b == 0 || (t.sums && t.seqlens && t.keep && t.counts), "evict_select: NULL pointer");
+  QCAU_CHECK_ARG(t.b >= 0 && t.max_seqlen >= 1 && t.budget >= 1, "evict_select: bad shape");
+  QCAU_CHECK_ARG(t.n_first >= 0 && t.n_recent >= 0 && t.n_first <= t.budget &&
+                     t.n_recent <= t.budget - t.n_first,
+                 "evict_select: the budget must hold n_first and n_recent tokens");
+  QCAU_CHECK_ARG(t.sums_stride >= t.max_seqlen && (t.sums_out == nullptr || t.out_stride >= t.max_seqlen),
+                 "evict_select: a row of sums must hold max_seqlen values");
+  if (t.b >= (1LL << 27) || t.max_seqlen >= (1LL << 30) || t.budget >= (1LL << 31) - 65536)
+    return fail(QCAU_ERR_UNSUPPORTED, "evict_select: batch too large for one call");
+  return QCAU_OK;
+}
+
 int check_keep(const qcau_keep_args& t) {
   QCAU_CHECK_ARG(t.b == 0 || (t.cache && t.block_table && t.dst_cache && t.dst_table && t.keep && t.counts),
                  "keep_rows: NULL pointer");
@@ -1622,17 +1635,32 @@ int qcau_attn_weight_sums(const qcau_tree_args* args, void* stream) {
 int qcau_evict_select(const qcau_select_args* args, void* stream) {
   QCAU_CHECK_ARG(args != nullptr, "evict_select: NULL arguments");
   const qcau_select_args& t = *args;
-  QCAU_CHECK_ARG(t.b == 0 || (t.sums && t.seqlens && t.keep && t.counts), "evict_select: NULL pointer");
-  QCAU_CHECK_ARG(t.b >= 0 && t.max_seqlen >= 1 && t.budget >= 1, "evict_select: bad shape");
-  QCAU_CHECK_ARG(t.n_first >= 0 && t.n_recent >= 0 && t.n_first <= t.budget &&
-                     t.n_recent <= t.budget - t.n_first,
-                 "evict_select: the budget must hold n_first and n_recent tokens");
-  QCAU_CHECK_ARG(t.sums_stride >= t.max_seqlen && (t.sums_out == nullptr || t.out_stride >= t.max_seqlen),
-                 "evict_select: a row of sums must hold max_seqlen values");
-  if (t.b >= (1LL << 27) || t.max_seqlen >= (1LL << 30) || t.budget >= (1LL << 31) - 65536)
-    return fail(QCAU_ERR_UNSUPPORTED, "evict_select: batch too large for one call");
+  const int rc = check_select(t);
+  if (rc) return rc;
   if (t.b == 0) return QCAU_OK;
   QCAU_CHECK_CUDA(launch_evict_select(t, to_stream(stream)));
+  return QCAU_OK;
+}
+
+int qcau_evict(const qcau_select_args* select, const qcau_keep_args* rows, void* stream) {
+  QCAU_CHECK_ARG(select != nullptr && rows != nullptr, "evict: NULL arguments");
+  const qcau_select_args& s = *select;
+  qcau_keep_args k = *rows;
+  k.keep = s.keep;
+  k.counts = s.counts;
+  k.start = nullptr;
+  k.b = s.b;
+  k.keep_stride = k.k = s.budget;
+  // all refusals first: the selection already changes the sums
+  int rc = check_select(s);
+  if (rc == QCAU_OK) rc = check_keep(k);
+  if (rc) return rc;
+  QCAU_CHECK_ARG(s.max_seqlen <= k.max_pages * k.page_size &&
+                     std::min(s.budget, s.max_seqlen) <= k.dst_max_pages * k.page_size,
+                 "evict: a block table does not hold the positions of sums, or the budget");
+  if (s.b == 0) return QCAU_OK;
+  QCAU_CHECK_CUDA(launch_evict_select(s, to_stream(stream)));
+  QCAU_CHECK_CUDA(launch_keep_rows(k, to_stream(stream)));
   return QCAU_OK;
 }
 

@@ -155,6 +155,7 @@ SIGNATURES = {
     "qcau_attn_weight_sums_workspace_size": ([_I64, _I64, _I64, _I64], _SZ),
     "qcau_attn_weight_sums": ([ctypes.POINTER(TreeArgs), _P], ctypes.c_int),
     "qcau_evict_select": ([ctypes.POINTER(SelectArgs), _P], ctypes.c_int),
+    "qcau_evict": ([ctypes.POINTER(SelectArgs), ctypes.POINTER(KeepArgs), _P], ctypes.c_int),
     "qcau_keep_rows": ([ctypes.POINTER(KeepArgs), _P], ctypes.c_int),
     "qcau_keep_rows_sums": ([ctypes.POINTER(KeepArgs), _P, _I64, _I64, _P], ctypes.c_int),
 }

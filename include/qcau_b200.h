@@ -626,6 +626,10 @@ int qcau_wait_flags(const uint32_t* flags, int64_t n, uint32_t epoch, void* stre
  *   [b]; among equal sums the lower position is kept; NaN ranks above every
  *   number.  sums_out (or NULL; may be sums, with the same stride) gets the
  *   kept sums in that order and 0 in the rest of [0, max_seqlen).
+ * evict: evict_select, then keep_rows of what it kept (rows' keep, counts,
+ *   start, keep_stride, b and k are not read).  A call that either refuses
+ *   changes nothing, and so does one whose block tables do not hold max_seqlen
+ *   positions, or the budget.
  * keep_rows: row start[i] + j of sequence i in dst_cache := its row start[i] +
  *   keep[i][j] in cache, j < counts[i] <= k (start NULL: 0).  keep is strictly
  *   ascending; keep [b, keep_stride].  dst_cache / dst_table may be cache /
@@ -691,6 +695,7 @@ size_t qcau_attn_weight_sums_workspace_size(int64_t b, int64_t s, int64_t h,
                                             int64_t max_seqlen);
 int qcau_attn_weight_sums(const qcau_tree_args* args, void* stream);
 int qcau_evict_select(const qcau_select_args* args, void* stream);
+int qcau_evict(const qcau_select_args* select, const qcau_keep_args* rows, void* stream);
 int qcau_keep_rows(const qcau_keep_args* args, void* stream);
 int qcau_keep_rows_sums(const qcau_keep_args* args, float* sums, int64_t sums_stride,
                         int64_t positions, void* stream);

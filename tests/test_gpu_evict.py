@@ -473,3 +473,27 @@ def test_calls_in_a_row_see_what_ran_before_them():
         for a, c in zip(got, slow[k]):
             assert torch.equal(a, c), k
     assert _lib.device_error() == 0
+
+
+def test_a_refused_eviction_changes_nothing():
+    """A cache view that is not 16-byte aligned, or whose pages are too many, is refused
+    before the sums are compacted in place."""
+    n = torch.full((1,), 128, dtype=torch.int32, device="cuda")
+    table = torch.tensor([[0, 1]], dtype=torch.int32, device="cuda")
+    flat = torch.randn(2 * 64 * 64 + 8, device="cuda").to(torch.bfloat16)
+    odd, even = flat[1:1 + 2 * 64 * 64].view(2, 64, 64), flat[:2 * 64 * 64].view(2, 64, 64)
+    sums = torch.rand(1, 128, device="cuda")
+    rows_before, sums_before = flat.clone(), sums.clone()
+    for cache, dst in ((odd, None), (even, odd)):
+        with pytest.raises(ValueError, match="aligned"):
+            evict(cache, table, n, sums, 20, dst_cache=dst)
+    many = 65536
+    with pytest.raises(NotImplementedError, match="too large"):
+        all_sums = sums.expand(many, 128).contiguous()
+        evict(even, table.expand(many, 2).contiguous(), n.expand(many).contiguous(), all_sums, 20)
+    torch.cuda.synchronize()
+    assert torch.equal(all_sums, sums_before.expand(many, 128))
+    assert torch.equal(sums, sums_before) and torch.equal(flat, rows_before)
+    evict(even, table, n, sums, 20)
+    assert not torch.equal(sums, sums_before)
+    assert _lib.device_error() == 0

@@ -211,3 +211,28 @@ def test_keep_rows_sums_refusals():
                               (dict(b=70000), NotImplementedError, "too large")):
         _expect(call(**change), exc, text)
     assert call(b=0) == 0
+
+
+@no_device
+def test_evict_refuses_before_anything_is_launched():
+    """What the move of the rows refuses is refused before the selection runs: it
+    changes the sums.  (A launch without a device would be another error.)"""
+    L = _lib.lib()
+    select = dict(sums=P[0], seqlens=P[1], keep=P[2], counts=P[3], out=P[0], stride=100, out_stride=100, b=1, n=100, budget=10,
+                  first=2, recent=3)
+    rows = dict(cache=P[4], table=P[5], dst=P[4], dst_table=P[5], keep=0, counts=0, start=0, lens=0, max_pages=4,
+                num_pages=8, dst_max_pages=4, dst_num_pages=8, keep_stride=0, b=0, k=0, d=576, page=64)
+
+    def call(s={}, r={}):
+        return L.qcau_evict(_lib.SelectArgs(*{**select, **s}.values()), _lib.KeepArgs(*{**rows, **r}.values()), None)
+
+    _expect(L.qcau_evict(None, None, None), ValueError, "NULL")
+    for s, r, exc, text in ((dict(budget=0), {}, ValueError, "bad shape"), (dict(first=9), {}, ValueError, "budget"),
+                            ({}, dict(cache=P[4] + 2), ValueError, "aligned"), ({}, dict(dst=P[4] + 8), ValueError, "aligned"),
+                            ({}, dict(d=24), ValueError, "multiple of 16"), ({}, dict(table=0), ValueError, "NULL"),
+                            (dict(b=70000), {}, NotImplementedError, "too large"),
+                            ({}, dict(num_pages=1 << 26), NotImplementedError, "too large"),
+                            (dict(n=257, stride=257, out_stride=257), {}, ValueError, "does not hold"),
+                            (dict(budget=80), dict(dst_max_pages=1), ValueError, "does not hold")):
+        _expect(call(s, r), exc, text)
+    assert call(dict(b=0)) == 0
