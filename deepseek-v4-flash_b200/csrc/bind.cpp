@@ -279,8 +279,7 @@ qcau_select_args check_select(const char* what, int index, const Tensor& sums, c
   s.max_seqlen = in.n;
   if (sums_out) {
     const Sums out = check_sums(what, *sums_out, index, b);
-    TORCH_CHECK_VALUE(out.n == in.n && (sums_out->data_ptr() != sums.data_ptr() || out.stride == in.stride), what,
-                      ": sums_out must have the shape of sums, and be sums or other memory");
+    TORCH_CHECK_VALUE(out.n == in.n, what, ": sums_out must have the shape of sums");
     s.sums_out = data<float>(sums_out);
     s.out_stride = out.stride;
   }

@@ -1500,6 +1500,21 @@ bool overlap(const void* x, int64_t x_bytes, const void* y, int64_t y_bytes) {
   return a < b + (uintptr_t)y_bytes && b < a + (uintptr_t)x_bytes;
 }
 
+// Whether rows of n values at x (every x_stride) and at y (every y_stride), b of each,
+// share a value.  Rows of two views of one wider buffer lie between one another: exact
+// where the strides are equal, by their extents where they differ.
+bool rows_overlap(const float* x, int64_t x_stride, const float* y, int64_t y_stride, int64_t b, int64_t n) {
+  const auto extent = [&](int64_t stride) { return ((b - 1) * stride + n) * (int64_t)sizeof(float); };
+  if (b < 1 || !overlap(x, extent(x_stride), y, extent(y_stride))) return false;
+  const int64_t off = (int64_t)(reinterpret_cast<uintptr_t>(y) - reinterpret_cast<uintptr_t>(x));
+  const int64_t step = x_stride * (int64_t)sizeof(float), row = n * (int64_t)sizeof(float);
+  if (x_stride != y_stride) return true;
+  // row i of y against row i + m of x: the two m around off / step, within the batch
+  for (int64_t m = off / step - 1; m <= off / step + 1; m++)
+    if (m > -b && m < b && off - m * step < row && m * step - off < row) return true;
+  return false;
+}
+
 // The TreeArgs whose sizes decide the workspaces.
 TreeArgs tree_sizes(int64_t b, int64_t s, int64_t h, int64_t max_seqlen) {
   TreeArgs a{};
@@ -1533,8 +1548,14 @@ int check_select(const qcau_select_args& t) {
                  "evict_select: the budget must hold n_first and n_recent tokens");
   QCAU_CHECK_ARG(t.sums_stride >= t.max_seqlen && (t.sums_out == nullptr || t.out_stride >= t.max_seqlen),
                  "evict_select: a row of sums must hold max_seqlen values");
-  if (t.b >= (1LL << 27) || t.max_seqlen >= (1LL << 30) || t.budget >= (1LL << 31) - 65536)
+  if (t.b >= (1LL << 27) || t.max_seqlen >= (1LL << 30) || t.budget >= (1LL << 31) - 65536 ||
+      t.sums_stride >= (1LL << 34) || t.out_stride >= (1LL << 34))
     return fail(QCAU_ERR_UNSUPPORTED, "evict_select: batch too large for one call");
+  // a sequence's block writes its row of sums_out when it has read its own row of sums alone
+  const bool same = t.sums_out == t.sums && t.out_stride == t.sums_stride;
+  QCAU_CHECK_ARG(t.sums_out == nullptr || same ||
+                     !rows_overlap(t.sums, t.sums_stride, t.sums_out, t.out_stride, t.b, t.max_seqlen),
+                 "evict_select: sums_out may be sums, with its stride, but not overlap it otherwise");
   return QCAU_OK;
 }
 

@@ -64,8 +64,9 @@ def select_rows(sums: torch.Tensor, seqlens: torch.Tensor, budget: int, *, n_fir
     Of the first seqlens[i] positions of sums [b, positions] fp32, the first
     n_first, the last n_recent and those of the largest sums, min(seqlens[i],
     budget) in all, ascending, -1 past the count.  Among equal sums the lower
-    position stays; NaN ranks above every number.  sums_out (may be sums itself)
-    gets the kept sums in the new order and 0 behind them.
+    position stays; NaN ranks above every number.  sums_out (sums
+    itself, or other memory) gets the kept sums in the new order and 0 behind
+    them.
     """
     return bind().select_rows(sums, seqlens, budget, n_first, n_recent, sums_out)
 

@@ -624,8 +624,8 @@ int qcau_wait_flags(const uint32_t* flags, int64_t n, uint32_t epoch, void* stre
  *   and those of the largest sums, count = min(seqlens[i], budget) in all, as
  *   ascending positions keep [b, budget] int32 (-1 past the count) and counts
  *   [b]; among equal sums the lower position is kept; NaN ranks above every
- *   number.  sums_out (or NULL; may be sums, with the same stride) gets the
- *   kept sums in that order and 0 in the rest of [0, max_seqlen).
+ *   number.  sums_out (or NULL; may be sums, with the same stride, and
+ *   otherwise may not overlap it) gets the kept sums in that order and 0 in the rest of [0, max_seqlen).
  * evict: evict_select, then keep_rows of what it kept (rows' keep, counts,
  *   start, keep_stride, b and k are not read).  A call that either refuses
  *   changes nothing, and so does one whose block tables do not hold max_seqlen

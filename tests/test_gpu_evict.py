@@ -497,3 +497,22 @@ def test_a_refused_eviction_changes_nothing():
     evict(even, table, n, sums, 20)
     assert not torch.equal(sums, sums_before)
     assert _lib.device_error() == 0
+
+
+def test_sums_out_over_part_of_the_sums():
+    """Views shifted against one another are refused and nothing is touched; the two
+    halves of one buffer's rows are other memory."""
+    buf = torch.rand(5, 200, device="cuda")
+    before = buf.clone()
+    n = torch.tensor([100, 90, 100], dtype=torch.int32, device="cuda")
+    flat = buf.view(-1)
+    for out in (buf[1:4, :100], buf[:3, 50:150], flat[1:601].view(3, 200)[:, :100], flat[:300].view(3, 100)):
+        with pytest.raises(ValueError, match="overlap"):
+            select_rows(buf[:3, :100], n, 20, sums_out=out)
+    torch.cuda.synchronize()
+    assert torch.equal(buf, before)
+    keep, _ = select_rows(buf[:3, :100], n, 20, sums_out=buf[:3, 100:])
+    assert torch.equal(keep.cpu(), plain_select(before, [100, 90, 100], 20, 0, 0))
+    assert torch.equal(buf[:3, 100:120], before[:3].gather(1, keep.long()))
+    assert torch.equal(buf[:3, :100], before[:3, :100]) and buf[:3, 120:].eq(0).all()
+    assert _lib.device_error() == 0

@@ -236,3 +236,35 @@ def test_evict_refuses_before_anything_is_launched():
                             (dict(budget=80), dict(dst_max_pages=1), ValueError, "does not hold")):
         _expect(call(s, r), exc, text)
     assert call(dict(b=0)) == 0
+
+
+def _rows(start, stride, b, n):
+    return {start + i * stride + j for i in range(b) for j in range(n)}
+
+
+@no_device
+def test_sums_out_that_overlaps_sums_is_refused():
+    """A block of one sequence would write what another's has not read.  Rows between the
+    other's rows share nothing; every offset of both is tried against the set of places."""
+    L = _lib.lib()
+
+    def refused(off, stride, out_stride, b, n):
+        at = P[0] + (1 << 14)
+        # (a misaligned cache: what passes the overlap check must not launch)
+        args = dict(sums=at, seqlens=P[1], keep=P[2], counts=P[3], out=at + 4 * off, stride=stride, out_stride=out_stride, b=b,
+                    n=n, budget=1, first=0, recent=0)
+        cache = dict(cache=P[4] + 2, table=P[5], dst=P[4], dst_table=P[5], keep=0, counts=0, start=0, lens=0, max_pages=4,
+                     num_pages=8, dst_max_pages=4, dst_num_pages=8, keep_stride=0, b=0, k=0, d=576, page=64)
+        rc = L.qcau_evict(_lib.SelectArgs(*args.values()), _lib.KeepArgs(*cache.values()), None)
+        with pytest.raises(ValueError) as e:
+            _lib.check(rc, "call")
+        assert "overlap" in str(e.value) or "aligned" in str(e.value)
+        return "overlap" in str(e.value)
+
+    for stride, b, n in ((10, 1, 10), (10, 3, 10), (20, 3, 10), (21, 3, 10), (17, 4, 10), (40, 2, 7)):
+        for off in range(-4 * stride - 3, 4 * stride + 4):
+            want = off != 0 and bool(_rows(0, stride, b, n) & _rows(off, stride, b, n))
+            assert refused(off, stride, stride, b, n) == want, (off, stride, b, n)
+    # other strides: by the extents, and the same pointer too
+    for off, want in ((0, True), (5, True), (29, True), (30, False), (-34, False), (-33, True)):
+        assert refused(off, 10, 12, 3, 10) is want, off
