@@ -1624,6 +1624,8 @@ int qcau_tree_attn(const qcau_tree_args* args, void* stream) {
   rc = check_tree_ws(attn_tree_workspace(a), t, "tree_attn");
   if (rc) return rc;
   if (t.b == 0) return QCAU_OK;
+  QCAU_CHECK_ARG(!overlap(t.cache, t.num_pages * t.page_size * t.d_qk * 2, t.o, t.b * t.s * t.h * 1024),
+                 "tree_attn: o must not overlap the cache");
   QCAU_CHECK_CUDA(launch_attn_tree_sm100(a, t.workspace, to_stream(stream)));
   return QCAU_OK;
 }

@@ -61,7 +61,8 @@ def tree_attn(q: torch.Tensor, cache: torch.Tensor, block_table: torch.Tensor,
     before the tree and to node j when mask[i, t, j]; mask is bool [b, s, s],
     or [s, s] for all sequences, or None for a chain (j <= t).  attn_sink [h].
 
-    Returns o [b, s, h, 512] bf16 (written to `out` when given), and with
+    Returns o [b, s, h, 512] bf16 (written to `out` when given, other
+    memory than q and the cache), and with
     return_lse the log-sum-exps [b, s, h] fp32 that attn_weight_sums takes.
     Nodes past tree_lens[i] get zeros and -inf.  max_seqlen bounds seqlens
     (None: what the block table holds) and sizes the launch.

@@ -610,7 +610,7 @@ int qcau_wait_flags(const uint32_t* flags, int64_t n, uint32_t epoch, void* stre
  *   raises QCAU_DEVERR_INDEX and ends the chain.
  * tree_attn: q [b, s, h, d_qk], o [b, s, h, 512] bf16, lse [b, s, h] fp32 or
  *   NULL: the natural logarithm of the softmax denominator, the sink's term
- *   (attn_sink [h] fp32 or NULL) included.  Any h and s; o may not overlap q.  Rows that see
+ *   (attn_sink [h] fp32 or NULL) included.  Any h and s; o may not overlap q or the cache.  Rows that see
  *   nothing get o = 0 and lse = the sink's value (-inf without one); rows of
  *   nodes t >= n get o = 0 and lse = -inf.  P is rounded to bf16 before P.V
  *   as in sparse_attn.

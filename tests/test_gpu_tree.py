@@ -579,3 +579,12 @@ def test_commit_refuses_other_sums():
             commit(cache, table, one, path, one, sums=sums)
     with pytest.raises(TypeError):
         commit(cache, table, one, path, one, sums=3)
+
+
+def test_output_over_the_cache_is_refused():
+    x = build(dict(lens=[200], nodes=[4], s=4, h=16, d=512))
+    before = x["cache"].clone()
+    with pytest.raises(ValueError, match="overlap the cache"):
+        tree_attn(x["q"], x["cache"], x["table"], x["seqlens"], softmax_scale=SCALE, out=x["cache"].view(-1)[:4 * 16 * 512].view(1, 4, 16, 512))
+    torch.cuda.synchronize()
+    assert torch.equal(x["cache"].view(torch.int16), before.view(torch.int16))

@@ -268,3 +268,13 @@ def test_sums_out_that_overlaps_sums_is_refused():
     # other strides: by the extents, and the same pointer too
     for off, want in ((0, True), (5, True), (29, True), (30, False), (-34, False), (-33, True)):
         assert refused(off, 10, 12, 3, 10) is want, off
+
+
+@no_device
+def test_output_over_the_cache_is_refused():
+    L = _lib.lib()
+    step = dict(q=P[0], cache=P[1], table=P[2], seqlens=P[3], nodes=0, mask=0, sink=0, o=P[1], lse=0, sums=0, ws=P[5],
+                stride=0, b=1, s=1, h=2, d=512, dv=512, page=64, max_pages=1, num_pages=1, most=64, sums_stride=0,
+                ws_bytes=1 << 30, scale=0.07, accumulate=0)
+    for o in (P[1], P[1] + 65536 - 16, P[1] - 2032):
+        _expect(L.qcau_tree_attn(_lib.TreeArgs(*{**step, "o": o}.values()), None), ValueError, "overlap the cache")
