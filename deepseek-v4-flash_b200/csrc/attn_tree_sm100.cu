@@ -95,7 +95,7 @@ struct TreeParams {
   float* lse;          // [b, s, h] or nullptr
   const float* sink;   // [h] or nullptr
   int chunks;          // 64-value chunks of a row: 9 or 8
-  float scale;
+  float score_scale;   // log2 units
   float* part_o;   // [pairs][2][128][512]
   float* part_ml;  // [pairs][2][128][2]: max (log2 units), sum
   int4* desc;      // [pairs]: the row whose pieces start at this pair {b or -1, group, rows of
@@ -395,7 +395,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     const int hl = row & 63, half = row >> 6;
     const int et = threadIdx.x - 64;      // 0..127 over warps 2-5
     const uint32_t lane_base = (uint32_t)(quarter * 32) << 16;
-    const float sl2 = p.scale * kLog2e * (1.f + 36 * kTruncPerStep);
+    const float sl2 = p.score_scale;
     const uint32_t s_free_l[2] = {mapa_shared(smem_u32(&sh->s_free[0]), 0),
                                   mapa_shared(smem_u32(&sh->s_free[1]), 0)};
     const uint32_t p_full_l = mapa_shared(smem_u32(&sh->p_full), 0);
@@ -946,7 +946,7 @@ cudaError_t launch_attn_tree_sm100(const TreeArgs& a, void* ws, cudaStream_t st)
   p.lse = a.lse;
   p.sink = a.sink;
   p.chunks = (int)(a.d_qk / 64);
-  p.scale = a.scale;
+  p.score_scale = tree_score_scale(a.scale, 1.4426950408889634, a.d_qk, (int)(a.d_qk / 16));  // one chain
   p.part_o = reinterpret_cast<float*>(ws);
   p.part_ml = p.part_o + (size_t)pairs * 2 * 128 * 512;
   p.desc = reinterpret_cast<int4*>(p.part_ml + (size_t)pairs * 2 * 128 * 2);

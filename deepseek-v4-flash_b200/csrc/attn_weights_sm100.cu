@@ -91,7 +91,7 @@ struct WeightsParams {
   float* part;       // [groups][b][part_stride] when groups > 1
   int64_t sums_stride, part_stride;
   int accumulate, chunks;
-  float scale;
+  float score_scale;  // log2 units
 };
 
 template <int N>
@@ -245,7 +245,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     const int hl = kSplit ? row & 63 : row, half = kSplit ? row >> 6 : 0;
     const int et = threadIdx.x - 64;
     const uint32_t lane_base = (uint32_t)(quarter * 32) << 16;
-    const float sl2 = p.scale * kLog2e * (1.f + C::kSteps * kTruncPerStep);
+    const float sl2 = p.score_scale;
     const uint32_t s_free_l[2] = {mapa_shared(smem_u32(&sh->s_free[0]), 0),
                                   mapa_shared(smem_u32(&sh->s_free[1]), 0)};
     const int64_t seq_rows = (int64_t)p.sh.s * p.sh.h;
@@ -474,7 +474,11 @@ cudaError_t launch_attn_weights_sm100(const TreeArgs& a, void* ws, cudaStream_t 
   p.part_stride = (a.max_len + 3) / 4 * 4;
   p.accumulate = a.accumulate;
   p.chunks = (int)(a.d_qk / 64);
-  p.scale = a.scale;
+  // (log2(e) as the kernel has it for the log-sum-exps: its rounding leaves the difference)
+  p.score_scale = tree_score_scale(a.scale, kLog2e, a.d_qk,
+                                   n == 256   ? WeightsCfg<256>::kSteps
+                                   : n == 128 ? WeightsCfg<128>::kSteps
+                                              : WeightsCfg<64>::kSteps);
   cudaError_t e = n == 256   ? run_weights<256>(a, p, tq, tk, pairs, st)
                   : n == 128 ? run_weights<128>(a, p, tq, tk, pairs, st)
                              : run_weights<64>(a, p, tq, tk, pairs, st);

@@ -23,12 +23,25 @@ constexpr int kTreePairs = 74;  // CTA pairs of a B200 (148 SMs)
 constexpr int kTreeRowCost = 2;
 
 // The tensor core truncates an accumulator to fp32 at every MMA step, towards
-// zero: scores come out short by a share that grows with the steps of their chain,
-// half an ulp of the running sum a step on average.  Measured (16384 tokens, rows
-// of standard deviations 1.7 and 4.3): 1.3e-7 of a score in chains of 9 steps,
-// 2.4e-7 in chains of 18, with about as much scatter.  The softmax scale takes the
-// mean back.
-constexpr float kTruncPerStep = 1.35e-8f;
+// zero: scores come out short by a share that grows with the steps of their chain.
+// Measured (slope of a score's error over the score, sequences of one token, 64 scales;
+// per step): queries independent of their token 0.95e-8 in chains of 9 steps, 1.1e-8 of
+// 18, 1.26e-8 of 32 and 36; queries that lean towards it, whose large scores carry a
+// softmax, 1.68e-8 in all of them.  The softmax scale takes a value between the two
+// back, which leaves a third or less.  It is a mean: a score whose partial sums cancel lost nothing in
+// proportion to itself, and is moved by it all the same (under 5e-7 of the score).
+constexpr double kTruncPerStep = 1.35e-8;
+
+// What a score q . k is multiplied by: softmax scale x log2(e), with the mean share back
+// that it lost in chains of `steps` MMAs of 16 dims (the last one shorter where d / 16 is
+// no multiple).  Of chains that a score is the sum of, each lost by its own steps of its
+// own share, steps over all steps: their mean is that of the squares.  In 64 bits,
+// rounded once: the shares are a few ulps of the scale.
+inline float tree_score_scale(float scale, double log2e, int64_t d_qk, int steps) {
+  const int64_t all = d_qk / 16, rest = all % steps;
+  const double mean = (double)(all / steps * steps * steps + rest * rest) / (double)all;
+  return (float)((double)scale * log2e * (1.0 + kTruncPerStep * mean));
+}
 
 struct TreeShape {
   const int32_t* table;      // [b, max_pages]
