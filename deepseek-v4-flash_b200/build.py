@@ -5,11 +5,13 @@ Python binding of its short calls (csrc/bind.cpp, against torch's headers) with 
 
 Objects go to deepseek-v4-flash_b200/_build/, the shared library to
 deepseek-v4-flash_b200/qcau_b200/libqcau_b200.so and _bind.so beside it.  A source
-is recompiled when it or any header under csrc/ or include/ is newer than its object.
+is recompiled when it or any header under csrc/ or include/ is newer than its object,
+the binding also when torch or Python are others than it was built for.
 """
 from __future__ import annotations
 
 import argparse
+import importlib.metadata
 import os
 import shutil
 import subprocess
@@ -24,6 +26,7 @@ CSRC = PKG_DIR / "csrc"
 BUILD = PKG_DIR / "_build"
 LIB = PKG_DIR / "qcau_b200" / "libqcau_b200.so"
 BIND = PKG_DIR / "qcau_b200" / "_bind.so"
+BIND_STAMP = BUILD / "bind.stamp"  # the torch and Python that BIND was built for
 SOURCES = ["capi.cu", "act_quant.cu", "rope_norm.cu", "fp8_gemm.cu", "bmm.cu",
            "attn_combine.cu", "attn_decode_sm100.cu", "attn_gather_sm100.cu", "kv_build.cu", "indexer.cu", "compress.cu",
            "indexer_score_sm100.cu", "attn_tree_sm100.cu", "attn_weights_sm100.cu", "evict.cu"]
@@ -77,10 +80,12 @@ def build(jobs: int = 8, verbose_ptxas: bool = False, force: bool = False) -> Pa
 
 
 def build_bind(force: bool = False) -> None:
-    """_bind.so: calls libqcau_b200.so (beside it) on torch tensors."""
+    """_bind.so: calls libqcau_b200.so (beside it) on torch tensors.  It holds for
+    one torch and one Python, which BIND_STAMP names."""
     src = CSRC / "bind.cpp"
-    if not force and BIND.exists() and BIND.stat().st_mtime >= max(src.stat().st_mtime,
-                                                                  _headers_mtime()):
+    stamp = f"torch {importlib.metadata.version('torch')}, {sysconfig.get_config_var('SOABI')}\n"
+    if (not force and BIND.exists() and BIND.stat().st_mtime >= max(src.stat().st_mtime, _headers_mtime())
+            and BIND_STAMP.exists() and BIND_STAMP.read_text() == stamp):
         return
     import torch
 
@@ -96,6 +101,8 @@ def build_bind(force: bool = False) -> None:
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:
         raise RuntimeError(f"binding failed:\n{r.stdout}\n{r.stderr}")
+    BIND_STAMP.parent.mkdir(parents=True, exist_ok=True)
+    BIND_STAMP.write_text(stamp)
 
 
 if __name__ == "__main__":
