@@ -6,12 +6,14 @@ Python binding of its short calls (csrc/bind.cpp, against torch's headers) with 
 Objects go to deepseek-v4-flash_b200/_build/, the shared library to
 deepseek-v4-flash_b200/qcau_b200/libqcau_b200.so and _bind.so beside it.  A source
 is recompiled when it or any header under csrc/ or include/ is newer than its object,
-the binding also when torch or Python are others than it was built for.
+the binding also when torch or Python are others than it was built for.  Without torch
+the library is built alone.
 """
 from __future__ import annotations
 
 import argparse
 import importlib.metadata
+import importlib.util
 import os
 import shutil
 import subprocess
@@ -83,6 +85,9 @@ def build_bind(force: bool = False) -> None:
     """_bind.so: calls libqcau_b200.so (beside it) on torch tensors.  It holds for
     one torch and one Python, which BIND_STAMP names."""
     src = CSRC / "bind.cpp"
+    if importlib.util.find_spec("torch") is None:
+        print("torch is not installed: the library is built without its Python binding", file=sys.stderr)
+        return
     stamp = f"torch {importlib.metadata.version('torch')}, {sysconfig.get_config_var('SOABI')}\n"
     if (not force and BIND.exists() and BIND.stat().st_mtime >= max(src.stat().st_mtime, _headers_mtime())
             and BIND_STAMP.exists() and BIND_STAMP.read_text() == stamp):

@@ -1,5 +1,5 @@
 """When the Python binding is built again: its torch and Python have to be those it was
-compiled against."""
+compiled against, and the C library alone needs neither."""
 import importlib.metadata
 import importlib.util
 import os
@@ -59,3 +59,9 @@ def test_binding_follows_its_source(compiler):
     os.utime(B.BIND, (1, 1))
     B.build_bind()
     assert len(compiler) == 2
+
+
+def test_library_alone_without_torch(compiler, monkeypatch, capsys):
+    monkeypatch.setattr(importlib.util, "find_spec", lambda name: None)
+    B.build_bind()
+    assert not compiler and "without its Python binding" in capsys.readouterr().err
