@@ -119,7 +119,7 @@ __device__ __forceinline__ void tree_norm(float m, float l, float sink, float& i
     return;
   }
   const float wm = m == -INFINITY ? 0.f : exp2f(m - top);
-  const float den = l * wm + exp2f(sk - top);
+  const float den = l * wm + (sk == top ? 1.f : exp2f(sk - top));  // (an infinite sink: 1)
   inv = den > 0.f || den != den ? wm / den : 0.f;
   lse = (top + log2f(den)) * kLn2;
 }

@@ -588,3 +588,22 @@ def test_output_over_the_cache_is_refused():
         tree_attn(x["q"], x["cache"], x["table"], x["seqlens"], softmax_scale=SCALE, out=x["cache"].view(-1)[:4 * 16 * 512].view(1, 4, 16, 512))
     torch.cuda.synchronize()
     assert torch.equal(x["cache"].view(torch.int16), before.view(torch.int16))
+
+
+@pytest.mark.parametrize("lens", [[60], [2500], [300] * 40])
+def test_infinite_sinks_take_all_the_weight(lens):
+    """A sink of +inf leaves its head zeros and lse = inf, one of -inf is none; the other
+    heads as they are (rows written whole, and merged from pieces)."""
+    x = build(dict(lens=lens, nodes=[5] * len(lens), s=5, h=16, mask="tree"))
+    args = (x["q"], x["cache"], x["table"], x["seqlens"], x["mask"])
+    sink = torch.linspace(-3, 3, 16, device="cuda")
+    o, lse = tree_attn(*args, softmax_scale=SCALE, attn_sink=sink, return_lse=True)
+    high, none, rest = [2, 9], [0, 15], [i for i in range(16) if i not in (0, 2, 9, 15)]
+    bare, bare_lse = tree_attn(*args, softmax_scale=SCALE, return_lse=True)
+    sink[high], sink[none] = math.inf, -math.inf
+    o2, lse2 = tree_attn(*args, softmax_scale=SCALE, attn_sink=sink, return_lse=True)
+    torch.cuda.synchronize()
+    assert torch.equal(o2[:, :, rest], o[:, :, rest]) and torch.equal(lse2[:, :, rest], lse[:, :, rest])
+    assert torch.equal(o2[:, :, none], bare[:, :, none]) and torch.equal(lse2[:, :, none], bare_lse[:, :, none])
+    assert o2[:, :, high].eq(0).all() and lse2[:, :, high].eq(math.inf).all()
+    assert _lib.device_error() == 0
