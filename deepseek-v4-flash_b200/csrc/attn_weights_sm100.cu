@@ -69,7 +69,8 @@ struct WeightsShared {
   uint64_t s_full[2], s_free[2];
   uint64_t xbar[2][4];  // M = 128: halves of a token's sum handed over: 2 warp pairs x 4 buffers
   float xsum[4][64];
-  float neg[4][WeightsCfg<N>::kCols];  // per epilogue warp: -lse * log2e of its columns
+  // per epilogue warp: -lse * log2e of its columns, read as 16-byte vectors
+  alignas(16) float neg[4][WeightsCfg<N>::kCols];
   uint32_t tmem_base;
   int abort;
   TreePlanShared plan;
