@@ -516,3 +516,17 @@ def test_sums_out_over_part_of_the_sums():
     assert torch.equal(buf[:3, 100:120], before[:3].gather(1, keep.long()))
     assert torch.equal(buf[:3, :100], before[:3, :100]) and buf[:3, 120:].eq(0).all()
     assert _lib.device_error() == 0
+
+
+@pytest.mark.parametrize("s,h,mask", [(1, 16, None), (5, 12, "tree"), (60, 1, "any"), (1, 128, None), (8, 16, "tree"), (25, 4, "any")])
+@pytest.mark.parametrize("d,page", [(512, 64), (512, 128), (576, 128), (512, 192)])
+def test_sums_of_both_widths_and_larger_pages(s, h, mask, d, page):
+    """Groups of 64 and 128 rows, whose tiles are two blocks a CTA: blocks of one page, of
+    two, and past the sequence's end; the last chain of a 512-wide row is shorter."""
+    x = build(dict(lens=[700, 257, 128, max(s, 65)], nodes=[s, s, s, s - s // 3], s=s, h=h, mask=mask, d=d, page=page))
+    lse = lse_of(x)
+    got = attn_weight_sums(x["q"], x["cache"], x["table"], x["seqlens"], lse, x["mask"], softmax_scale=SCALE,
+                           tree_lens=x["tree_lens"])
+    torch.cuda.synchronize()
+    check_sums(x, lse, got)
+    assert _lib.device_error() == 0

@@ -607,3 +607,32 @@ def test_infinite_sinks_take_all_the_weight(lens):
     assert torch.equal(o2[:, :, none], bare[:, :, none]) and torch.equal(lse2[:, :, none], bare_lse[:, :, none])
     assert o2[:, :, high].eq(0).all() and lse2[:, :, high].eq(math.inf).all()
     assert _lib.device_error() == 0
+
+
+def test_captured_behind_work_of_another_stream():
+    """A capture whose call depends on kernels of two streams, and is waited for by a third."""
+    x = build(dict(lens=[900, 700], nodes=[4, 4], s=4, h=16, mask="tree"), stale=0.0)
+    base, other = torch.cuda.Stream(), torch.cuda.Stream()
+    q, lens = x["q"].clone(), x["seqlens"].clone()
+    want = tree_attn(x["q"] * 2, x["cache"], x["table"], x["seqlens"] - 40, x["mask"], softmax_scale=SCALE)
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph, stream=base):
+        other.wait_stream(base)
+        q.copy_(x["q"] * 2)
+        with torch.cuda.stream(other):
+            lens.copy_(x["seqlens"] - 40)
+        base.wait_stream(other)
+        o = tree_attn(q, x["cache"], x["table"], lens, x["mask"], softmax_scale=SCALE)
+        other.wait_stream(base)
+        with torch.cuda.stream(other):
+            twice = o.float() * 2
+        base.wait_stream(other)
+    for _ in range(3):
+        q.zero_()
+        lens.fill_(4)
+        o.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(o, want) and torch.equal(twice, want.float() * 2)
+    assert _lib.device_error() == 0
