@@ -498,8 +498,9 @@ constexpr int kSumThreads = 1024;
 // keep[i] to place start + i, then 0 from the last kept one to the row's end.  In place:
 // keep is strictly ascending, so a chunk of i reads at or behind the places that it
 // writes, and the barrier between its loads and its stores is all that is needed.
-// Bound by latency at a drafting step's few nodes, then by one SM's stores of zeros
-// (4 bytes a position).
+// Bound by latency at a drafting step's few nodes (1 to 3 us on top of the rows' move,
+// sequences of up to 32768 positions), then by one SM's stores of zeros, 4 bytes a
+// position (9 us for one of 131072, 10 for 32 of them).
 __global__ void __launch_bounds__(kSumThreads)
     keep_sums_kernel(qcau_keep_args p, float* sums, int64_t stride, int64_t positions, int* err) {
   cudaGridDependencySynchronize();
