@@ -1552,7 +1552,7 @@ int check_select(const qcau_select_args& t) {
       t.sums_stride >= (1LL << 34) || t.out_stride >= (1LL << 34))
     return fail(QCAU_ERR_UNSUPPORTED, "evict_select: batch too large for one call");
   // a sequence's block writes its row of sums_out when it has read its own row of sums alone
-  const bool same = t.sums_out == t.sums && t.out_stride == t.sums_stride;
+  const bool same = t.sums_out == t.sums && (t.out_stride == t.sums_stride || t.b == 1);
   QCAU_CHECK_ARG(t.sums_out == nullptr || same ||
                      !rows_overlap(t.sums, t.sums_stride, t.sums_out, t.out_stride, t.b, t.max_seqlen),
                  "evict_select: sums_out may be sums, with its stride, but not overlap it otherwise");

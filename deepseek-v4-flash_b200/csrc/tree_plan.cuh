@@ -28,8 +28,9 @@ constexpr int kTreeRowCost = 2;
 // per step): queries independent of their token 0.95e-8 in chains of 9 steps, 1.1e-8 of
 // 18, 1.26e-8 of 32 and 36; queries that lean towards it, whose large scores carry a
 // softmax, 1.68e-8 in all of them.  The softmax scale takes a value between the two
-// back, which leaves a third or less.  It is a mean: a score whose partial sums cancel lost nothing in
-// proportion to itself, and is moved by it all the same (under 5e-7 of the score).
+// back, which leaves a third or less.  It is a mean: a score whose partial sums cancel
+// lost nothing in proportion to itself, and is moved by it all the same (under 5e-7 of
+// the score).
 constexpr double kTruncPerStep = 1.35e-8;
 
 // What a score q . k is multiplied by: softmax scale x log2(e), with the mean share back

@@ -610,8 +610,8 @@ int qcau_wait_flags(const uint32_t* flags, int64_t n, uint32_t epoch, void* stre
  *   raises QCAU_DEVERR_INDEX and ends the chain.
  * tree_attn: q [b, s, h, d_qk], o [b, s, h, 512] bf16, lse [b, s, h] fp32 or
  *   NULL: the natural logarithm of the softmax denominator, the sink's term
- *   (attn_sink [h] fp32 or NULL) included.  Any h and s; o may not overlap q or the cache.  Rows that see
- *   nothing get o = 0 and lse = the sink's value (-inf without one); rows of
+ *   (attn_sink [h] fp32 or NULL) included.  Any h and s; o may not overlap q or
+ *   the cache.  Rows that see nothing get o = 0 and lse = the sink's value (-inf without one); rows of
  *   nodes t >= n get o = 0 and lse = -inf.  P is rounded to bf16 before P.V
  *   as in sparse_attn.
  * attn_weight_sums: sums[i][p] (+)= sum over the query rows of sequence i
@@ -624,8 +624,9 @@ int qcau_wait_flags(const uint32_t* flags, int64_t n, uint32_t epoch, void* stre
  *   and those of the largest sums, count = min(seqlens[i], budget) in all, as
  *   ascending positions keep [b, budget] int32 (-1 past the count) and counts
  *   [b]; among equal sums the lower position is kept; NaN ranks above every
- *   number.  sums_out (or NULL; may be sums, with the same stride, and
- *   otherwise may not overlap it) gets the kept sums in that order and 0 in the rest of [0, max_seqlen).
+ *   number.  sums_out (or NULL; may be sums, with the same stride, and may not
+ *   overlap it otherwise) gets the kept sums in that order and 0 in the rest of
+ *   [0, max_seqlen).
  * evict: evict_select, then keep_rows of what it kept (rows' keep, counts,
  *   start, keep_stride, b and k are not read).  A call that either refuses
  *   changes nothing, and so does one whose block tables do not hold max_seqlen

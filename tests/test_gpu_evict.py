@@ -530,3 +530,15 @@ def test_sums_of_both_widths_and_larger_pages(s, h, mask, d, page):
     torch.cuda.synchronize()
     check_sums(x, lse, got)
     assert _lib.device_error() == 0
+
+
+def test_one_sequence_s_sums_in_place_whatever_the_stride():
+    """A view of one row has no stride to speak of: the same memory is the same sums."""
+    buf = torch.rand(1, 300, device="cuda")
+    one = buf[:, :100]                       # stride 300
+    same = torch.as_strided(buf, (1, 100), (100, 1))
+    before, n = one.clone(), torch.tensor([100], dtype=torch.int32, device="cuda")
+    keep, _ = select_rows(one, n, 20, sums_out=same)
+    assert torch.equal(keep.cpu(), plain_select(before, [100], 20, 0, 0))
+    assert torch.equal(buf[:, :20], before.gather(1, keep.long())) and buf[:, 20:100].eq(0).all()
+    assert _lib.device_error() == 0
