@@ -20,7 +20,7 @@ most recent ones and those of the largest sums stay.  A step with draft trees
     # sequences over the budget come down to it
     keep, lens = evict(pc.cache, pc.block_table, pc.seqlens, sums, budget, n_first=first,
                        n_recent=recent)
-    pc.truncate(seqs, [int(lens[i]) for i in seqs])
+    pc.truncate(range(len(lens)), lens.tolist())
 
 The latent row of a token is shared by all heads, so one choice is made per
 sequence.  Rows keep the rotation of the position they were written at: a

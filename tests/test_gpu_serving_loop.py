@@ -98,3 +98,33 @@ def test_documented_step_over_many_steps(s, h, budget):
             assert torch.equal(sums[i, :len(keep)].double().cpu(), at_evict[i][keep]) and sums[i, len(keep):].eq(0).all()
         assert pc.length(1) == 0 and sums[1].eq(0).all()
     assert evicted  # each case comes over its budget
+
+
+def test_sequences_that_do_not_draft_are_brought_down_too():
+    """A sequence with tokens and no nodes in this step: its weights, rows and length are
+    kept as they are until it is over the budget."""
+    d, h, s, budget = 576, 16, 3, 100
+    pc = Filled(num_pages=20, max_seqs=2, max_pages=5)
+    pc.rng = torch.Generator().manual_seed(5)
+    pc.append([0, 1], [80, 150])
+    rows = pc.fresh[80:]
+    sums = torch.rand(2, 320, device="cuda")
+    sums[0, 80:], sums[1, 150:] = 0, 0
+    before = sums[1].clone()
+    nodes = torch.tensor([s, 0], dtype=torch.int32, device="cuda")
+    lacking = dict(tree_lens=nodes)
+    names = dict(pc=pc, seqs=[0], s=s, parents=torch.tensor([[-1, 0, 0]] * 2, dtype=torch.int32, device="cuda"),
+                 q=torch.randn(2, s, h, d, generator=pc.rng).to(torch.bfloat16).cuda(), scale=SCALE, sums=sums,
+                 path=torch.tensor([[0, 2, -1]] * 2, dtype=torch.int32, device="cuda"),
+                 accepted=torch.tensor([2, 0], dtype=torch.int32, device="cuda"), lengths=[82], budget=budget, first=2, recent=9,
+                 tree_mask=tree_mask, tree_attn=lambda *a, **k: tree_attn(*a, **k, **lacking), commit=commit, evict=E.evict,
+                 attn_weight_sums=lambda *a, **k: E.attn_weight_sums(*a, **k, **lacking))
+    exec(documented_step(), names)
+    torch.cuda.synchronize()
+    key = before[:150].double().cpu()
+    key[:2], key[141:] = 1e30, 1e30
+    keep = torch.sort(torch.sort(key, descending=True, stable=True).indices[:budget]).values
+    assert pc.length(0) == 82 and pc.length(1) == budget and pc.seqlens.tolist() == [82, budget]
+    assert torch.equal(R.gather(pc.cache, pc.block_table, 1, budget).cpu(), rows[keep])
+    assert torch.equal(sums[1, :budget].cpu(), before.cpu()[keep]) and sums[1, budget:].eq(0).all()
+    assert _lib.device_error() == 0
